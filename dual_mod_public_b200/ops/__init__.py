@@ -23,4 +23,6 @@ def default_ops(device):
     return _cache[key]
 
 
-__all__ = ["TorchOps", "default_ops"]
+from .packed import TokenLogprobs, cached_attention, packed_attention, token_logprobs  # noqa: E402  (needs default_ops)
+
+__all__ = ["TorchOps", "default_ops", "packed_attention", "cached_attention", "token_logprobs", "TokenLogprobs"]

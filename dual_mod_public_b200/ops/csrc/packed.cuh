@@ -1,0 +1,166 @@
+// Helpers of the attention over packed sequences (packed_attn_fwd.cu, packed_attn_bwd.cu): which keys a row of the packed
+// axis sees, tile loads of [row, head, dim] tensors, and the tensor-memory operand forms of tcgen05.
+#pragma once
+#include <cuda_fp16.h>
+
+#include "tc05.cuh"
+
+namespace packed {
+
+using namespace tc05;
+
+constexpr int TILE = 128;               // rows of a query tile and of a key block
+constexpr float LOG2E = 1.4426950408889634f;
+
+// ---- sequences -------------------------------------------------------------------------------------------------------
+// `cu` holds n + 1 ascending row numbers; sequence s is the rows [cu[s], cu[s + 1]).  A row outside [cu[0], cu[n]) belongs
+// to no sequence.  The values live on the device and are not checked there: every result is clamped, so a wrong table
+// gives wrong outputs but no access out of range.
+
+// first index whose entry is greater than `row` (0 .. n + 1)
+__device__ __forceinline__ int upper_index(const int* __restrict__ cu, int n, int row) {
+  int a = 0, b = n + 1;
+  while (a < b) {
+    const int m = (a + b) >> 1;
+    if (__ldg(cu + m) > row) b = m; else a = m + 1;
+  }
+  return a;
+}
+// first key that query `row` sees (row + 1: none)
+__device__ __forceinline__ int first_key(const int* __restrict__ cu, int n, int window, int row) {
+  const int u = upper_index(cu, n, row);
+  if (u == 0 || u == n + 1) return row + 1;
+  int lo = min(row, max(0, __ldg(cu + u - 1)));
+  if (window > 0) lo = max(lo, row - window + 1);
+  return lo;
+}
+// last query that sees key `row` (row - 1: none)
+__device__ __forceinline__ int last_query(const int* __restrict__ cu, int n, int window, int rows, int row) {
+  const int u = upper_index(cu, n, row);
+  if (u == 0 || u == n + 1) return row - 1;
+  int hi = max(row, min(rows, __ldg(cu + u)) - 1);
+  if (window > 0) hi = (int)min((long long)hi, (long long)row + window - 1);
+  return hi;
+}
+
+// ---- waits ------------------------------------------------------------------------------------------------------------
+// One try before the clock is read: most waits of a running pipeline are over when they are asked for.
+__device__ __forceinline__ bool wait_quick(uint32_t bar, uint32_t parity, volatile int* err) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok ? true : mbar_wait(bar, parity, err);
+}
+// by a whole warp; the same answer in every lane
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatile int* err) {
+  return __all_sync(0xffffffffu, wait_quick(bar, parity, err));
+}
+
+// ---- element types ----------------------------------------------------------------------------------------------------
+template <typename T>
+struct Elem;
+template <>
+struct Elem<bf16> {
+  static constexpr uint32_t fmt = 1;
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16(lo, hi); }
+  static __device__ __forceinline__ float2 unpack(uint32_t u) { return unpack_bf16(u); }
+};
+template <>
+struct Elem<__half> {
+  static constexpr uint32_t fmt = 0;
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+  }
+  static __device__ __forceinline__ float2 unpack(uint32_t u) {
+    return __half22float2(*reinterpret_cast<__half2*>(&u));
+  }
+};
+// instruction descriptor of kind::f16, both operands of type T, fp32 accumulator (instr_desc of tc05.cuh is bf16 only)
+template <typename T>
+__host__ __device__ constexpr uint32_t mma_desc(int m, int n, int a_mn, int b_mn) {
+  return (1u << 4) | (Elem<T>::fmt << 7) | (Elem<T>::fmt << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
+         ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+
+// ---- tcgen05 ----------------------------------------------------------------------------------------------------------
+// D (+)= A B with A in tensor memory: 128 lanes, two 16-bit elements per 32-bit column, 8 columns per K step of 16
+__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "r"(tmem_a), "l"(db), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// this thread's TMEM lane, 32 consecutive 32-bit columns starting at `taddr`
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
+        "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]),
+        "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// A tile of 128 rows x DH dims lies in shared memory as DH / 64 slabs of 128 rows x 128 bytes (128-byte swizzle).  The same
+// tile serves as an operand whose reduction runs over the dims (K-major: 32 bytes per step of 16, 8-row groups 1024 bytes
+// apart) and as one whose reduction runs over the rows (MN-major: 2048 bytes per step of 16 rows, slabs 16 KB apart).
+constexpr uint32_t SLAB = TILE * 128;
+__device__ __forceinline__ uint64_t desc_dims(uint32_t tile, int k) {
+  return make_desc(tile + (k / 4) * SLAB + (k % 4) * 32, 16, 1024);
+}
+__device__ __forceinline__ uint64_t desc_rows(uint32_t tile, int k) { return make_desc(tile + k * 2048, SLAB, 1024); }
+
+template <int DH>
+__device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, uint32_t bar, int head, int row) {
+#pragma unroll
+  for (int s = 0; s < DH / 64; ++s) tma_load_3d(dst + s * SLAB, map, bar, 64 * s, head, row);
+}
+
+// Zero the rows of a tile that belong to no sequence (their contents are the caller's padding and may be anything, and
+// 0 x NaN would reach the product).  A whole warp; row0: the packed row of the tile's first row.
+template <int DH>
+__device__ __forceinline__ void blank_rows(uint8_t* tile, int row0, int begin, int end, int lane) {
+  for (int r = 0; r < TILE; ++r) {
+    if (row0 + r >= begin && row0 + r < end) continue;
+    for (int c = lane; c < DH / 8; c += 32)
+      *reinterpret_cast<uint4*>(tile + (c / 8) * SLAB + r * 128 + (c % 8) * 16) = make_uint4(0, 0, 0, 0);
+  }
+  fence_async_smem();
+  __syncwarp();
+}
+
+// 32 bytes of one row per store: a full sector, although neighbouring threads write different rows
+__device__ __forceinline__ void st_global_32(void* p, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
+// ---- host -------------------------------------------------------------------------------------------------------------
+// element (row, head, dim) of a 16-bit tensor at row * rs + head * hs + dim (strides in elements); boxes of 128 rows x 64
+// dims of one head, dims and rows outside the tensor read as zero
+inline int make_map_rows(CUtensorMap* m, const void* ptr, int dims, int heads, long long rows, long long rs, long long hs) {
+  EncodeFn enc = encode_fn();
+  if (!enc) return -10;
+  cuuint64_t shape[3] = {(cuuint64_t)dims, (cuuint64_t)heads, (cuuint64_t)rows};
+  cuuint64_t strides[2] = {(cuuint64_t)hs * 2, (cuuint64_t)rs * 2};
+  cuuint32_t box[3] = {64, 1, TILE};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(ptr), shape, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : -11;
+}
+
+}  // namespace packed

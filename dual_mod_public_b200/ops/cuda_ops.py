@@ -85,9 +85,15 @@ class _Sigs:
     dmb_attn_dkv_tc = [_p, _p, _p, _p, _i, _p, _p, _v, _i, _p, _p, _v, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i, _p, _p]
     dmb_attn_fwd_tc = [_p, _v, _i, _p, _p, _v, _i, _p, _i, _p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i, _i, _i,
                        _i, _i, _p, _p]
+    dmb_packed_attn_fwd = [_p, _ll, _ll, _p, _ll, _ll, _p, _ll, _ll, _p, _i, _p, _p, _i, _i, _i, _i, _i, _f, _i, _p, _p]
+    dmb_cached_attn = [_p, _ll, _ll, _p, _ll, _ll, _ll, _p, _ll, _ll, _ll, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _i, _f,
+                       _i, _p]
+    dmb_logprob_fwd = [_p, _ll, _p, _ll, _i, _i, _i, _p, _p, _p, _p, _p, _p]
+    dmb_logprob_bwd = [_p, _ll, _p, _ll, _i, _i, _p, _p, _p, _p, _p, _p]
 
 
 BF16 = torch.bfloat16
+F16 = torch.float16
 F32 = torch.float32
 
 
@@ -1018,3 +1024,106 @@ class CudaOps(TorchOps):
                                        extra.data_ptr() if extra is not None else None, out.data_ptr(),
                                        int(out_dtype == F32), rows, d, h, 1e-5, self._st()), "rmsn_bwd")
         return out
+
+    # ---- packed sequences (ops/packed.py) ---------------------------------------------------
+    def _here(self):
+        """Launches go to the current device: the table's own while one of its kernels is launched."""
+        return torch.cuda.device(self.device)
+
+    @staticmethod
+    def _rows16(t):
+        """(tensor, strides of all dims but the last) as the tensor maps and 16-byte copies take it: dense last dim, every
+        other stride a positive multiple of 16 bytes, base on a 16-byte boundary; copied when it is not.  The stride of
+        a dim of size 1 does not matter and is given as the dense one."""
+        def strides(u):
+            dense, out = u.shape[-1], []
+            for n, s in zip(reversed(u.shape[:-1]), reversed(u.stride()[:-1])):
+                out.append(dense if n == 1 else s)
+                dense *= n
+            return out[::-1]
+        st = strides(t)
+        if ((t.shape[-1] != 1 and t.stride(-1) != 1) or t.data_ptr() % 16 or any(s % 8 or s <= 0 for s in st)):
+            t = t.clone(memory_format=torch.contiguous_format)
+            st = strides(t)
+        return t, st
+
+    @staticmethod
+    def _packed_ok(q):
+        return q.dtype in (BF16, F16) and q.shape[-1] % 8 == 0 and q.shape[-1] <= 128
+
+    def packed_attn_fwd(self, q, k, v, cu, window, scale, need_lse=True):
+        if not self._packed_ok(q):
+            self._fell_back("packed_attn_fwd")
+            return super().packed_attn_fwd(q, k, v, cu, window, scale, need_lse)
+        (q, qs), (k, ks), (v, vs) = self._rows16(q), self._rows16(k), self._rows16(v)
+        T, Hq, D = q.shape
+        o = torch.empty(T, Hq, D, dtype=q.dtype, device=q.device)
+        lse = torch.empty(Hq, T, dtype=F32, device=q.device) if need_lse else None
+        if T:
+            with self._here():
+                self._ck(self.lib.dmb_packed_attn_fwd(
+                    q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], cu.data_ptr(),
+                    cu.numel() - 1, o.data_ptr(), lse.data_ptr() if need_lse else None, T, Hq, k.shape[1], D, window, scale,
+                    int(q.dtype == F16), self._tc_err.data_ptr(), self._st()), "packed_attn_fwd")
+        return o, lse
+
+    def cached_attn(self, q, k, v, lengths, window, scale):
+        if not self._packed_ok(q):
+            self._fell_back("cached_attn")
+            return super().cached_attn(q, k, v, lengths, window, scale)
+        (q, qs), (k, ks), (v, vs) = self._rows16(q), self._rows16(k), self._rows16(v)
+        B, Hq, D = q.shape
+        P, Hkv = k.shape[1], k.shape[2]
+        o = torch.empty(B, Hq, D, dtype=q.dtype, device=q.device)
+        if B == 0:
+            return o
+        chunk, splits = self.cache_chunks(B, Hkv, min(P, window) if window else P)
+        part = torch.empty(B * Hq * splits * (D + 2), dtype=F32, device=q.device) if splits > 1 else None
+        with self._here():
+            self._ck(self.lib.dmb_cached_attn(
+                q.data_ptr(), qs[0], qs[1], k.data_ptr(), *ks, v.data_ptr(), *vs, lengths.data_ptr(), o.data_ptr(),
+                part.data_ptr() if splits > 1 else None, part[B * Hq * splits * D:].data_ptr() if splits > 1 else None,
+                B, P, Hq, Hkv, D, window, chunk, splits, scale, int(q.dtype == F16), self._st()), "cached_attn")
+        return o
+
+    @staticmethod
+    def cache_chunks(B, Hkv, longest):
+        """(keys per block, blocks per sequence and key head).  Lengths are known on the device only, so a chunk is a fixed
+        number of keys and blocks behind a sequence's live rows end at once."""
+        chunk = 1024
+        while chunk > 128 and B * Hkv * -(-longest // chunk) < 4 * 148:
+            chunk //= 2
+        return chunk, max(1, -(-longest // chunk))
+
+    def token_logprobs_fwd(self, x, tokens, top, need_stats=True):
+        if x.shape[1] != 1 and x.stride(1) != 1:
+            x = x.contiguous()
+        N, V = x.shape
+        dev = x.device
+        both = torch.empty(2, N, dtype=F32, device=dev)
+        stats = torch.empty(N, 2, dtype=F32, device=dev) if need_stats else None
+        top_logp = torch.empty(N, top, dtype=F32, device=dev)
+        top_ids = torch.empty(N, top, dtype=torch.int64, device=dev)
+        if N:
+            with self._here():
+                self._ck(self.lib.dmb_logprob_fwd(
+                    x.data_ptr(), x.stride(0), tokens.data_ptr(), N, V, self._LOGIT_TYPES[x.dtype], top, both.data_ptr(),
+                    both[1].data_ptr(), stats.data_ptr() if need_stats else None, top_logp.data_ptr(), top_ids.data_ptr(),
+                    self._st()), "token_logprobs_fwd")
+        return both[0], both[1], stats, top_logp, top_ids
+
+    _LOGIT_TYPES = {F32: 0, BF16: 1, F16: 2}
+
+    def token_logprobs_bwd(self, x, tokens, stats, entropy, g_logp, g_entropy):
+        if x.shape[1] != 1 and x.stride(1) != 1:
+            x = x.contiguous()
+        N, V = x.shape
+        dx = torch.empty(N, V, dtype=x.dtype, device=x.device)
+        if N:
+            gl, gh = (None if g is None else g.float().contiguous() for g in (g_logp, g_entropy))
+            with self._here():
+                self._ck(self.lib.dmb_logprob_bwd(
+                    x.data_ptr(), x.stride(0), tokens.data_ptr(), N, V, self._LOGIT_TYPES[x.dtype], stats.data_ptr(),
+                    entropy.data_ptr(), None if gl is None else gl.data_ptr(), None if gh is None else gh.data_ptr(),
+                    dx.data_ptr(), self._st()), "token_logprobs_bwd")
+        return dx

@@ -1,0 +1,166 @@
+"""Attention and token scores for sequences of different lengths, without padding.
+
+    from dual_mod_public_b200.ops import packed_attention, cached_attention, token_logprobs
+
+    o = packed_attention(q, k, v, cu_seqlens)             # q [T, Hq, D], k / v [T, Hkv, D]; differentiable
+    o = cached_attention(q, k_cache, v_cache, lengths)    # q [B, Hq, D], caches [B, P, Hkv, D]; one token per sequence
+    r = token_logprobs(logits, tokens, top=5)             # logits [..., V] -> r.logp, r.entropy, r.top_logp, r.top_ids
+
+On a B200 these run the kernels of csrc/packed_attn_fwd.cu, packed_attn_bwd.cu, cached_attn.cu and logprob.cu, on the
+tensors' own device and its current stream; on CPU the torch statements of `packed_math.py`.  No call reads a value back to
+the host, so each can be captured into a CUDA graph, and none keeps state between calls.  Results are bitwise repeatable.
+
+Kernel arguments: bf16 or fp16 (attention; gradients: bf16), bf16, fp16 or fp32 (scores); head dims that are multiples of 8
+up to 128.  Attention of other types or head dims runs the torch statement and is counted in `default_ops(device).fallbacks`
+(`DMB_STRICT_OPS=1` raises instead).  Views whose strides a tensor map cannot describe (rows not on 16-byte boundaries,
+expanded dims) are copied first.
+
+Arguments that the host can see are checked and refused with TypeError or ValueError.  Device values are not: `cu_seqlens`
+that do not ascend or lengths outside the cache give wrong outputs but never an access out of range (`lengths` are clamped
+to [0, P]).
+"""
+
+from __future__ import annotations
+
+import math
+from typing import NamedTuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import default_ops
+
+MAX_TOP = 32
+_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def _need(ok, what, error=ValueError):
+    if not ok:
+        raise error(what)
+
+
+def _check_attention(q, k, v, index, name, kv_dims, scale, window):
+    for t, n in ((q, "q"), (k, "k"), (v, "v"), (index, name)):
+        _need(isinstance(t, torch.Tensor), f"{n}: a tensor is wanted", TypeError)
+    _need(q.dtype in _FLOATS and k.dtype == q.dtype and v.dtype == q.dtype,
+          f"q, k and v of one type (bf16, fp16 or fp32) are wanted, got {q.dtype}, {k.dtype}, {v.dtype}", TypeError)
+    _need(index.dtype == torch.int32 and index.dim() == 1, f"{name}: a 1-d int32 tensor is wanted", TypeError)
+    _need(q.device == k.device == v.device == index.device, f"q, k, v and {name} have to be on one device")
+    _need(q.dim() == 3 and k.dim() == kv_dims and k.shape == v.shape,
+          f"q of 3 dims and k, v of {kv_dims} dims and equal shape are wanted, got {tuple(q.shape)}, {tuple(k.shape)}, "
+          f"{tuple(v.shape)}")
+    Hq, D, Hkv = q.shape[1], q.shape[2], k.shape[-2]
+    _need(q.shape[0] == k.shape[0] and k.shape[-1] == D and D > 0, "q and k, v differ in rows or head dim")
+    _need(Hkv > 0 and Hq > 0 and Hq % Hkv == 0, f"{Hq} query heads are not a multiple of {Hkv} key heads")
+    _need(isinstance(window, int) and 0 <= window < 1 << 31, "window: a number of tokens (0: all) is wanted")
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    _need(scale > 0 and math.isfinite(scale), "scale has to be positive and finite")
+    return scale
+
+
+class _PackedAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, cu, window, scale):
+        ops = default_ops(q.device)
+        o, lse = ops.packed_attn_fwd(q, k, v, cu, window, scale)
+        ctx.save_for_backward(q, k, v, o, lse, cu)
+        ctx.window, ctx.scale = window, scale
+        return o
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do):
+        q, k, v, o, lse, cu = ctx.saved_tensors
+        dq, dk, dv = default_ops(q.device).packed_attn_bwd(do, q, k, v, o, lse, cu, ctx.window, ctx.scale)
+        return dq, dk, dv, None, None, None
+
+
+def packed_attention(q, k, v, cu_seqlens, *, window=0, scale=None):
+    """Causal attention over sequences packed on the row axis.
+
+    q [T, Hq, D], k / v [T, Hkv, D] with Hq a multiple of Hkv (query head h reads key head h // (Hq // Hkv));
+    cu_seqlens int32 [N + 1], ascending: sequence s is the rows [cu_seqlens[s], cu_seqlens[s + 1]) and may be empty.  A row
+    sees the rows of its own sequence up to itself, the last `window` of them when window > 0.  Rows outside
+    [cu_seqlens[0], cu_seqlens[N]) are padding: their output and gradients are zero and what they hold is not read into
+    any other row.  `scale` defaults to 1 / sqrt(D).  Returns o [T, Hq, D] in q's type; differentiable in q, k and v.
+
+    Inside a sequence the inputs have to be finite: a weight of zero times an infinite or NaN value row is NaN, and the
+    matrix products run over blocks of 128 rows, so such a row reaches other rows of its block."""
+    scale = _check_attention(q, k, v, cu_seqlens, "cu_seqlens", 3, scale, window)
+    _need(cu_seqlens.numel() >= 1, "cu_seqlens: at least one entry is wanted")
+    _need(q.shape[0] < (1 << 31) - 256, "too many rows")
+    cu_seqlens = cu_seqlens.contiguous()
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _PackedAttention.apply(q, k, v, cu_seqlens, window, scale)
+    return default_ops(q.device).packed_attn_fwd(q, k, v, cu_seqlens, window, scale, need_lse=False)[0]
+
+
+def cached_attention(q, k_cache, v_cache, lengths, *, window=0, scale=None):
+    """Attention of one new token per sequence over a cache with a live length per sequence.
+
+    q [B, Hq, D]; k_cache / v_cache [B, P, Hkv, D]; lengths int32 [B]: sequence b reads the rows [0, lengths[b]) of its
+    cache, which include the new token's own (the last `window` of them when window > 0).  Rows behind the live length are
+    never read, whatever they hold.  A length of zero gives zeros.  Returns o [B, Hq, D].  Not differentiable: a tensor
+    that requires a gradient is refused while gradients are enabled."""
+    scale = _check_attention(q, k_cache, v_cache, lengths, "lengths", 4, scale, window)
+    _need(lengths.numel() == q.shape[0], "lengths: one entry per sequence is wanted")
+    _need(not (torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad)),
+          "cached_attention has no gradient: call it under torch.no_grad()")
+    _need(k_cache.shape[1] < 1 << 31, "too many cache rows")
+    return default_ops(q.device).cached_attn(q, k_cache, v_cache, lengths.contiguous(), window, scale)
+
+
+class TokenLogprobs(NamedTuple):
+    logp: torch.Tensor                   # [...] fp32, differentiable
+    entropy: torch.Tensor                # [...] fp32, differentiable
+    top_logp: torch.Tensor | None        # [..., top] fp32, largest first
+    top_ids: torch.Tensor | None         # [..., top] int64
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, tokens, top):
+        logp, entropy, stats, top_logp, top_ids = default_ops(x.device).token_logprobs_fwd(x, tokens, top)
+        ctx.save_for_backward(x, tokens, stats, entropy)
+        ctx.mark_non_differentiable(top_logp, top_ids)
+        ctx.set_materialize_grads(False)
+        return logp, entropy, top_logp, top_ids
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_logp, g_entropy, *_):
+        if g_logp is None and g_entropy is None:
+            return None, None, None
+        x, tokens, stats, entropy = ctx.saved_tensors
+        return default_ops(x.device).token_logprobs_bwd(x, tokens, stats, entropy, g_logp, g_entropy), None, None
+
+
+def token_logprobs(logits, tokens, *, top=0):
+    """Scores of given tokens under rows of logits.
+
+    logits [..., V] (bf16, fp16 or fp32), tokens int64 [...].  Returns `TokenLogprobs`: logp = log softmax(logits)[token],
+    entropy of the row, and with top > 0 (at most 32) the `top` largest log probabilities with their ids, largest first,
+    equal ones by ascending id.  All sums in fp32; outputs fp32.  A negative token means the row has no target: logp 0 and no
+    gradient through it; a token >= V gives NaN.  logp and entropy are differentiable in the logits, the alternatives
+    are not.  -inf logits (masked entries) are fine; a row of nothing else gives NaN."""
+    for t, n in ((logits, "logits"), (tokens, "tokens")):
+        _need(isinstance(t, torch.Tensor), f"{n}: a tensor is wanted", TypeError)
+    _need(logits.dtype in _FLOATS, f"logits of bf16, fp16 or fp32 are wanted, got {logits.dtype}", TypeError)
+    _need(tokens.dtype == torch.int64, f"tokens of int64 are wanted, got {tokens.dtype}", TypeError)
+    _need(logits.device == tokens.device, "logits and tokens have to be on one device")
+    _need(logits.dim() >= 1 and logits.shape[:-1] == tokens.shape and logits.shape[-1] > 0,
+          f"tokens of the logits' leading shape are wanted, got {tuple(logits.shape)} and {tuple(tokens.shape)}")
+    V, lead = logits.shape[-1], tokens.shape
+    _need(V < 1 << 31, "too many columns")
+    _need(isinstance(top, int) and 0 <= top <= min(MAX_TOP, V), f"top: 0 to {min(MAX_TOP, V)} is wanted, got {top}")
+    flat = len(lead) == 1
+    x, y = (logits, tokens.contiguous()) if flat else (logits.reshape(-1, V), tokens.reshape(-1).contiguous())
+    if torch.is_grad_enabled() and logits.requires_grad:
+        logp, entropy, top_logp, top_ids = _TokenLogprobs.apply(x, y, top)
+    else:
+        logp, entropy, _, top_logp, top_ids = default_ops(x.device).token_logprobs_fwd(x, y, top, need_stats=False)
+    if not flat:
+        logp, entropy = logp.view(lead), entropy.view(lead)
+        if top:
+            top_logp, top_ids = top_logp.view(*lead, top), top_ids.view(*lead, top)
+    return TokenLogprobs(logp, entropy, top_logp if top else None, top_ids if top else None)

@@ -7,6 +7,7 @@ from __future__ import annotations
 import torch
 
 from ..engines import fused_math as fm
+from . import packed_math as pm
 
 
 def _into(out, vals, accumulate):
@@ -373,3 +374,24 @@ class TorchOps:
     # ---- head ---------------------------------------------------------------------------
     def ce_chunk(self, logits, targets, inv_n):
         return fm.ce_chunk(logits, targets, inv_n)
+
+    # ---- packed sequences (ops/packed.py) ---------------------------------------------------
+    def packed_attn_fwd(self, q, k, v, cu, window, scale, need_lse=True):
+        """Causal attention over packed sequences: (o [T, Hq, D], lse [Hq, T] fp32 or None)."""
+        return pm.packed_attn_fwd(q, k, v, cu, window, scale)
+
+    def packed_attn_bwd(self, do, q, k, v, o, lse, cu, window, scale):
+        """Its gradients (dq, dk, dv) from the output, its gradient and lse."""
+        return pm.packed_attn_bwd(do, q, k, v, o, lse, cu, window, scale)
+
+    def cached_attn(self, q, k, v, lengths, window, scale):
+        """One query per sequence over the live rows of a cache: o [B, Hq, D]."""
+        return pm.cached_attn(q, k, v, lengths, window, scale)
+
+    def token_logprobs_fwd(self, x, tokens, top, need_stats=True):
+        """(logp, entropy, stats [N, 2] or None, top_logp, top_ids) of rows of logits x [N, V]."""
+        return pm.token_logprobs_fwd(x, tokens, top)
+
+    def token_logprobs_bwd(self, x, tokens, stats, entropy, g_logp, g_entropy):
+        """Gradient of the logits; g_logp / g_entropy fp32 [N] or None."""
+        return pm.token_logprobs_bwd(x, tokens, stats, entropy, g_logp, g_entropy)
