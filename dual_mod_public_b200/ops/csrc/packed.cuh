@@ -148,6 +148,15 @@ __device__ __forceinline__ void st_global_32(void* p, const uint32_t (&v)[8]) {
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------
+// The driver call that encodes tensor maps wants a current context, and a thread that has made no runtime call yet (autograd
+// runs backward passes on threads of its own) has none: naming the thread's device makes it current.
+inline int bind_context() {
+  int d = 0;
+  cudaError_t e = cudaGetDevice(&d);
+  if (e == cudaSuccess) e = cudaSetDevice(d);
+  return (int)e;
+}
+
 // element (row, head, dim) of a 16-bit tensor at row * rs + head * hs + dim (strides in elements); boxes of 128 rows x 64
 // dims of one head, dims and rows outside the tensor read as zero
 inline int make_map_rows(CUtensorMap* m, const void* ptr, int dims, int heads, long long rows, long long rs, long long hs) {

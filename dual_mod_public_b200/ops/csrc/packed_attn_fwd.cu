@@ -322,7 +322,8 @@ extern "C" int dmb_packed_attn_fwd(const void* q, long long q_rs, long long q_hs
   if (T <= 0) return 0;
   if (D <= 0 || D > 128 || (D & 7) || Hkv <= 0 || Hq % Hkv || nseq < 0) return -1;
   CUtensorMap mq, mk, mv;
-  int rc = make_map_rows(&mq, q, D, Hq, T, q_rs, q_hs);
+  int rc = bind_context();
+  if (rc == 0) rc = make_map_rows(&mq, q, D, Hq, T, q_rs, q_hs);
   if (rc == 0) rc = make_map_rows(&mk, k, D, Hkv, T, k_rs, k_hs);
   if (rc == 0) rc = make_map_rows(&mv, v, D, Hkv, T, v_rs, v_hs);
   if (rc) return rc;

@@ -86,6 +86,8 @@ class _Sigs:
     dmb_attn_fwd_tc = [_p, _v, _i, _p, _p, _v, _i, _p, _i, _p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i, _i, _i,
                        _i, _i, _p, _p]
     dmb_packed_attn_fwd = [_p, _ll, _ll, _p, _ll, _ll, _p, _ll, _ll, _p, _i, _p, _p, _i, _i, _i, _i, _i, _f, _i, _p, _p]
+    dmb_packed_attn_bwd = [_p, _ll, _ll, _p, _ll, _ll, _p, _ll, _ll, _p, _ll, _ll, _p, _p, _p, _i, _p, _p, _p, _p, _i, _i, _i, _i,
+                           _i, _f, _p, _p]
     dmb_cached_attn = [_p, _ll, _ll, _p, _ll, _ll, _ll, _p, _ll, _ll, _ll, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _i, _f,
                        _i, _p]
     dmb_logprob_fwd = [_p, _ll, _p, _ll, _i, _i, _i, _p, _p, _p, _p, _p, _p]
@@ -1066,6 +1068,25 @@ class CudaOps(TorchOps):
                     cu.numel() - 1, o.data_ptr(), lse.data_ptr() if need_lse else None, T, Hq, k.shape[1], D, window, scale,
                     int(q.dtype == F16), self._tc_err.data_ptr(), self._st()), "packed_attn_fwd")
         return o, lse
+
+    def packed_attn_bwd(self, do, q, k, v, o, lse, cu, window, scale):
+        # dS = P (dP - delta) has no natural scale: in fp16 it underflows where the gradient does, so fp16 takes fp32 math
+        if not self._packed_ok(q) or q.dtype != BF16 or do.dtype != BF16:
+            self._fell_back("packed_attn_bwd")
+            return super().packed_attn_bwd(do, q, k, v, o, lse, cu, window, scale)
+        (do, gs), (q, qs), (k, ks), (v, vs) = self._rows16(do), self._rows16(q), self._rows16(k), self._rows16(v)
+        T, Hq, D = q.shape
+        Hkv = k.shape[1]
+        dq = torch.empty(T, Hq, D, dtype=BF16, device=q.device)
+        dk, dv = (torch.empty(T, Hkv, D, dtype=BF16, device=q.device) for _ in range(2))
+        if T:
+            aux = torch.empty(2 * Hq * (-(-T // 128) * 128), dtype=F32, device=q.device)
+            with self._here():
+                self._ck(self.lib.dmb_packed_attn_bwd(
+                    do.data_ptr(), *gs, q.data_ptr(), *qs, k.data_ptr(), *ks, v.data_ptr(), *vs, o.data_ptr(), lse.data_ptr(),
+                    cu.data_ptr(), cu.numel() - 1, aux.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), T, Hq, Hkv, D,
+                    window, scale, self._tc_err.data_ptr(), self._st()), "packed_attn_bwd")
+        return dq, dk, dv
 
     def cached_attn(self, q, k, v, lengths, window, scale):
         if not self._packed_ok(q):

@@ -11,7 +11,7 @@ F64_NEAR = dict(rtol=2e-5, atol=2e-5)          # fp32 statements of values of or
 
 
 def rnd(*shape, seed=0):
-    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed))
+    return torch.randn(shape, generator=torch.Generator().manual_seed(seed))
 
 
 @pytest.mark.parametrize("edges", [(0, 50), (0, 1, 1, 20, 50), (3, 10, 40), (0,), (0, 0)])
