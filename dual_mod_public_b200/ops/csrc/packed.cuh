@@ -43,9 +43,13 @@ __device__ __forceinline__ int last_query(const int* __restrict__ cu, int n, int
   return hi;
 }
 
-// ---- waits ------------------------------------------------------------------------------------------------------------
-// One try before the clock is read: most waits of a running pipeline are over when they are asked for.
-__device__ __forceinline__ bool wait_quick(uint32_t bar, uint32_t parity, volatile int* err) {
+// ---- waits and issue --------------------------------------------------------------------------------------------------
+// A wait of a whole warp, bounded like mbar_wait: when it runs out it raises *err, and every later wait of the block returns
+// at once, so the roles run to their ends on whatever lies in shared and tensor memory (all addresses stay in range) and the
+// block reports the error.  One try comes before the clock is read: most waits of a running pipeline are over when asked for.
+// No result and no vote: what follows stays warp-uniform for the compiler, which puts the operands of the tcgen05
+// instructions into uniform registers only then (issuing one took 80 cycles otherwise).
+__device__ __forceinline__ void wait(uint32_t bar, uint32_t parity, volatile int* err) {
   uint32_t ok;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
@@ -54,12 +58,29 @@ __device__ __forceinline__ bool wait_quick(uint32_t bar, uint32_t parity, volati
       : "=r"(ok)
       : "r"(bar), "r"(parity)
       : "memory");
-  return ok ? true : mbar_wait(bar, parity, err);
+  if (!ok) mbar_wait(bar, parity, err);
+  __syncwarp();
 }
-// by a whole warp; the same answer in every lane
-__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatile int* err) {
-  return __all_sync(0xffffffffu, wait_quick(bar, parity, err));
+// true in one lane of a converged warp, always the same one
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
 }
+// after a wait that ran out: an issuing warp lets its products in flight end before tensor memory is released
+__device__ __forceinline__ void drain_products(uint32_t bar, volatile int* err) {
+  if (!*err) return;
+  volatile int ignore = 0;
+  if (elect_one()) umma_commit(bar);
+  __syncwarp();
+  mbar_wait(bar, 0, &ignore);
+}
+// a value that is the same in all lanes, known as such to the compiler
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 
 // ---- element types ----------------------------------------------------------------------------------------------------
 template <typename T>
@@ -110,6 +131,24 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
         "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
+// the same with 16 columns
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // A tile of 128 rows x DH dims lies in shared memory as DH / 64 slabs of 128 rows x 128 bytes (128-byte swizzle).  The same
@@ -120,6 +159,9 @@ __device__ __forceinline__ uint64_t desc_dims(uint32_t tile, int k) {
   return make_desc(tile + (k / 4) * SLAB + (k % 4) * 32, 16, 1024);
 }
 __device__ __forceinline__ uint64_t desc_rows(uint32_t tile, int k) { return make_desc(tile + k * 2048, SLAB, 1024); }
+// what step k adds to the descriptor of step 0 (addresses count 16 bytes and stay below 2^18, so nothing carries over)
+__device__ __forceinline__ constexpr uint64_t dims_step(int k) { return ((k / 4) * SLAB + (k % 4) * 32) >> 4; }
+__device__ __forceinline__ constexpr uint64_t rows_step(int k) { return (k * 2048) >> 4; }
 
 template <int DH>
 __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, uint32_t bar, int head, int row) {
@@ -145,6 +187,66 @@ __device__ __forceinline__ void st_global_32(void* p, const uint32_t (&v)[8]) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
                "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                : "memory");
+}
+
+// ---- pairs of fp32 ----------------------------------------------------------------------------------------------------
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair(float lo, float hi) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void split(f32x2 v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float ex2(float v) {               // special-function unit; results below 2^-126 are zero
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+// 2^y of a pair on the FMA pipe, for finite y <= 126 (below -126: 2^-126).  y = n + f with n = round(y), |f| <= 1/2; 2^f by the
+// minimax polynomial of degree 4 in relative error (Remez exchange on [-1/2, 1/2]: 2.7e-6), n added to the exponent field.
+__device__ __forceinline__ void ex2_pair(f32x2 y, float& lo, float& hi) {
+  float a, b;
+  split(y, a, b);
+  y = pair(fmaxf(a, -126.f), fmaxf(b, -126.f));
+  const f32x2 magic = pair(12582912.f, 12582912.f);           // 1.5 x 2^23: its sum with y holds n in the low bits
+  const f32x2 r = add2(y, magic);
+  const f32x2 n = add2(r, pair(-12582912.f, -12582912.f));
+  const f32x2 f = fma2(n, pair(-1.f, -1.f), y);
+  f32x2 p = fma2(f, pair(0.009570102207362652f, 0.009570102207362652f), pair(0.05591785907745361f, 0.05591785907745361f));
+  p = fma2(p, f, pair(0.240247443318367f, 0.240247443318367f));
+  p = fma2(p, f, pair(0.6931217908859253f, 0.6931217908859253f));
+  p = fma2(p, f, pair(0.9999992847442627f, 0.9999992847442627f));
+  float pa, pb, ra, rb;
+  split(p, pa, pb);
+  split(r, ra, rb);
+  lo = __uint_as_float(__float_as_uint(pa) + (__float_as_uint(ra) << 23));
+  hi = __uint_as_float(__float_as_uint(pb) + (__float_as_uint(rb) << 23));
+}
+// maximum that is NaN when any operand is
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------

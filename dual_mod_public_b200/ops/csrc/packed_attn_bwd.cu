@@ -73,17 +73,12 @@ __device__ __forceinline__ void load_bulk(uint32_t dst, const void* src, uint32_
 
 // one row of a gradient: DH columns of tensor memory, scaled, to D bf16
 template <int DH>
-__device__ __forceinline__ void store_row(uint32_t taddr, bf16* dst, int D, float scale, bool some, bool live) {
+__device__ __forceinline__ void store_row(uint32_t taddr, bf16* dst, int D, float scale, bool live) {
 #pragma unroll
   for (int c = 0; c < DH / 32; ++c) {
     uint32_t r[32];
-    if (some) {
-      tmem_ld32(taddr + 32 * c, r);
-      tmem_ld_wait();
-    } else {
-#pragma unroll
-      for (int i = 0; i < 32; ++i) r[i] = 0;
-    }
+    tmem_ld32(taddr + 32 * c, r);
+    tmem_ld_wait();
     if (!live) continue;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -125,18 +120,19 @@ __global__ void __launch_bounds__(NT, 1) packed_dkv_kernel(
     return;
   }
   const uint32_t bar0 = base + C::bar_off;
-  // barriers: own, sfull, dpfull, pfull, dsfull, done, qfull[ST], gfull[ST], empty[ST]
-  const uint32_t own = bar0, sfull = bar0 + 8, dpfull = bar0 + 16, pfull = bar0 + 24, dsfull = bar0 + 32, done = bar0 + 40;
-  auto qfull = [&](int s) { return bar0 + 48 + 8u * s; };
-  auto gfull = [&](int s) { return bar0 + 48 + 8u * (C::ST + s); };
-  auto empty = [&](int s) { return bar0 + 48 + 8u * (2 * C::ST + s); };
+  // barriers: own, sfull, dpfull, pfull, dsfull, done, drained, qfull[ST], gfull[ST], empty[ST]
+  const uint32_t own = bar0, sfull = bar0 + 8, dpfull = bar0 + 16, pfull = bar0 + 24, dsfull = bar0 + 32, done = bar0 + 40,
+                 drained = bar0 + 48;
+  auto qfull = [&](int s) { return bar0 + 56 + 8u * s; };
+  auto gfull = [&](int s) { return bar0 + 56 + 8u * (C::ST + s); };
+  auto empty = [&](int s) { return bar0 + 56 + 8u * (2 * C::ST + s); };
   volatile uint32_t* tslot = reinterpret_cast<volatile uint32_t*>(smem + C::bar_off + 240);
   volatile int* serr = reinterpret_cast<volatile int*>(smem + C::bar_off + 248);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   // the first keys of a long sequence are seen by the most queries: they come first
   const int kh = blockIdx.x % g.Hkv, kt = blockIdx.x / g.Hkv, key0 = kt * TILE;
   const int last = last_query(g.cu, g.nseq, g.window, g.T, min(g.T, key0 + TILE) - 1);
-  const int nq = max(kt, last / TILE) - kt + 1, n_it = nq * g.group;         // query tiles kt .. kt + nq - 1 of each head
+  const int nq = uniform(max(kt, last / TILE)) - kt + 1, n_it = nq * g.group;         // query tiles kt .. kt + nq - 1 of each head
 
   if (threadIdx.x == 0) {
     *serr = 0;
@@ -146,6 +142,7 @@ __global__ void __launch_bounds__(NT, 1) packed_dkv_kernel(
     mbar_init(pfull, 8);
     mbar_init(dsfull, 8);
     mbar_init(done, 1);
+    mbar_init(drained, 1);
     for (int s = 0; s < C::ST; ++s) {
       mbar_init(qfull(s), 1);
       mbar_init(gfull(s), 1);
@@ -157,7 +154,7 @@ __global__ void __launch_bounds__(NT, 1) packed_dkv_kernel(
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tm = *tslot;
+  const uint32_t tm = uniform(*tslot);
   const uint32_t tS = tm, tdP = tm + TILE, tdV = tm + 2 * TILE, tdK = tdV + DH;
   const uint32_t sK = base + C::own_off, sV = sK + C::TB;
   auto sQ = [&](int s) { return base + C::ring_off + s * 2 * C::TB; };
@@ -166,16 +163,18 @@ __global__ void __launch_bounds__(NT, 1) packed_dkv_kernel(
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");          // 2 x 216 + 72 = 3 x 168
     if (warp == 9) {
-      if (lane == 0) {
+      if (elect_one()) {
         mbar_expect_tx(own, 2 * C::TB);
         load_tile<DH>(sK, &tmK, own, kh, key0);
         load_tile<DH>(sV, &tmV, own, kh, key0);
-        int i = 0;
-        for (; i < n_it; ++i) {
-          const int s = i % C::ST, h = kh * g.group + i / nq, q0 = (kt + i % nq) * TILE;
-          const float* ax = g.aux + (long long)h * g.Tp + q0;
-          const uint32_t sa = base + C::aux_off + s * 1024;
-          if (!wait_quick(empty(s), ((i / C::ST) & 1) ^ 1, serr)) break;
+      }
+      int i = 0, qi = 0, h = kh * g.group;
+      for (; i < n_it && !*serr; ++i) {
+        const int s = i % C::ST, q0 = (kt + qi) * TILE;
+        const float* ax = g.aux + (long long)h * g.Tp + q0;
+        const uint32_t sa = base + C::aux_off + s * 1024;
+        wait(empty(s), ((i / C::ST) & 1) ^ 1, serr);
+        if (elect_one()) {
           mbar_expect_tx(qfull(s), C::TB + 512);
           load_tile<DH>(sQ(s), &tmQ, qfull(s), h, q0);
           load_bulk(sa, ax, 512, qfull(s));
@@ -183,67 +182,77 @@ __global__ void __launch_bounds__(NT, 1) packed_dkv_kernel(
           load_tile<DH>(sG(s), &tmG, gfull(s), h, q0);
           load_bulk(sa + 512, ax + (long long)g.Hq * g.Tp, 512, gfull(s));
         }
-        if (*serr) {
-          volatile int ignore = 0;
-          mbar_wait(own, 0, &ignore);
-          for (int u = max(0, i - C::ST); u < i; ++u) {
-            mbar_wait(qfull(u % C::ST), (u / C::ST) & 1, &ignore);
-            mbar_wait(gfull(u % C::ST), (u / C::ST) & 1, &ignore);
-          }
+        if (++qi == nq) { qi = 0; ++h; }
+      }
+      if (*serr) {          // a wait ran out: let the copies in flight land before the CTA ends
+        volatile int ignore = 0;
+        mbar_wait(own, 0, &ignore);
+        for (int u = max(0, i - C::ST); u < i; ++u) {
+          mbar_wait(qfull(u % C::ST), (u / C::ST) & 1, &ignore);
+          mbar_wait(gfull(u % C::ST), (u / C::ST) & 1, &ignore);
         }
       }
     } else if (warp == 8) {
       constexpr uint32_t idS = mma_desc<bf16>(TILE, TILE, 0, 0), idG = mma_desc<bf16>(TILE, DH, 0, 1);
       const int begin = max(0, __ldg(g.cu)), end = min(g.T, __ldg(g.cu + g.nseq));
-      auto padded = [&](int i) {
-        const int q0 = (kt + i % nq) * TILE;
-        return q0 < begin || q0 + TILE > end;
-      };
-      auto scores = [&](int i) {                         // S^T = K Q_i^T
+      auto padded = [&](int q0) { return q0 < begin || q0 + TILE > end; };
+      auto scores = [&](int i, int q0) {                 // S^T = K Q_i^T
         const int s = i % C::ST;
-        if (!wait_warp(qfull(s), (i / C::ST) & 1, serr)) return false;
-        if (padded(i)) blank_rows<DH>(smem + C::ring_off + s * 2 * C::TB, (kt + i % nq) * TILE, begin, end, lane);
+        wait(qfull(s), (i / C::ST) & 1, serr);
+        if (padded(q0)) blank_rows<DH>(smem + C::ring_off + s * 2 * C::TB, q0, begin, end, lane);
         tc_fence_after();
-        if (lane == 0) {
+        if (elect_one()) {
+          const uint64_t k = desc_dims(sK, 0), q = desc_dims(sQ(s), 0);
 #pragma unroll
-          for (int k = 0; k < DH / 16; ++k) umma_bf16(tS, desc_dims(sK, k), desc_dims(sQ(s), k), idS, k != 0);
+          for (int u = 0; u < DH / 16; ++u) umma_bf16(tS, k + dims_step(u), q + dims_step(u), idS, u != 0);
           umma_commit(sfull);
         }
-        return true;
+        __syncwarp();
       };
-      auto dscores = [&](int i) {                        // dP^T = V dO_i^T
+      auto dscores = [&](int i, int q0) {                // dP^T = V dO_i^T
         const int s = i % C::ST;
-        if (!wait_warp(gfull(s), (i / C::ST) & 1, serr)) return false;
-        if (padded(i)) blank_rows<DH>(smem + C::ring_off + s * 2 * C::TB + C::TB, (kt + i % nq) * TILE, begin, end, lane);
+        wait(gfull(s), (i / C::ST) & 1, serr);
+        if (padded(q0)) blank_rows<DH>(smem + C::ring_off + s * 2 * C::TB + C::TB, q0, begin, end, lane);
         tc_fence_after();
-        if (lane == 0) {
+        if (elect_one()) {
+          const uint64_t v = desc_dims(sV, 0), go = desc_dims(sG(s), 0);
 #pragma unroll
-          for (int k = 0; k < DH / 16; ++k) umma_bf16(tdP, desc_dims(sV, k), desc_dims(sG(s), k), idS, k != 0);
+          for (int u = 0; u < DH / 16; ++u) umma_bf16(tdP, v + dims_step(u), go + dims_step(u), idS, u != 0);
           umma_commit(dpfull);
         }
-        return true;
+        __syncwarp();
       };
-      bool alive = wait_warp(own, 0, serr) && scores(0) && dscores(0);
-      for (int i = 0; i < n_it && alive; ++i) {
+      wait(own, 0, serr);
+      scores(0, key0);
+      dscores(0, key0);
+      int qi = 0;
+      for (int i = 0; i < n_it; ++i) {
         const int s = i % C::ST;
-        if (!wait_warp(pfull, i & 1, serr)) { alive = false; break; }
+        if (++qi == nq) qi = 0;                          // of the next step
+        wait(pfull, i & 1, serr);
         tc_fence_after();
-        if (lane == 0)
+        if (elect_one()) {
+          const uint64_t go = desc_rows(sG(s), 0);
 #pragma unroll
-          for (int k = 0; k < TILE / 16; ++k)           // the halves of P^T lie behind each other's scores: 0 .. 31 and 64 .. 95
-            umma_ts(tdV, tS + (k / 4) * 64 + (k % 4) * 8, desc_rows(sG(s), k), idG, i > 0 || k != 0);
-        if (i + 1 < n_it && !scores(i + 1)) { alive = false; break; }
-        if (!wait_warp(dsfull, i & 1, serr)) { alive = false; break; }
-        tc_fence_after();
-        if (lane == 0) {
-#pragma unroll
-          for (int k = 0; k < TILE / 16; ++k)
-            umma_ts(tdK, tdP + (k / 4) * 64 + (k % 4) * 8, desc_rows(sQ(s), k), idG, i > 0 || k != 0);
-          umma_commit(empty(s));
+          for (int u = 0; u < TILE / 16; ++u)            // the halves of P^T lie behind each other's scores: 0 .. 31 and 64 .. 95
+            umma_ts(tdV, tS + (u / 4) * 64 + (u % 4) * 8, go + rows_step(u), idG, i > 0 || u != 0);
         }
-        if (i + 1 < n_it && !dscores(i + 1)) { alive = false; break; }
+        __syncwarp();
+        if (i + 1 < n_it) scores(i + 1, key0 + qi * TILE);
+        wait(dsfull, i & 1, serr);
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t q = desc_rows(sQ(s), 0);
+#pragma unroll
+          for (int u = 0; u < TILE / 16; ++u)
+            umma_ts(tdK, tdP + (u / 4) * 64 + (u % 4) * 8, q + rows_step(u), idG, i > 0 || u != 0);
+          umma_commit(empty(s));
+          if (i + 1 == n_it) umma_commit(done);
+        }
+        __syncwarp();
+        if (i + 1 < n_it) dscores(i + 1, key0 + qi * TILE);
       }
-      if (alive && lane == 0) umma_commit(done);
+      drain_products(drained, serr);
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
@@ -251,12 +260,14 @@ __global__ void __launch_bounds__(NT, 1) packed_dkv_kernel(
     const uint32_t tl = (uint32_t)((warp & 3) * 32) << 16;
     const int hi = key < g.T ? last_query(g.cu, g.nseq, g.window, g.T, key) : key - 1;
     const int w_hi = __shfl_sync(0xffffffffu, hi, 0), w_key = key - lane + 31;        // hi ascends with the key
-    bool alive = true;
+    int qi = 0;
     for (int i = 0; i < n_it; ++i) {
-      const int s = i % C::ST, q0 = (kt + i % nq) * TILE + half * 64;
+      const int s = i % C::ST, q0 = (kt + qi) * TILE + half * 64;
+      if (++qi == nq) qi = 0;
       const float4* lse = reinterpret_cast<const float4*>(smem + C::aux_off + s * 1024) + half * 16;
       const float4* delta = lse + 32;
-      if (!wait_warp(sfull, i & 1, serr) || !wait_warp(qfull(s), (i / C::ST) & 1, serr)) { alive = false; break; }
+      wait(sfull, i & 1, serr);
+      wait(qfull(s), (i / C::ST) & 1, serr);               // lse arrived with the queries
       tc_fence_after();
       uint32_t x[2][32];
       tmem_ld32(tS + tl + half * 64, x[0]);
@@ -288,7 +299,8 @@ __global__ void __launch_bounds__(NT, 1) packed_dkv_kernel(
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(pfull);
-      if (!wait_warp(dpfull, i & 1, serr) || !wait_warp(gfull(s), (i / C::ST) & 1, serr)) { alive = false; break; }
+      wait(dpfull, i & 1, serr);
+      wait(gfull(s), (i / C::ST) & 1, serr);
       tc_fence_after();
       tmem_ld32(tdP + tl + half * 64, x[0]);
       tmem_ld32(tdP + tl + half * 64 + 32, x[1]);
@@ -317,11 +329,11 @@ __global__ void __launch_bounds__(NT, 1) packed_dkv_kernel(
       __syncwarp();
       if (lane == 0) mbar_arrive(dsfull);
     }
-    const bool some = alive && wait_warp(done, 0, serr);
+    wait(done, 0, serr);
     tc_fence_after();
     const long long off = ((long long)key * g.Hkv + kh) * g.D;
-    if (half == 0) store_row<DH>(tdV + tl, dv + off, g.D, 1.f, some, key < g.T);
-    else store_row<DH>(tdK + tl, dk + off, g.D, g.scale, some, key < g.T);
+    if (half == 0) store_row<DH>(tdV + tl, dv + off, g.D, 1.f, key < g.T);
+    else store_row<DH>(tdK + tl, dk + off, g.D, g.scale, key < g.T);
   }
   tc_fence_before();
   __syncthreads();
@@ -343,16 +355,17 @@ __global__ void __launch_bounds__(NT, 1) packed_dq_kernel(
     return;
   }
   const uint32_t bar0 = base + C::bar_off;
-  // barriers: own, sfull, dpfull, sread, dsfull, done, kfull[ST], vfull[ST], empty[ST]
-  const uint32_t own = bar0, sfull = bar0 + 8, dpfull = bar0 + 16, sread = bar0 + 24, dsfull = bar0 + 32, done = bar0 + 40;
-  auto kfull = [&](int s) { return bar0 + 48 + 8u * s; };
-  auto vfull = [&](int s) { return bar0 + 48 + 8u * (C::ST + s); };
-  auto empty = [&](int s) { return bar0 + 48 + 8u * (2 * C::ST + s); };
+  // barriers: own, sfull, dpfull, sread, dsfull, done, drained, kfull[ST], vfull[ST], empty[ST]
+  const uint32_t own = bar0, sfull = bar0 + 8, dpfull = bar0 + 16, sread = bar0 + 24, dsfull = bar0 + 32, done = bar0 + 40,
+                 drained = bar0 + 48;
+  auto kfull = [&](int s) { return bar0 + 56 + 8u * s; };
+  auto vfull = [&](int s) { return bar0 + 56 + 8u * (C::ST + s); };
+  auto empty = [&](int s) { return bar0 + 56 + 8u * (2 * C::ST + s); };
   volatile uint32_t* tslot = reinterpret_cast<volatile uint32_t*>(smem + C::bar_off + 240);
   volatile int* serr = reinterpret_cast<volatile int*>(smem + C::bar_off + 248);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int h = blockIdx.x % g.Hq, qt = g.tiles - 1 - blockIdx.x / g.Hq, row0 = qt * TILE;
-  const int kb0 = min(qt, first_key(g.cu, g.nseq, g.window, row0) / TILE), n_it = qt - kb0 + 1;
+  const int kb0 = uniform(min(qt, first_key(g.cu, g.nseq, g.window, row0) / TILE)), n_it = qt - kb0 + 1;
 
   if (threadIdx.x == 0) {
     *serr = 0;
@@ -362,6 +375,7 @@ __global__ void __launch_bounds__(NT, 1) packed_dq_kernel(
     mbar_init(sread, 8);
     mbar_init(dsfull, 8);
     mbar_init(done, 1);
+    mbar_init(drained, 1);
     for (int s = 0; s < C::ST; ++s) {
       mbar_init(kfull(s), 1);
       mbar_init(vfull(s), 1);
@@ -373,7 +387,7 @@ __global__ void __launch_bounds__(NT, 1) packed_dq_kernel(
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tm = *tslot;
+  const uint32_t tm = uniform(*tslot);
   const uint32_t tS = tm, tdP = tm + TILE, tdQ = tm + 2 * TILE;
   const uint32_t sQ = base + C::own_off, sG = sQ + C::TB;
   auto sK = [&](int s) { return base + C::ring_off + s * 2 * C::TB; };
@@ -382,72 +396,82 @@ __global__ void __launch_bounds__(NT, 1) packed_dq_kernel(
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 9) {
-      if (lane == 0) {
-        const int kh = h / g.group;
+      const int kh = h / g.group;
+      if (elect_one()) {
         mbar_expect_tx(own, 2 * C::TB);
         load_tile<DH>(sQ, &tmQ, own, h, row0);
         load_tile<DH>(sG, &tmG, own, h, row0);
-        int i = 0;
-        for (; i < n_it; ++i) {
-          const int s = i % C::ST, k0 = (kb0 + i) * TILE;
-          if (!wait_quick(empty(s), ((i / C::ST) & 1) ^ 1, serr)) break;
+      }
+      int i = 0;
+      for (; i < n_it && !*serr; ++i) {
+        const int s = i % C::ST, k0 = (kb0 + i) * TILE;
+        wait(empty(s), ((i / C::ST) & 1) ^ 1, serr);
+        if (elect_one()) {
           mbar_expect_tx(kfull(s), C::TB);
           load_tile<DH>(sK(s), &tmK, kfull(s), kh, k0);
           mbar_expect_tx(vfull(s), C::TB);
           load_tile<DH>(sV(s), &tmV, vfull(s), kh, k0);
         }
-        if (*serr) {
-          volatile int ignore = 0;
-          mbar_wait(own, 0, &ignore);
-          for (int u = max(0, i - C::ST); u < i; ++u) {
-            mbar_wait(kfull(u % C::ST), (u / C::ST) & 1, &ignore);
-            mbar_wait(vfull(u % C::ST), (u / C::ST) & 1, &ignore);
-          }
+      }
+      if (*serr) {
+        volatile int ignore = 0;
+        mbar_wait(own, 0, &ignore);
+        for (int u = max(0, i - C::ST); u < i; ++u) {
+          mbar_wait(kfull(u % C::ST), (u / C::ST) & 1, &ignore);
+          mbar_wait(vfull(u % C::ST), (u / C::ST) & 1, &ignore);
         }
       }
     } else if (warp == 8) {
       constexpr uint32_t idS = mma_desc<bf16>(TILE, TILE, 0, 0), idG = mma_desc<bf16>(TILE, DH, 0, 1);
       const int begin = max(0, __ldg(g.cu)), end = min(g.T, __ldg(g.cu + g.nseq));
-      auto scores = [&](int i) {
+      auto scores = [&](int i) {                         // S = Q K_i^T
         const int s = i % C::ST, k0 = (kb0 + i) * TILE;
-        if (!wait_warp(kfull(s), (i / C::ST) & 1, serr)) return false;
+        wait(kfull(s), (i / C::ST) & 1, serr);
         if (k0 < begin || k0 + TILE > end) blank_rows<DH>(smem + C::ring_off + s * 2 * C::TB, k0, begin, end, lane);
         tc_fence_after();
-        if (lane == 0) {
+        if (elect_one()) {
+          const uint64_t q = desc_dims(sQ, 0), k = desc_dims(sK(s), 0);
 #pragma unroll
-          for (int k = 0; k < DH / 16; ++k) umma_bf16(tS, desc_dims(sQ, k), desc_dims(sK(s), k), idS, k != 0);
+          for (int u = 0; u < DH / 16; ++u) umma_bf16(tS, q + dims_step(u), k + dims_step(u), idS, u != 0);
           umma_commit(sfull);
         }
-        return true;
+        __syncwarp();
       };
-      auto dscores = [&](int i) {
+      auto dscores = [&](int i) {                        // dP = dO V_i^T
         const int s = i % C::ST;
-        if (!wait_warp(vfull(s), (i / C::ST) & 1, serr)) return false;
+        wait(vfull(s), (i / C::ST) & 1, serr);
         tc_fence_after();
-        if (lane == 0) {
+        if (elect_one()) {
+          const uint64_t go = desc_dims(sG, 0), v = desc_dims(sV(s), 0);
 #pragma unroll
-          for (int k = 0; k < DH / 16; ++k) umma_bf16(tdP, desc_dims(sG, k), desc_dims(sV(s), k), idS, k != 0);
+          for (int u = 0; u < DH / 16; ++u) umma_bf16(tdP, go + dims_step(u), v + dims_step(u), idS, u != 0);
           umma_commit(dpfull);
         }
-        return true;
+        __syncwarp();
       };
-      bool alive = wait_warp(own, 0, serr) && scores(0) && dscores(0);
-      for (int i = 0; i < n_it && alive; ++i) {
+      wait(own, 0, serr);
+      scores(0);
+      dscores(0);
+      for (int i = 0; i < n_it; ++i) {
         const int s = i % C::ST;
-        if (!wait_warp(sread, i & 1, serr)) { alive = false; break; }
-        tc_fence_after();
-        if (i + 1 < n_it && !scores(i + 1)) { alive = false; break; }
-        if (!wait_warp(dsfull, i & 1, serr)) { alive = false; break; }
-        tc_fence_after();
-        if (lane == 0) {
-#pragma unroll
-          for (int k = 0; k < TILE / 16; ++k)
-            umma_ts(tdQ, tdP + (k / 4) * 64 + (k % 4) * 8, desc_rows(sK(s), k), idG, i > 0 || k != 0);
-          umma_commit(empty(s));
+        if (i + 1 < n_it) {
+          wait(sread, i & 1, serr);
+          scores(i + 1);
         }
-        if (i + 1 < n_it && !dscores(i + 1)) { alive = false; break; }
+        wait(dsfull, i & 1, serr);
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t k = desc_rows(sK(s), 0);
+#pragma unroll
+          for (int u = 0; u < TILE / 16; ++u)
+            umma_ts(tdQ, tdP + (u / 4) * 64 + (u % 4) * 8, k + rows_step(u), idG, i > 0 || u != 0);
+          umma_commit(empty(s));
+          if (i + 1 == n_it) umma_commit(done);
+        }
+        __syncwarp();
+        if (i + 1 < n_it) dscores(i + 1);
       }
-      if (alive && lane == 0) umma_commit(done);
+      drain_products(drained, serr);
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
@@ -456,10 +480,9 @@ __global__ void __launch_bounds__(NT, 1) packed_dq_kernel(
     const int lo = row < g.T ? first_key(g.cu, g.nseq, g.window, row) : row + 1;
     const int w_lo = __shfl_sync(0xffffffffu, lo, 31), w_row = row - lane;
     const float L = g.aux[(long long)h * g.Tp + row], delta = g.aux[((long long)g.Hq + h) * g.Tp + row];
-    bool alive = true;
     for (int i = 0; i < n_it; ++i) {
       const int k0 = (kb0 + i) * TILE + half * 64;
-      if (!wait_warp(sfull, i & 1, serr)) { alive = false; break; }
+      wait(sfull, i & 1, serr);
       tc_fence_after();
       uint32_t x[2][32];
       tmem_ld32(tS + tl + half * 64, x[0]);
@@ -471,7 +494,7 @@ __global__ void __launch_bounds__(NT, 1) packed_dq_kernel(
       float p[64];
 #pragma unroll
       for (int c = 0; c < 64; ++c) p[c] = exp2f(fmaf(__uint_as_float(x[c >> 5][c & 31]), g.scale_log2, -L));
-      if (!wait_warp(dpfull, i & 1, serr)) { alive = false; break; }
+      wait(dpfull, i & 1, serr);
       tc_fence_after();
       tmem_ld32(tdP + tl + half * 64, x[0]);
       tmem_ld32(tdP + tl + half * 64 + 32, x[1]);
@@ -495,9 +518,9 @@ __global__ void __launch_bounds__(NT, 1) packed_dq_kernel(
       __syncwarp();
       if (lane == 0) mbar_arrive(dsfull);
     }
-    const bool some = alive && wait_warp(done, 0, serr);
+    wait(done, 0, serr);
     tc_fence_after();
-    if (half == 0) store_row<DH>(tdQ + tl, dq + ((long long)row * g.Hq + h) * g.D, g.D, g.scale, some, row < g.T);
+    if (half == 0) store_row<DH>(tdQ + tl, dq + ((long long)row * g.Hq + h) * g.D, g.D, g.scale, row < g.T);
   }
   tc_fence_before();
   __syncthreads();

@@ -9,13 +9,19 @@
 // One CTA per (head, pair of query tiles), 256 rows; key blocks of 128 stream through a shared-memory ring and serve both:
 //   warps 0..3   softmax of tile 0: every thread owns one row = one lane of tensor memory
 //   warps 4..7   softmax of tile 1
-//   warp 8       issues S_a = Q_a K^T and O_a += P_a V; P comes from tensor memory, where it overwrites the scores it is
-//                made from, so the scores of a tile's next block are issued right behind the product that reads P.  While
-//                one tile's softmax runs, the tensor pipe works for the other
-//   warp 9       TMA loads
-// The running maximum is allowed to lag by up to 8 octaves (P <= 256, exact in the fp32 accumulator's range and no loss of
-// relative precision in 16 bits): O is rescaled in tensor memory only when a row's maximum outgrows that, which after the
-// first blocks is rare.  Sums are fp32; P is rounded to the operand type, half an ulp per weight (2^-9 relative for bf16).
+//   warps 8, 9   S = Q K^T, and O += P V with P in tensor memory, issued in two parts as the softmax finishes them
+//   warp 10      TMA loads
+// Scores stay in tensor memory only until the softmax has read them into registers, and P has columns of its own, so the next
+// scores are formed while the exponentials of the last ones run.  D = 64: both tiles have 128 columns for S (512 columns: 2 x
+// (128 S + 64 P + 64 O)).  D = 128: they take turns with one S (128 + 2 x (64 P + 128 O)).  The turns cost little, since S is
+// held for a product, its latency and one read, and they keep the two tiles half a block apart: one tile's exponentials run
+// while the tensor pipe works for the other.
+//
+// What bounds: 128 x 128 exponentials take 1024 cycles of the special-function unit, as long as the products at D = 128 and
+// twice as long at D = 64.  So of every eight pairs EMU are computed by a polynomial on the FMA pipe (packed.cuh), in blocks
+// without masked entries.  The running maximum is allowed to lag by up to 8 octaves (P <= 256, exact in the fp32 accumulator's
+// range and no loss of relative precision in 16 bits): O is rescaled in tensor memory only when a row's maximum outgrows
+// that, which after the first blocks is rare.  Sums are fp32; P is rounded to the operand type.
 //
 // Every mbarrier wait is bounded in time; on expiry the kernel raises a flag in global memory, stops waiting, lets its own
 // copies land (bounded) and releases its tensor memory.
@@ -25,11 +31,21 @@ using namespace packed;
 
 namespace {
 
-constexpr int NT = 384;              // two softmax warpgroups, one for loads and MMA issue (two of its warps idle)
+constexpr int NT = 384;                 // two softmax warpgroups, one for issue and loads (one of its warps idles)
 constexpr float LAG = 8.f;              // octaves
+#ifndef EMU64
+#define EMU64 3
+#endif
+#ifndef EMU128
+#define EMU128 2
+#endif
 
 template <int DH>
 struct Cfg {
+  static constexpr bool TURNS = DH == 128;                 // one S for both tiles
+  static constexpr int EMU = DH == 64 ? EMU64 : EMU128;    // pairs of eight on the FMA pipe
+  static constexpr int S_STEP = TURNS ? 0 : TILE;          // tensor memory columns: S, P, O
+  static constexpr int P_OFF = TURNS ? TILE : 2 * TILE + 2 * DH, O_OFF = 2 * TILE;
   static constexpr int TB = TILE * DH * 2;                 // one tile
   static constexpr int SLOTS = DH == 128 ? 5 : 8;
   static constexpr int q_off = 0, ring_off = 2 * TB;
@@ -43,6 +59,28 @@ struct Geo {
   float scale_log2;
 };
 
+// 32 weights of a row from 32 scores: exp2(s * scale - sub); returns their sum, leaves the packed columns in p
+template <typename T, int EMU>
+__device__ __forceinline__ f32x2 weights(const uint32_t (&x)[32], float scale, float sub, uint32_t (&p)[16]) {
+  f32x2 sum[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
+  const f32x2 sc = pair(scale, scale), sb = pair(-sub, -sub);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const f32x2 y = fma2(pair(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), sc, sb);
+    float p0, p1;
+    if ((i * EMU) % 8 + EMU > 7) {                          // EMU of eight, spread evenly
+      ex2_pair(y, p0, p1);
+    } else {
+      split(y, p0, p1);
+      p0 = ex2(p0);
+      p1 = ex2(p1);
+    }
+    sum[i & 1] = add2(sum[i & 1], pair(p0, p1));
+    p[i] = Elem<T>::pack(p0, p1);
+  }
+  return add2(sum[0], sum[1]);
+}
+
 template <typename T, int DH>
 __global__ void __launch_bounds__(NT, 1) packed_fwd_kernel(
     const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -55,45 +93,47 @@ __global__ void __launch_bounds__(NT, 1) packed_fwd_kernel(
     return;
   }
   const uint32_t bar0 = base + C::bar_off;
-  // barriers: qfull, sfull[2], pfull[2], ofull[2], full[SLOTS], empty[SLOTS]
+  // barriers: qfull, sfull[2], sread[2], plo[2], phi[2], pvdone[2], drained, full[SLOTS], empty[SLOTS]
   const uint32_t qfull = bar0;
   auto sfull = [&](int a) { return bar0 + 8u * (1 + a); };
-  auto pfull = [&](int a) { return bar0 + 8u * (3 + a); };
-  auto ofull = [&](int a) { return bar0 + 8u * (5 + a); };
-  auto full = [&](int s) { return bar0 + 8u * (7 + s); };
-  auto empty = [&](int s) { return bar0 + 8u * (7 + C::SLOTS + s); };
-  volatile uint32_t* tslot = reinterpret_cast<volatile uint32_t*>(smem + C::bar_off + 8 * 23);
-  volatile int* serr = reinterpret_cast<volatile int*>(smem + C::bar_off + 8 * 24);
+  auto sread = [&](int a) { return bar0 + 8u * (3 + a); };
+  auto plo = [&](int a) { return bar0 + 8u * (5 + a); };
+  auto phi = [&](int a) { return bar0 + 8u * (7 + a); };
+  auto pvdone = [&](int a) { return bar0 + 8u * (9 + a); };
+  const uint32_t drained = bar0 + 8u * 11;
+  auto full = [&](int s) { return bar0 + 8u * (12 + s); };
+  auto empty = [&](int s) { return bar0 + 8u * (12 + C::SLOTS + s); };
+  volatile uint32_t* tslot = reinterpret_cast<volatile uint32_t*>(smem + C::bar_off + 240);
+  volatile int* serr = reinterpret_cast<volatile int*>(smem + C::bar_off + 248);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   // the longest rows of a long sequence first
-  const int h = blockIdx.x % g.Hq, pair = g.pairs - 1 - blockIdx.x / g.Hq;
-  const int row0 = pair * 2 * TILE;
-  // key blocks [b0[a], b1[a]) of each tile; blocks are aligned to 128 rows, so the last one of a tile is its diagonal
-  int b0[2], b1[2];
-#pragma unroll
-  for (int a = 0; a < 2; ++a) {
+  const int h = blockIdx.x % g.Hq, two = g.pairs - 1 - blockIdx.x / g.Hq;
+  const int row0 = two * 2 * TILE;
+  // key blocks [first, last) of a tile; blocks are aligned to 128 rows, so the last one of a tile is its diagonal.  A first
+  // row without keys starts at itself: its tile's later rows begin no earlier.
+  auto first_block = [&](int a) {
     const int r = row0 + a * TILE;
-    b0[a] = b1[a] = 0;
-    if (r < g.T) {
-      b1[a] = r / TILE + 1;
-      b0[a] = min(first_key(g.cu, g.nseq, g.window, r) / TILE, b1[a]);
-      // a first row without keys starts at itself: its tile's later rows begin no earlier
-    }
-  }
-  const int B0 = b1[0] == b0[0] ? b0[1] : (b1[1] == b0[1] ? b0[0] : min(b0[0], b0[1])), B1 = max(b1[0], b1[1]);
+    return r < g.T ? first_key(g.cu, g.nseq, g.window, r) / TILE : 0;
+  };
+  auto last_block = [&](int a) { return row0 + a * TILE < g.T ? row0 / TILE + a + 1 : 0; };
+  const int first0 = uniform(first_block(0)), first1 = uniform(first_block(1)), last0 = last_block(0), last1 = last_block(1);
+  const int B1 = max(last0, last1), B0 = last1 ? min(first0, first1) : first0;
 
   if (threadIdx.x == 0) {
     *serr = 0;
     mbar_init(qfull, 1);
     for (int a = 0; a < 2; ++a) {
       mbar_init(sfull(a), 1);
-      mbar_init(pfull(a), 4);
-      mbar_init(ofull(a), 1);
+      mbar_init(sread(a), 4);
+      mbar_init(plo(a), 4);
+      mbar_init(phi(a), 4);
+      mbar_init(pvdone(a), 1);
     }
+    mbar_init(drained, C::TURNS ? 1 : 2);
     for (int s = 0; s < C::SLOTS; ++s) {
       mbar_init(full(s), 1);
-      mbar_init(empty(s), 1);
+      mbar_init(empty(s), C::TURNS ? 1 : 2);     // one release per issuing warp
     }
     fence_barrier_init();
   }
@@ -101,111 +141,142 @@ __global__ void __launch_bounds__(NT, 1) packed_fwd_kernel(
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tm = *tslot;
-  auto tS = [&](int a) { return tm + a * TILE; };
-  auto tO = [&](int a) { return tm + 2 * TILE + a * DH; };
+  const uint32_t tm = uniform(*tslot);
+  auto tS = [&](int a) { return tm + a * C::S_STEP; };
+  auto tP = [&](int a) { return tm + C::P_OFF + a * (TILE / 2); };
+  auto tO = [&](int a) { return tm + C::O_OFF + a * DH; };
 
   // 384 threads launch with 168 registers each; 2 x 216 + 72 = 3 x 168
   if (warp >= 8) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-  if (warp == 9) {
-    // ---------------- TMA loads: K and V of a block in turn ----------------
-    if (lane == 0 && B1 > B0) {
-      mbar_expect_tx(qfull, 2 * C::TB);
-      load_tile<DH>(base + C::q_off, &tmQ, qfull, h, row0);
-      load_tile<DH>(base + C::q_off + C::TB, &tmQ, qfull, h, row0 + TILE);     // rows past the end read as zero
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 10) {
+      // ---------------- TMA loads: K and V of a block in turn ----------------
       const int kh = h / g.group, n = 2 * (B1 - B0);
-      int i = 0;
-      for (; i < n; ++i) {
-        const int s = i % C::SLOTS;
-        if (!wait_quick(empty(s), ((i / C::SLOTS) & 1) ^ 1, serr)) break;
-        mbar_expect_tx(full(s), C::TB);
-        load_tile<DH>(base + C::ring_off + s * C::TB, (i & 1) ? &tmV : &tmK, full(s), kh, (B0 + (i >> 1)) * TILE);
+      if (elect_one()) {
+        mbar_expect_tx(qfull, 2 * C::TB);
+        load_tile<DH>(base + C::q_off, &tmQ, qfull, h, row0);
+        load_tile<DH>(base + C::q_off + C::TB, &tmQ, qfull, h, row0 + TILE);   // rows past the end read as zero
       }
-      if (*serr) {      // a role gave up: let the copies in flight land before the CTA ends
+      int i = 0;
+      for (; i < n && !*serr; ++i) {
+        const int s = i % C::SLOTS;
+        wait(empty(s), ((i / C::SLOTS) & 1) ^ 1, serr);
+        if (elect_one()) {
+          mbar_expect_tx(full(s), C::TB);
+          load_tile<DH>(base + C::ring_off + s * C::TB, (i & 1) ? &tmV : &tmK, full(s), kh, (B0 + (i >> 1)) * TILE);
+        }
+      }
+      if (*serr) {        // a wait ran out: let the copies in flight land before the CTA ends
         volatile int ignore = 0;
         mbar_wait(qfull, 0, &ignore);
         for (int u = max(0, i - C::SLOTS); u < i; ++u) mbar_wait(full(u % C::SLOTS), (u / C::SLOTS) & 1, &ignore);
       }
-    }
-  } else if (warp == 8) {
-    // ---------------- MMA issue (the whole warp waits, one lane issues) ----------------
-    constexpr uint32_t idS = mma_desc<T>(TILE, TILE, 0, 0), idO = mma_desc<T>(TILE, DH, 0, 1);
-    const int begin = max(0, __ldg(g.cu)), end = min(g.T, __ldg(g.cu + g.nseq));
-    auto issue_S = [&](int a, int slot) {
-      if (lane == 0) {
-        const uint32_t q = base + C::q_off + a * C::TB, k = base + C::ring_off + slot * C::TB;
+    } else if (warp < (C::TURNS ? 9 : 10)) {
+      // ---------------- products (the whole warp waits, one lane issues) ----------------
+      constexpr uint32_t idS = mma_desc<T>(TILE, TILE, 0, 0), idO = mma_desc<T>(TILE, DH, 0, 1);
+      const int begin = max(0, __ldg(g.cu)), end = min(g.T, __ldg(g.cu + g.nseq));
+      auto slot_full = [&](int i) { wait(full(i % C::SLOTS), (i / C::SLOTS) & 1, serr); };
+      auto scores = [&](int a, int j, bool release) {               // S = Q K_j^T into columns that are free
+        const int i = 2 * (j - B0), s = i % C::SLOTS;
+        slot_full(i);
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t q = desc_dims(base + C::q_off + a * C::TB, 0), k = desc_dims(base + C::ring_off + s * C::TB, 0);
 #pragma unroll
-        for (int s = 0; s < DH / 16; ++s) umma_bf16(tS(a), desc_dims(q, s), desc_dims(k, s), idS, s != 0);
-        umma_commit(sfull(a));
-      }
-    };
-    bool alive = B1 > B0 && wait_warp(qfull, 0, serr) && wait_warp(full(0), 0, serr);
-    int np[2] = {0, 0};                 // P tiles taken, per tile
-    if (alive) {
-      tc_fence_after();
-#pragma unroll
-      for (int a = 0; a < 2; ++a)
-        if (b0[a] <= B0 && B0 < b1[a]) issue_S(a, 0);
-      if (lane == 0) umma_commit(empty(0));
-    }
-    for (int j = B0; j < B1 && alive; ++j) {
-      const int iv = 2 * (j - B0) + 1, sv = iv % C::SLOTS;          // ring positions of V_j and K_{j+1}
-      const int ik = iv + 1, sk = ik % C::SLOTS;
-      const bool more = j + 1 < B1;
-      if (!wait_warp(full(sv), (iv / C::SLOTS) & 1, serr)) { alive = false; break; }
-      if (j * TILE < begin || (j + 1) * TILE > end) blank_rows<DH>(smem + C::ring_off + sv * C::TB, j * TILE, begin, end, lane);
-      bool k_here = false;
-#pragma unroll
-      for (int a = 0; a < 2; ++a) {
-        if (j >= b0[a] && j < b1[a]) {
-          if (!wait_warp(pfull(a), np[a] & 1, serr)) { alive = false; break; }
-          ++np[a];
-          tc_fence_after();
-          if (lane == 0) {
-            const uint32_t v = base + C::ring_off + sv * C::TB;
-#pragma unroll
-            for (int s = 0; s < TILE / 16; ++s) umma_ts(tO(a), tS(a) + 8 * s, desc_rows(v, s), idO, j > b0[a] || s != 0);
-            if (j + 1 == b1[a]) umma_commit(ofull(a));
-          }
+          for (int u = 0; u < DH / 16; ++u) umma_bf16(tS(a), q + dims_step(u), k + dims_step(u), idS, u != 0);
+          umma_commit(sfull(a));
+          if (release) umma_commit(empty(s));
         }
-        if (more && j + 1 >= b0[a] && j + 1 < b1[a]) {
-          if (!k_here) {
-            if (!wait_warp(full(sk), (ik / C::SLOTS) & 1, serr)) { alive = false; break; }
-            k_here = true;
-            tc_fence_after();
-          }
-          issue_S(a, sk);
+        __syncwarp();
+      };
+      auto values = [&](int a, int j, int n, bool release) {        // O += P V_j, n-th block of the tile
+        const int i = 2 * (j - B0) + 1, s = i % C::SLOTS;
+        slot_full(i);
+        if (j * TILE < begin || (j + 1) * TILE > end) blank_rows<DH>(smem + C::ring_off + s * C::TB, j * TILE, begin, end, lane);
+        const uint64_t v = desc_rows(base + C::ring_off + s * C::TB, 0);
+        wait(plo(a), n & 1, serr);
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int u = 0; u < 6; ++u) umma_ts(tO(a), tP(a) + 8 * u, v + rows_step(u), idO, n > 0 || u != 0);
         }
+        __syncwarp();
+        wait(phi(a), n & 1, serr);
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int u = 6; u < 8; ++u) umma_ts(tO(a), tP(a) + 8 * u, v + rows_step(u), idO, 1);
+          if (release) umma_commit(empty(s));
+          umma_commit(pvdone(a));
+        }
+        __syncwarp();
+      };
+      wait(qfull, 0, serr);
+      if (C::TURNS) {
+        // one warp for both tiles: S is free once the scores of the turn before have been read
+        auto has = [&](int a, int j) { return a ? j >= first1 && j < last1 : j >= first0 && j < last0; };
+        int before = -1, phase = 0;                                 // tile of the turn before, and which of its reads
+        auto turn = [&](int a, int j) {
+          if (before >= 0) wait(sread(before), phase & 1, serr);
+          before = a;
+          phase = j - (a ? first1 : first0);
+          scores(a, j, a == 1 || !has(1, j));
+        };
+        if (has(0, B0)) turn(0, B0);
+        if (has(1, B0)) turn(1, B0);
+        for (int j = B0; j < B1; ++j) {
+          if (has(0, j + 1)) turn(0, j + 1);
+          if (has(0, j)) values(0, j, j - first0, !has(1, j));
+          if (has(1, j + 1)) turn(1, j + 1);
+          if (has(1, j)) values(1, j, j - first1, true);
+        }
+      } else {
+        // a warp per tile; the next scores go behind the softmax's read of the last ones
+        const int a = warp - 8, b0 = a ? first1 : first0, b1 = a ? last1 : last0;
+        auto skip = [&](int j) {                                    // a block of the other tile only
+          for (int i = 2 * (j - B0); i < 2 * (j - B0) + 2; ++i) {
+            slot_full(i);
+            if (elect_one()) mbar_arrive(empty(i % C::SLOTS));
+            __syncwarp();
+          }
+        };
+        for (int j = B0; j < (b1 > b0 ? b0 : B1); ++j) skip(j);
+        if (b1 > b0) scores(a, b0, true);
+        for (int j = b0, n = 0; j < b1; ++j, ++n) {
+          if (j + 1 < b1) {
+            wait(sread(a), n & 1, serr);
+            scores(a, j + 1, true);
+          }
+          values(a, j, n, true);
+        }
+        for (int j = max(b1, B0); b1 > b0 && j < B1; ++j) skip(j);
       }
-      if (alive && lane == 0) {
-        umma_commit(empty(sv));
-        if (more) umma_commit(empty(sk));
-      }
+      drain_products(drained, serr);
     }
-  }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     // ---------------- softmax: one row per thread ----------------
-    const int a = warp >> 2, r = (warp & 3) * 32 + lane;
-    const int row = row0 + a * TILE + r;
+    const int a = warp >> 2, b0 = a ? first1 : first0, b1 = a ? last1 : last0;
+    const int row = row0 + a * TILE + (warp & 3) * 32 + lane;
     const uint32_t tl = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_addr = tS(a) + tl, o_addr = tO(a) + tl;
+    const uint32_t s_addr = tS(a) + tl, o_addr = tO(a) + tl, p_addr = tP(a) + tl;
     const int lo = row < g.T ? first_key(g.cu, g.nseq, g.window, row) : row + 1;
-    const int tile_lo = __shfl_sync(0xffffffffu, lo, 31);          // lo ascends: the last row's is the warp's greatest
-    const int w_row0 = row - lane;
+    const int w_lo = __shfl_sync(0xffffffffu, lo, 31), w_row = row - lane;          // lo ascends with the row
     float m = -INFINITY, l = 0.f;
-    bool alive = true;
     int n = 0;
-    for (int j = b0[a]; j < b1[a]; ++j, ++n) {
-      if (!wait_warp(sfull(a), n & 1, serr)) { alive = false; break; }
+    for (int j = b0; j < b1; ++j, ++n) {
+      wait(sfull(a), n & 1, serr);
       tc_fence_after();
       uint32_t x[4][32];
 #pragma unroll
       for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + 32 * c, x[c]);
       tmem_ld_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(sread(a));
       const int k0 = j * TILE;
-      if (k0 < tile_lo || k0 + TILE - 1 > w_row0) {                // some row of this warp masks some key of this block
+      const bool mask = k0 < w_lo || k0 + TILE - 1 > w_row;          // some row of this warp hides some key of this block
+      if (mask) {
         const int c_lo = lo - k0, c_hi = row - k0;
 #pragma unroll
         for (int c = 0; c < 128; ++c)
@@ -216,14 +287,18 @@ __global__ void __launch_bounds__(NT, 1) packed_fwd_kernel(
       for (int c = 0; c < 4; ++c) {
         mx[c] = __uint_as_float(x[c][0]);
 #pragma unroll
-        for (int i = 1; i < 32; ++i) mx[c] = fmaxf(mx[c], __uint_as_float(x[c][i]));
+        for (int i = 1; i < 31; i += 2) mx[c] = max3_nan(mx[c], __uint_as_float(x[c][i]), __uint_as_float(x[c][i + 1]));
+        mx[c] = max_nan(mx[c], __uint_as_float(x[c][31]));
       }
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * g.scale_log2;
-      // m: the exponent that is subtracted; -inf while the row has seen no key
-      const bool grow = top > m + LAG || (m == -INFINITY && top > -INFINITY);
+      const float top = max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3])) * g.scale_log2;
+      // m: the exponent that is subtracted; -inf while the row has seen no key.  A NaN score makes the sum NaN for good.
+      const bool grow = !(top <= m + LAG) || (m == -INFINITY && top > -INFINITY);
       const float m_new = grow ? top : m;
-      if (__any_sync(0xffffffffu, grow && l > 0.f)) {
-        const float f = grow ? exp2f(m - m_new) : 1.f;             // m = -inf: exp2(-inf) = 0, and O is still zero
+      const bool rescale = __any_sync(0xffffffffu, grow && m != -INFINITY);
+      if (rescale) {
+        wait(pvdone(a), (n - 1) & 1, serr);                          // n > 0: some row has an m
+        tc_fence_after();
+        const float f = grow ? ex2(m - m_new) : 1.f;                 // m = -inf: 0, and O is still zero
         l *= f;
 #pragma unroll
         for (int c = 0; c < DH / 32; ++c) {
@@ -237,28 +312,30 @@ __global__ void __launch_bounds__(NT, 1) packed_fwd_kernel(
       }
       m = m_new;
       const float sub = m == -INFINITY ? 0.f : m;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      f32x2 sum = pair(0.f, 0.f);
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {                                 // 64 keys = 32 columns of packed weights
-        uint32_t p[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float p0 = exp2f(fmaf(__uint_as_float(x[2 * c + (i >> 4)][2 * (i & 15)]), g.scale_log2, -sub));
-          const float p1 = exp2f(fmaf(__uint_as_float(x[2 * c + (i >> 4)][2 * (i & 15) + 1]), g.scale_log2, -sub));
-          sum[i & 1] += p0;
-          sum[2 + (i & 1)] += p1;
-          p[i] = Elem<T>::pack(p0, p1);
+      for (int c = 0; c < 4; ++c) {                                  // 32 keys = 16 columns of packed weights
+        uint32_t p[16];
+        sum = add2(sum, mask ? weights<T, 0>(x[c], g.scale_log2, sub, p) : weights<T, C::EMU>(x[c], g.scale_log2, sub, p));
+        if (c == 0 && n > 0 && !rescale) {                           // the last product has read the last weights
+          wait(pvdone(a), (n - 1) & 1, serr);
+          tc_fence_after();
         }
-        tmem_st32(s_addr + 32 * c, p);
+        tmem_st16(p_addr + 16 * c, p);
+        if (c >= 2) {
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(c == 2 ? plo(a) : phi(a));
+        }
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(pfull(a));
+      float s0, s1;
+      split(sum, s0, s1);
+      l += s0 + s1;
     }
     // ---------------- output ----------------
-    const bool some = alive && b1[a] > b0[a] && wait_warp(ofull(a), 0, serr);
+    const bool some = n > 0;
+    if (some) wait(pvdone(a), (n - 1) & 1, serr);
     tc_fence_after();
     const float inv = some && l != 0.f ? 1.f / l : 0.f;             // no key: zero (NaN sums stay NaN)
     T* o_row = out + ((long long)row * g.Hq + h) * g.D;
