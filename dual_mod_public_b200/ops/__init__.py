@@ -9,10 +9,17 @@ import torch
 from .torch_ops import TorchOps
 
 _cache = {}
+_tables = {}                          # the same by the argument itself: a call per operator is on the hot path of small ones
 
 
 def default_ops(device):
-    device = torch.device(device)
+    table = _tables.get(device)
+    if table is None:
+        table = _tables[device] = _find_table(torch.device(device))
+    return table
+
+
+def _find_table(device):
     key = (device.type, device.index)
     if key not in _cache:
         if device.type == "cuda":

@@ -9,7 +9,7 @@
 // One CTA per (head, pair of query tiles), 256 rows; key blocks of 128 stream through a shared-memory ring and serve both:
 //   warps 0..3   softmax of tile 0: every thread owns one row = one lane of tensor memory
 //   warps 4..7   softmax of tile 1
-//   warps 8, 9   S = Q K^T, and O += P V with P in tensor memory, issued in two parts as the softmax finishes them
+//   warps 8, 9   S = Q K^T, and O += P V with P in tensor memory
 //   warp 10      TMA loads
 // Scores stay in tensor memory only until the softmax has read them into registers, and P has columns of its own, so the next
 // scores are formed while the exponentials of the last ones run.  D = 64: both tiles have 128 columns for S (512 columns: 2 x
@@ -33,17 +33,12 @@ namespace {
 
 constexpr int NT = 384;                 // two softmax warpgroups, one for issue and loads (one of its warps idles)
 constexpr float LAG = 8.f;              // octaves
-#ifndef EMU64
-#define EMU64 3
-#endif
-#ifndef EMU128
-#define EMU128 2
-#endif
 
 template <int DH>
 struct Cfg {
   static constexpr bool TURNS = DH == 128;                 // one S for both tiles
-  static constexpr int EMU = DH == 64 ? EMU64 : EMU128;    // pairs of eight on the FMA pipe
+  // pairs of eight on the FMA pipe; 8192 rows, 16 heads: D = 64 1: 188.0, 2: 188.7, 3: 196.2 us; D = 128 1: 223.9, 2: 229.9, 3: 232.8
+  static constexpr int EMU = DH == 64 ? 2 : 1;
   static constexpr int S_STEP = TURNS ? 0 : TILE;          // tensor memory columns: S, P, O
   static constexpr int P_OFF = TURNS ? TILE : 2 * TILE + 2 * DH, O_OFF = 2 * TILE;
   static constexpr int TB = TILE * DH * 2;                 // one tile
@@ -93,16 +88,15 @@ __global__ void __launch_bounds__(NT, 1) packed_fwd_kernel(
     return;
   }
   const uint32_t bar0 = base + C::bar_off;
-  // barriers: qfull, sfull[2], sread[2], plo[2], phi[2], pvdone[2], drained, full[SLOTS], empty[SLOTS]
+  // barriers: qfull, sfull[2], sread[2], pfull[2], pvdone[2], drained, full[SLOTS], empty[SLOTS]
   const uint32_t qfull = bar0;
   auto sfull = [&](int a) { return bar0 + 8u * (1 + a); };
   auto sread = [&](int a) { return bar0 + 8u * (3 + a); };
-  auto plo = [&](int a) { return bar0 + 8u * (5 + a); };
-  auto phi = [&](int a) { return bar0 + 8u * (7 + a); };
-  auto pvdone = [&](int a) { return bar0 + 8u * (9 + a); };
-  const uint32_t drained = bar0 + 8u * 11;
-  auto full = [&](int s) { return bar0 + 8u * (12 + s); };
-  auto empty = [&](int s) { return bar0 + 8u * (12 + C::SLOTS + s); };
+  auto pfull = [&](int a) { return bar0 + 8u * (5 + a); };
+  auto pvdone = [&](int a) { return bar0 + 8u * (7 + a); };
+  const uint32_t drained = bar0 + 8u * 9;
+  auto full = [&](int s) { return bar0 + 8u * (10 + s); };
+  auto empty = [&](int s) { return bar0 + 8u * (10 + C::SLOTS + s); };
   volatile uint32_t* tslot = reinterpret_cast<volatile uint32_t*>(smem + C::bar_off + 240);
   volatile int* serr = reinterpret_cast<volatile int*>(smem + C::bar_off + 248);
 
@@ -126,8 +120,7 @@ __global__ void __launch_bounds__(NT, 1) packed_fwd_kernel(
     for (int a = 0; a < 2; ++a) {
       mbar_init(sfull(a), 1);
       mbar_init(sread(a), 4);
-      mbar_init(plo(a), 4);
-      mbar_init(phi(a), 4);
+      mbar_init(pfull(a), 4);
       mbar_init(pvdone(a), 1);
     }
     mbar_init(drained, C::TURNS ? 1 : 2);
@@ -194,18 +187,11 @@ __global__ void __launch_bounds__(NT, 1) packed_fwd_kernel(
         slot_full(i);
         if (j * TILE < begin || (j + 1) * TILE > end) blank_rows<DH>(smem + C::ring_off + s * C::TB, j * TILE, begin, end, lane);
         const uint64_t v = desc_rows(base + C::ring_off + s * C::TB, 0);
-        wait(plo(a), n & 1, serr);
+        wait(pfull(a), n & 1, serr);
         tc_fence_after();
         if (elect_one()) {
 #pragma unroll
-          for (int u = 0; u < 6; ++u) umma_ts(tO(a), tP(a) + 8 * u, v + rows_step(u), idO, n > 0 || u != 0);
-        }
-        __syncwarp();
-        wait(phi(a), n & 1, serr);
-        tc_fence_after();
-        if (elect_one()) {
-#pragma unroll
-          for (int u = 6; u < 8; ++u) umma_ts(tO(a), tP(a) + 8 * u, v + rows_step(u), idO, 1);
+          for (int u = 0; u < TILE / 16; ++u) umma_ts(tO(a), tP(a) + 8 * u, v + rows_step(u), idO, n > 0 || u != 0);
           if (release) umma_commit(empty(s));
           umma_commit(pvdone(a));
         }
@@ -322,13 +308,11 @@ __global__ void __launch_bounds__(NT, 1) packed_fwd_kernel(
           tc_fence_after();
         }
         tmem_st16(p_addr + 16 * c, p);
-        if (c >= 2) {
-          tmem_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(c == 2 ? plo(a) : phi(a));
-        }
       }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(pfull(a));
       float s0, s1;
       split(sum, s0, s1);
       l += s0 + s1;

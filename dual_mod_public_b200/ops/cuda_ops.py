@@ -127,6 +127,7 @@ class CudaOps(TorchOps):
         self.gemm = None                       # set by enable_gemm()
         self.strict = os.environ.get("DMB_STRICT_OPS", "0") == "1"
         self._tc_err = torch.zeros(1, dtype=torch.int32, device=self.device)   # raised by the tcgen05 attention kernels
+        self._tc_err_ptr = self._tc_err.data_ptr()
         if os.environ.get("DMB_GEMM", "tcgen05") == "tcgen05":
             from .gemm import Tcgen05Gemm
             self.gemm = Tcgen05Gemm(self.lib, self.device)
@@ -1028,15 +1029,37 @@ class CudaOps(TorchOps):
         return out
 
     # ---- packed sequences (ops/packed.py) ---------------------------------------------------
-    def _here(self):
-        """Launches go to the current device: the table's own while one of its kernels is launched."""
-        return torch.cuda.device(self.device)
+    # The smallest of these calls take the device a few microseconds, so what the host does per call is kept short.
+    def _launch(self, fn, what, *args):
+        """fn(*args, stream) on this table's device and its current stream."""
+        index = self._index
+        if index is None:
+            index = self._index = torch.cuda.current_device() if self.device.index is None else self.device.index
+        stream = torch._C._cuda_getCurrentRawStream(index)
+        if torch.cuda.current_device() == index:
+            rc = fn(*args, stream)
+        else:
+            with torch.cuda.device(index):
+                rc = fn(*args, stream)
+        if rc != 0:
+            raise RuntimeError(f"{what} failed with code {rc}")
+        self.launches += 1
+
+    _index = None
 
     @staticmethod
     def _rows16(t):
         """(tensor, strides of all dims but the last) as the tensor maps and 16-byte copies take it: dense last dim, every
         other stride a positive multiple of 16 bytes, base on a 16-byte boundary; copied when it is not.  The stride of
-        a dim of size 1 does not matter and is given as the dense one."""
+        a dim of size 1 does not matter and may be replaced by the dense one."""
+        st = t.stride()
+        if st[-1] == 1 and not t.data_ptr() & 15:
+            for s in st[:-1]:
+                if s <= 0 or s & 7:
+                    break
+            else:
+                return t, st[:-1]
+
         def strides(u):
             dense, out = u.shape[-1], []
             for n, s in zip(reversed(u.shape[:-1]), reversed(u.stride()[:-1])):
@@ -1044,14 +1067,15 @@ class CudaOps(TorchOps):
                 dense *= n
             return out[::-1]
         st = strides(t)
-        if ((t.shape[-1] != 1 and t.stride(-1) != 1) or t.data_ptr() % 16 or any(s % 8 or s <= 0 for s in st)):
+        if (t.shape[-1] != 1 and t.stride(-1) != 1) or t.data_ptr() & 15 or any(s <= 0 or s & 7 for s in st):
             t = t.clone(memory_format=torch.contiguous_format)
             st = strides(t)
         return t, st
 
     @staticmethod
     def _packed_ok(q):
-        return q.dtype in (BF16, F16) and q.shape[-1] % 8 == 0 and q.shape[-1] <= 128
+        D = q.shape[-1]
+        return (q.dtype is BF16 or q.dtype is F16) and D <= 128 and not D & 7
 
     def packed_attn_fwd(self, q, k, v, cu, window, scale, need_lse=True):
         if not self._packed_ok(q):
@@ -1059,33 +1083,31 @@ class CudaOps(TorchOps):
             return super().packed_attn_fwd(q, k, v, cu, window, scale, need_lse)
         (q, qs), (k, ks), (v, vs) = self._rows16(q), self._rows16(k), self._rows16(v)
         T, Hq, D = q.shape
-        o = torch.empty(T, Hq, D, dtype=q.dtype, device=q.device)
-        lse = torch.empty(Hq, T, dtype=F32, device=q.device) if need_lse else None
+        o = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
+        lse = torch.empty((Hq, T), dtype=F32, device=q.device) if need_lse else None
         if T:
-            with self._here():
-                self._ck(self.lib.dmb_packed_attn_fwd(
-                    q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], cu.data_ptr(),
-                    cu.numel() - 1, o.data_ptr(), lse.data_ptr() if need_lse else None, T, Hq, k.shape[1], D, window, scale,
-                    int(q.dtype == F16), self._tc_err.data_ptr(), self._st()), "packed_attn_fwd")
+            self._launch(self.lib.dmb_packed_attn_fwd, "packed_attn_fwd", q.data_ptr(), *qs, k.data_ptr(), *ks, v.data_ptr(),
+                         *vs, cu.data_ptr(), cu.shape[0] - 1, o.data_ptr(), lse.data_ptr() if need_lse else None, T, Hq,
+                         k.shape[1], D, window, scale, q.dtype is F16, self._tc_err_ptr)
         return o, lse
 
     def packed_attn_bwd(self, do, q, k, v, o, lse, cu, window, scale):
         # dS = P (dP - delta) has no natural scale: in fp16 it underflows where the gradient does, so fp16 takes fp32 math
-        if not self._packed_ok(q) or q.dtype != BF16 or do.dtype != BF16:
+        if not self._packed_ok(q) or q.dtype is not BF16 or do.dtype is not BF16:
             self._fell_back("packed_attn_bwd")
             return super().packed_attn_bwd(do, q, k, v, o, lse, cu, window, scale)
         (do, gs), (q, qs), (k, ks), (v, vs) = self._rows16(do), self._rows16(q), self._rows16(k), self._rows16(v)
         T, Hq, D = q.shape
         Hkv = k.shape[1]
-        dq = torch.empty(T, Hq, D, dtype=BF16, device=q.device)
-        dk, dv = (torch.empty(T, Hkv, D, dtype=BF16, device=q.device) for _ in range(2))
+        dev = q.device
+        dq = torch.empty((T, Hq, D), dtype=BF16, device=dev)
+        dk = torch.empty((T, Hkv, D), dtype=BF16, device=dev)
+        dv = torch.empty((T, Hkv, D), dtype=BF16, device=dev)
         if T:
-            aux = torch.empty(2 * Hq * (-(-T // 128) * 128), dtype=F32, device=q.device)
-            with self._here():
-                self._ck(self.lib.dmb_packed_attn_bwd(
-                    do.data_ptr(), *gs, q.data_ptr(), *qs, k.data_ptr(), *ks, v.data_ptr(), *vs, o.data_ptr(), lse.data_ptr(),
-                    cu.data_ptr(), cu.numel() - 1, aux.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), T, Hq, Hkv, D,
-                    window, scale, self._tc_err.data_ptr(), self._st()), "packed_attn_bwd")
+            aux = torch.empty(2 * Hq * (-(-T // 128) * 128), dtype=F32, device=dev)
+            self._launch(self.lib.dmb_packed_attn_bwd, "packed_attn_bwd", do.data_ptr(), *gs, q.data_ptr(), *qs, k.data_ptr(),
+                         *ks, v.data_ptr(), *vs, o.data_ptr(), lse.data_ptr(), cu.data_ptr(), cu.shape[0] - 1, aux.data_ptr(),
+                         dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), T, Hq, Hkv, D, window, scale, self._tc_err_ptr)
         return dq, dk, dv
 
     def cached_attn(self, q, k, v, lengths, window, scale):
@@ -1095,16 +1117,17 @@ class CudaOps(TorchOps):
         (q, qs), (k, ks), (v, vs) = self._rows16(q), self._rows16(k), self._rows16(v)
         B, Hq, D = q.shape
         P, Hkv = k.shape[1], k.shape[2]
-        o = torch.empty(B, Hq, D, dtype=q.dtype, device=q.device)
+        o = torch.empty((B, Hq, D), dtype=q.dtype, device=q.device)
         if B == 0:
             return o
         chunk, splits = self.cache_chunks(B, Hkv, min(P, window) if window else P)
-        part = torch.empty(B * Hq * splits * (D + 2), dtype=F32, device=q.device) if splits > 1 else None
-        with self._here():
-            self._ck(self.lib.dmb_cached_attn(
-                q.data_ptr(), qs[0], qs[1], k.data_ptr(), *ks, v.data_ptr(), *vs, lengths.data_ptr(), o.data_ptr(),
-                part.data_ptr() if splits > 1 else None, part[B * Hq * splits * D:].data_ptr() if splits > 1 else None,
-                B, P, Hq, Hkv, D, window, chunk, splits, scale, int(q.dtype == F16), self._st()), "cached_attn")
+        part, po, pml = None, None, None
+        if splits > 1:
+            part = torch.empty(B * Hq * splits * (D + 2), dtype=F32, device=q.device)
+            po = part.data_ptr()
+            pml = po + B * Hq * splits * D * 4
+        self._launch(self.lib.dmb_cached_attn, "cached_attn", q.data_ptr(), *qs, k.data_ptr(), *ks, v.data_ptr(), *vs,
+                     lengths.data_ptr(), o.data_ptr(), po, pml, B, P, Hq, Hkv, D, window, chunk, splits, scale, q.dtype is F16)
         return o
 
     @staticmethod
@@ -1116,35 +1139,35 @@ class CudaOps(TorchOps):
             chunk //= 2
         return chunk, max(1, -(-longest // chunk))
 
+    _LOGIT_TYPES = {F32: 0, BF16: 1, F16: 2}
+
     def token_logprobs_fwd(self, x, tokens, top, need_stats=True):
-        if x.shape[1] != 1 and x.stride(1) != 1:
+        if x.stride(1) != 1 and x.shape[1] != 1:
             x = x.contiguous()
         N, V = x.shape
         dev = x.device
-        both = torch.empty(2, N, dtype=F32, device=dev)
-        stats = torch.empty(N, 2, dtype=F32, device=dev) if need_stats else None
-        top_logp = torch.empty(N, top, dtype=F32, device=dev)
-        top_ids = torch.empty(N, top, dtype=torch.int64, device=dev)
+        logp = torch.empty(N, dtype=F32, device=dev)
+        entropy = torch.empty(N, dtype=F32, device=dev)
+        stats = torch.empty((N, 2), dtype=F32, device=dev) if need_stats else None
+        top_logp = top_ids = None
+        if top:
+            top_logp = torch.empty((N, top), dtype=F32, device=dev)
+            top_ids = torch.empty((N, top), dtype=torch.int64, device=dev)
         if N:
-            with self._here():
-                self._ck(self.lib.dmb_logprob_fwd(
-                    x.data_ptr(), x.stride(0), tokens.data_ptr(), N, V, self._LOGIT_TYPES[x.dtype], top, both.data_ptr(),
-                    both[1].data_ptr(), stats.data_ptr() if need_stats else None, top_logp.data_ptr(), top_ids.data_ptr(),
-                    self._st()), "token_logprobs_fwd")
-        return both[0], both[1], stats, top_logp, top_ids
-
-    _LOGIT_TYPES = {F32: 0, BF16: 1, F16: 2}
+            self._launch(self.lib.dmb_logprob_fwd, "token_logprobs_fwd", x.data_ptr(), x.stride(0), tokens.data_ptr(), N, V,
+                         self._LOGIT_TYPES[x.dtype], top, logp.data_ptr(), entropy.data_ptr(),
+                         stats.data_ptr() if need_stats else None, top_logp.data_ptr() if top else None,
+                         top_ids.data_ptr() if top else None)
+        return logp, entropy, stats, top_logp, top_ids
 
     def token_logprobs_bwd(self, x, tokens, stats, entropy, g_logp, g_entropy):
-        if x.shape[1] != 1 and x.stride(1) != 1:
+        if x.stride(1) != 1 and x.shape[1] != 1:
             x = x.contiguous()
         N, V = x.shape
-        dx = torch.empty(N, V, dtype=x.dtype, device=x.device)
+        dx = torch.empty((N, V), dtype=x.dtype, device=x.device)
         if N:
             gl, gh = (None if g is None else g.float().contiguous() for g in (g_logp, g_entropy))
-            with self._here():
-                self._ck(self.lib.dmb_logprob_bwd(
-                    x.data_ptr(), x.stride(0), tokens.data_ptr(), N, V, self._LOGIT_TYPES[x.dtype], stats.data_ptr(),
-                    entropy.data_ptr(), None if gl is None else gl.data_ptr(), None if gh is None else gh.data_ptr(),
-                    dx.data_ptr(), self._st()), "token_logprobs_bwd")
+            self._launch(self.lib.dmb_logprob_bwd, "token_logprobs_bwd", x.data_ptr(), x.stride(0), tokens.data_ptr(), N, V,
+                         self._LOGIT_TYPES[x.dtype], stats.data_ptr(), entropy.data_ptr(),
+                         None if gl is None else gl.data_ptr(), None if gh is None else gh.data_ptr(), dx.data_ptr())
         return dx

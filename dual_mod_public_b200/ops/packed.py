@@ -32,29 +32,35 @@ from . import default_ops
 
 MAX_TOP = 32
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
-
-
-def _need(ok, what, error=ValueError):
-    if not ok:
-        raise error(what)
+_T = torch.Tensor
 
 
 def _check_attention(q, k, v, index, name, kv_dims, scale, window):
-    for t, n in ((q, "q"), (k, "k"), (v, "v"), (index, name)):
-        _need(isinstance(t, torch.Tensor), f"{n}: a tensor is wanted", TypeError)
-    _need(q.dtype in _FLOATS and k.dtype == q.dtype and v.dtype == q.dtype,
-          f"q, k and v of one type (bf16, fp16 or fp32) are wanted, got {q.dtype}, {k.dtype}, {v.dtype}", TypeError)
-    _need(index.dtype == torch.int32 and index.dim() == 1, f"{name}: a 1-d int32 tensor is wanted", TypeError)
-    _need(q.device == k.device == v.device == index.device, f"q, k, v and {name} have to be on one device")
-    _need(q.dim() == 3 and k.dim() == kv_dims and k.shape == v.shape,
-          f"q of 3 dims and k, v of {kv_dims} dims and equal shape are wanted, got {tuple(q.shape)}, {tuple(k.shape)}, "
-          f"{tuple(v.shape)}")
-    Hq, D, Hkv = q.shape[1], q.shape[2], k.shape[-2]
-    _need(q.shape[0] == k.shape[0] and k.shape[-1] == D and D > 0, "q and k, v differ in rows or head dim")
-    _need(Hkv > 0 and Hq > 0 and Hq % Hkv == 0, f"{Hq} query heads are not a multiple of {Hkv} key heads")
-    _need(isinstance(window, int) and 0 <= window < 1 << 31, "window: a number of tokens (0: all) is wanted")
-    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    _need(scale > 0 and math.isfinite(scale), "scale has to be positive and finite")
+    """The scale; raises for arguments that do not fit.  One pass over the conditions that hold for a call that fits."""
+    if not isinstance(q, _T) or not isinstance(k, _T) or not isinstance(v, _T) or not isinstance(index, _T):
+        raise TypeError(f"q, k, v and {name}: tensors are wanted")
+    dtype, device, qs, ks = q.dtype, q.device, q.shape, k.shape
+    if dtype not in _FLOATS or k.dtype is not dtype or v.dtype is not dtype:
+        raise TypeError(f"q, k and v of one type (bf16, fp16 or fp32) are wanted, got {q.dtype}, {k.dtype}, {v.dtype}")
+    if index.dtype is not torch.int32 or index.dim() != 1:
+        raise TypeError(f"{name}: a 1-d int32 tensor is wanted")
+    if k.device != device or v.device != device or index.device != device:
+        raise ValueError(f"q, k, v and {name} have to be on one device")
+    if len(qs) != 3 or len(ks) != kv_dims or v.shape != ks:
+        raise ValueError(f"q of 3 dims and k, v of {kv_dims} dims and equal shape are wanted, got {tuple(qs)}, {tuple(ks)}, "
+                         f"{tuple(v.shape)}")
+    Hq, D, Hkv = qs[1], qs[2], ks[-2]
+    if qs[0] != ks[0] or ks[-1] != D or D == 0:
+        raise ValueError(f"q and k, v differ in rows or head dim: {tuple(qs)}, {tuple(ks)}")
+    if Hkv == 0 or Hq == 0 or Hq % Hkv:
+        raise ValueError(f"{Hq} query heads are not a multiple of {Hkv} key heads")
+    if not isinstance(window, int) or not 0 <= window < 1 << 31:
+        raise ValueError(f"window: a number of tokens (0: all) is wanted, got {window!r}")
+    if scale is None:
+        return 1.0 / math.sqrt(D)
+    scale = float(scale)
+    if not 0 < scale < math.inf:
+        raise ValueError(f"scale has to be positive and finite, got {scale}")
     return scale
 
 
@@ -87,8 +93,10 @@ def packed_attention(q, k, v, cu_seqlens, *, window=0, scale=None):
     Inside a sequence the inputs have to be finite: a weight of zero times an infinite or NaN value row is NaN, and the
     matrix products run over blocks of 128 rows, so such a row reaches other rows of its block."""
     scale = _check_attention(q, k, v, cu_seqlens, "cu_seqlens", 3, scale, window)
-    _need(cu_seqlens.numel() >= 1, "cu_seqlens: at least one entry is wanted")
-    _need(q.shape[0] < (1 << 31) - 256, "too many rows")
+    if cu_seqlens.shape[0] < 1:
+        raise ValueError("cu_seqlens: at least one entry is wanted")
+    if q.shape[0] >= (1 << 31) - 256:
+        raise ValueError("too many rows")
     cu_seqlens = cu_seqlens.contiguous()
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _PackedAttention.apply(q, k, v, cu_seqlens, window, scale)
@@ -103,10 +111,12 @@ def cached_attention(q, k_cache, v_cache, lengths, *, window=0, scale=None):
     never read, whatever they hold.  A length of zero gives zeros.  Returns o [B, Hq, D].  Not differentiable: a tensor
     that requires a gradient is refused while gradients are enabled."""
     scale = _check_attention(q, k_cache, v_cache, lengths, "lengths", 4, scale, window)
-    _need(lengths.numel() == q.shape[0], "lengths: one entry per sequence is wanted")
-    _need(not (torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad)),
-          "cached_attention has no gradient: call it under torch.no_grad()")
-    _need(k_cache.shape[1] < 1 << 31, "too many cache rows")
+    if lengths.shape[0] != q.shape[0]:
+        raise ValueError("lengths: one entry per sequence is wanted")
+    if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
+        raise ValueError("cached_attention has no gradient: call it under torch.no_grad()")
+    if k_cache.shape[1] >= 1 << 31:
+        raise ValueError("too many cache rows")
     return default_ops(q.device).cached_attn(q, k_cache, v_cache, lengths.contiguous(), window, scale)
 
 
@@ -122,7 +132,8 @@ class _TokenLogprobs(torch.autograd.Function):
     def forward(ctx, x, tokens, top):
         logp, entropy, stats, top_logp, top_ids = default_ops(x.device).token_logprobs_fwd(x, tokens, top)
         ctx.save_for_backward(x, tokens, stats, entropy)
-        ctx.mark_non_differentiable(top_logp, top_ids)
+        if top:
+            ctx.mark_non_differentiable(top_logp, top_ids)
         ctx.set_materialize_grads(False)
         return logp, entropy, top_logp, top_ids
 
@@ -143,19 +154,25 @@ def token_logprobs(logits, tokens, *, top=0):
     equal ones by ascending id.  All sums in fp32; outputs fp32.  A negative token means the row has no target: logp 0 and no
     gradient through it; a token >= V gives NaN.  logp and entropy are differentiable in the logits, the alternatives
     are not.  -inf logits (masked entries) are fine; a row of nothing else gives NaN."""
-    for t, n in ((logits, "logits"), (tokens, "tokens")):
-        _need(isinstance(t, torch.Tensor), f"{n}: a tensor is wanted", TypeError)
-    _need(logits.dtype in _FLOATS, f"logits of bf16, fp16 or fp32 are wanted, got {logits.dtype}", TypeError)
-    _need(tokens.dtype == torch.int64, f"tokens of int64 are wanted, got {tokens.dtype}", TypeError)
-    _need(logits.device == tokens.device, "logits and tokens have to be on one device")
-    _need(logits.dim() >= 1 and logits.shape[:-1] == tokens.shape and logits.shape[-1] > 0,
-          f"tokens of the logits' leading shape are wanted, got {tuple(logits.shape)} and {tuple(tokens.shape)}")
-    V, lead = logits.shape[-1], tokens.shape
-    _need(V < 1 << 31, "too many columns")
-    _need(isinstance(top, int) and 0 <= top <= min(MAX_TOP, V), f"top: 0 to {min(MAX_TOP, V)} is wanted, got {top}")
+    if not isinstance(logits, _T) or not isinstance(tokens, _T):
+        raise TypeError("logits and tokens: tensors are wanted")
+    if logits.dtype not in _FLOATS:
+        raise TypeError(f"logits of bf16, fp16 or fp32 are wanted, got {logits.dtype}")
+    if tokens.dtype is not torch.int64:
+        raise TypeError(f"tokens of int64 are wanted, got {tokens.dtype}")
+    if logits.device != tokens.device:
+        raise ValueError("logits and tokens have to be on one device")
+    shape, lead = logits.shape, tokens.shape
+    if len(shape) == 0 or shape[:-1] != lead or shape[-1] == 0:
+        raise ValueError(f"tokens of the logits' leading shape are wanted, got {tuple(shape)} and {tuple(lead)}")
+    V = shape[-1]
+    if V >= 1 << 31 or tokens.numel() >= 1 << 31:
+        raise ValueError("too many rows or columns")
+    if not isinstance(top, int) or not 0 <= top <= min(MAX_TOP, V):
+        raise ValueError(f"top: 0 to {min(MAX_TOP, V)} is wanted, got {top!r}")
     flat = len(lead) == 1
     x, y = (logits, tokens.contiguous()) if flat else (logits.reshape(-1, V), tokens.reshape(-1).contiguous())
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if logits.requires_grad and torch.is_grad_enabled():
         logp, entropy, top_logp, top_ids = _TokenLogprobs.apply(x, y, top)
     else:
         logp, entropy, _, top_logp, top_ids = default_ops(x.device).token_logprobs_fwd(x, y, top, need_stats=False)
