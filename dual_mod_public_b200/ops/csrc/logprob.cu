@@ -3,31 +3,25 @@
 //   m = max x,  S = sum exp(x - m),  logp = (x_y - m) - log S,  H = log S - sum p (x - m),  p = exp(x - m) / S
 //   d x = g_logp (1[y] - p) - g_H p (log p + H)
 //
-// Both passes stream the row once with 16-byte loads and are bound by DRAM.  Forward: a block per row, eight loads in flight
-// per thread, running maximum and sums per thread (fp32; a thread adds V / 256 terms, the rest is a tree), so nothing of the
-// row is kept.  Differences to the maximum are formed before they are scaled: a row whose entries all are the type's lowest
-// value is uniform, as it should be.
-// Alternatives: every eighth thread group's maximum is an entry of the row, so the top-th largest of those 32 maxima bounds
-// the top-th largest entry from below; only threads whose own maximum reaches the bound look at their part of the row again
-// (from L2), and what reaches the bound, a few entries more than `top`, is ranked by (value, lower index first).
+// Both passes stream the row once with 16-byte loads and are bound by DRAM.  Forward: a group of threads per row (a warp, 256
+// or 1024 threads, see `fwd`), two sets of loads in flight per thread, running maximum and sums per thread (fp32; a thread adds
+// its part of the row, the rest is a tree), so nothing of the row is kept.  A block takes rows in turn and requests the next
+// row's first part before it joins the sums of the last.  Differences to the maximum are formed before they are scaled: a row
+// whose entries all are the type's lowest value is uniform, as it should be.
+// Alternatives: the maxima of 32 parts of the row are entries of it, so the top-th largest of them bounds the top-th largest
+// entry from below; only threads whose own maximum reaches the bound look at their entries again (from L2), and what reaches
+// the bound, a few entries more than `top`, is ranked by (value, lower index first).
 // A row has no target where its token is negative: logp = 0, no gradient through it.  A token beyond the vocabulary gives NaN.
-#include <cuda_fp16.h>
-
-#include "common.cuh"
+#include "packed.cuh"
 
 namespace {
 
-constexpr int NT = 256, U = 8, GROUPS = 32, MAX_TOP = 32, CAP = 1024;
+constexpr int MAX_TOP = 32;
 constexpr float L2E = 1.4426950408889634f;
 // exp of anything below this is zero in fp32; keeps 0 x (-inf) out of the sums
 constexpr float LOWEST = -200.f;
 
-// one exponential on the special-function unit; results below 2^-126 are zero
-__device__ __forceinline__ float ex2(float v) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
+using packed::ex2;
 
 template <typename T>
 struct Vec;   // 16 bytes of a row
@@ -39,6 +33,9 @@ struct Vec<float> {
   }
   static __device__ __forceinline__ uint4 put(const float (&f)[4]) {
     return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  }
+  static __device__ __forceinline__ float top(const uint4& u) {       // the largest, NaN aside
+    return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
   }
   static __device__ __forceinline__ float one(float v) { return v; }
   static __device__ __forceinline__ float from(float v) { return v; }
@@ -56,6 +53,11 @@ struct Vec<bf16> {
   }
   static __device__ __forceinline__ uint4 put(const float (&f)[8]) {
     return make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
+  }
+  static __device__ __forceinline__ float top(const uint4& u) {
+    auto h = [](uint32_t w) { return *reinterpret_cast<const bf162*>(&w); };
+    const bf162 m = __hmax2(__hmax2(h(u.x), h(u.y)), __hmax2(h(u.z), h(u.w)));
+    return fmaxf(__bfloat162float(m.x), __bfloat162float(m.y));
   }
   static __device__ __forceinline__ float one(bf16 v) { return __bfloat162float(v); }
   static __device__ __forceinline__ bf16 from(float v) { return __float2bfloat16_rn(v); }
@@ -80,6 +82,11 @@ struct Vec<__half> {
       w[i] = *reinterpret_cast<const uint32_t*>(&v);
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  static __device__ __forceinline__ float top(const uint4& u) {
+    auto h = [](uint32_t w) { return *reinterpret_cast<const __half2*>(&w); };
+    const __half2 m = __hmax2(__hmax2(h(u.x), h(u.y)), __hmax2(h(u.z), h(u.w)));
+    return fmaxf(__half2float(m.x), __half2float(m.y));
   }
   static __device__ __forceinline__ float one(__half v) { return __half2float(v); }
   static __device__ __forceinline__ __half from(float v) { return __float2half_rn(v); }
@@ -107,208 +114,290 @@ struct Run {
     s *= f;
     m = top;
   }
-  __device__ __forceinline__ void add(float x) {
-    const float d = x - m, p = ex2(d * L2E);
+  __device__ __forceinline__ void one(float v) {
+    if (v > m) raise(v);
+    if (v == -INFINITY) return;                               // adds nothing, also where m is -inf
+    const float d = v - m, p = ex2(d * L2E);
     s += p;
     e = fmaf(p, fmaxf(d, LOWEST), e);
   }
-  __device__ __forceinline__ void join(float m2, float s2, float e2) {
-    const float top = fmaxf(m, m2);
-    if (top == -INFINITY) return;
-    const float d1 = m - top, d2 = m2 - top;
-    const float f1 = ex2(d1 * L2E), f2 = ex2(d2 * L2E);
-    e = f1 * fmaf(fmaxf(d1, LOWEST), s, e) + f2 * fmaf(fmaxf(d2, LOWEST), s2, e2);
-    s = f1 * s + f2 * s2;
-    m = top;
+  // K vectors at once; `live` of them count
+  template <typename T, int K>
+  __device__ __forceinline__ void many(const uint4 (&u)[K], int live) {
+    constexpr int N = Vec<T>::N;
+    float top = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (k < live) top = fmaxf(top, Vec<T>::top(u[k]));
+    if (top > m) raise(top);
+    const packed::f32x2 nm = packed::pair(-m, -m), l2 = packed::pair(L2E, L2E);
+    packed::f32x2 s2 = packed::pair(0.f, 0.f), e2 = packed::pair(0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (k < live) {
+        float v[N];
+        Vec<T>::get(u[k], v);
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+          const packed::f32x2 d = packed::add2(packed::pair(v[i], v[i + 1]), nm), y = packed::mul2(d, l2);
+          float y0, y1;
+          packed::split(y, y0, y1);
+          const packed::f32x2 p = packed::pair(ex2(y0), ex2(y1));
+          s2 = packed::add2(s2, p);
+          e2 = packed::fma2(p, d, e2);
+        }
+      }
+    float s0, s1, e0, e1;
+    packed::split(s2, s0, s1);
+    packed::split(e2, e0, e1);
+    if (e0 + e1 == e0 + e1) {
+      s += s0 + s1;
+      e += e0 + e1;
+      return;
+    }
+#pragma unroll 1
+    for (int k = 0; k < K; ++k) {                             // -inf among them (0 x inf above), or NaN: one by one
+      uint4 w = u[0];
+#pragma unroll
+      for (int q = 1; q < K; ++q)
+        if (q == k) w = u[q];
+      float v[N];
+      Vec<T>::get(w, v);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (k < live) one(v[i]);
+    }
   }
 };
 
 __device__ __forceinline__ bool ahead(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
 
-// the entries of this thread's part of the row, each with its index
-template <typename T, typename F>
-__device__ __forceinline__ void each_own(const T* x, const Cut& c, int V, F f) {
-  const int t = threadIdx.x;
-  if (t < c.head) f(Vec<T>::one(x[t]), t);
-  const uint4* body = reinterpret_cast<const uint4*>(x + c.head);
-  for (int i = t; i < c.nvec; i += NT) {
-    float v[Vec<T>::N];
-    Vec<T>::get(__ldg(body + i), v);
-#pragma unroll
-    for (int k = 0; k < Vec<T>::N; ++k) f(v[k], c.head + i * Vec<T>::N + k);
-  }
-  if (c.tail0 + t < V) f(Vec<T>::one(x[c.tail0 + t]), c.tail0 + t);
+__device__ __forceinline__ uint4 load_stream(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
 }
 
-template <typename T, bool TOP>
-__global__ void __launch_bounds__(NT) logprob_fwd_kernel(const T* __restrict__ logits, long long rs,
-                                                         const long long* __restrict__ tokens, int V, int top,
-                                                         float* __restrict__ logp, float* __restrict__ entropy,
-                                                         float2* __restrict__ stats, float* __restrict__ top_logp,
-                                                         long long* __restrict__ top_ids) {
-  constexpr int N = Vec<T>::N;
-  const long long row = blockIdx.x;
+// A group of NT threads per row; blocks of max(NT, 256) threads.
+template <int NT>
+struct Group {
+  static constexpr int BLOCK = NT < 256 ? 256 : NT, ROWS = BLOCK / NT, WARPS = NT / 32;
+  static constexpr int CAP = NT == 32 ? 96 : 1024;            // candidates that a list holds
+  static __device__ __forceinline__ void sync() {
+    if (NT == 32) __syncwarp(); else __syncthreads();
+  }
+};
+template <int NT>
+struct Shared {                                               // of one group
+  float m[Group<NT>::WARPS], s[Group<NT>::WARPS], e[Group<NT>::WARPS], part[32], bound;
+  int n;
+  float cv[Group<NT>::CAP];
+  int ci[Group<NT>::CAP];
+};
+
+template <int NT, typename T, bool TOP>
+__global__ void __launch_bounds__(Group<NT>::BLOCK, NT == 1024 ? 1 : 4)
+logprob_fwd_kernel(const T* __restrict__ logits, long long rs, const long long* __restrict__ tokens, int rows, int V, int top,
+                   float* __restrict__ logp, float* __restrict__ entropy, float2* __restrict__ stats,
+                   float* __restrict__ top_logp, long long* __restrict__ top_ids) {
+  using G = Group<NT>;
+  constexpr int N = Vec<T>::N, K = 4;
+  __shared__ Shared<NT> shared[G::ROWS];
+  Shared<NT>& sh = shared[threadIdx.x / NT];
+  const int t = threadIdx.x % NT, lane = t & 31, warp = t >> 5;
+  const long long step = (long long)gridDim.x * G::ROWS;
+  long long row = (long long)blockIdx.x * G::ROWS + threadIdx.x / NT;
+  if (row >= rows) return;                                    // a whole group leaves
   const T* x = logits + row * rs;
-  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  const Cut c = cut_row(x, V);
-  Run r{-INFINITY, 0.f, 0.f};
-  auto single = [&](float v) {
-    if (v > r.m) r.raise(v);
-    if (v != -INFINITY) r.add(v);                     // -inf adds nothing; NaN and +inf make the sums NaN
+  Cut c = cut_row(x, V);
+  // two sets of K vectors are in flight: vectors t + NT k of the body, k = 0 .. K - 1 and K .. 2 K - 1, then on
+  uint4 a[K], b[K];
+  auto fetch = [&](uint4 (&u)[K], const T* xr, const Cut& cr, int i) {
+    const uint4* body = reinterpret_cast<const uint4*>(xr + cr.head);
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (i + k * NT < cr.nvec) u[k] = load_stream(body + i + k * NT);
   };
-  if (t < c.head) single(Vec<T>::one(x[t]));
-  if (c.tail0 + t < V) single(Vec<T>::one(x[c.tail0 + t]));
-  const uint4* body = reinterpret_cast<const uint4*>(x + c.head);
-  for (int i = t; i < c.nvec; i += NT * U) {
-    uint4 u[U];
+  // everything that a row's sums wait for is requested a row ahead
+  T edge0 = T(), edge1 = T();                                 // this thread's entry before and behind the vectors
+  long long y = 0;
+  auto fetch_first = [&](const T* xr, const Cut& cr, long long r) {
+    fetch(a, xr, cr, t);
+    fetch(b, xr, cr, t + K * NT);
+    if (t < cr.head) edge0 = xr[t];
+    if (cr.tail0 + t < V) edge1 = xr[cr.tail0 + t];
+    y = tokens[r];
+  };
+  fetch_first(x, c, row);
+  for (;;) {
+    Run r{-INFINITY, 0.f, 0.f};
+    const long long target = y;
+    if (t < c.head) r.one(Vec<T>::one(edge0));
+    if (c.tail0 + t < V) r.one(Vec<T>::one(edge1));
+    for (int i = t; i < c.nvec; i += 2 * K * NT) {
+      r.template many<T, K>(a, min(K, (c.nvec - i + NT - 1) / NT));
+      fetch(a, x, c, i + 2 * K * NT);
+      if (i + K * NT < c.nvec) r.template many<T, K>(b, min(K, (c.nvec - i - K * NT + NT - 1) / NT));
+      fetch(b, x, c, i + 3 * K * NT);
+    }
+    // the next row's first vectors travel while this row's sums are joined
+    const long long next = row + step;
+    const T* xn = logits + next * rs;
+    Cut cn = c;
+    if (next < rows) {
+      cn = cut_row(xn, V);
+      fetch_first(xn, cn, next);
+    }
+    float xy = 0.f;
+    if (t == 0 && target >= 0 && target < V) xy = Vec<T>::one(x[target]);
+    // ---- the row's sums: within the warp, then across warps ----
+    const float own = r.m;
+    if (TOP) {                                                // maxima of the groups of NT / 32 threads
+      float part = own;
 #pragma unroll
-    for (int k = 0; k < U; ++k)
-      if (i + k * NT < c.nvec) u[k] = __ldg(body + i + k * NT);
+      for (int o = 1; o < NT / 32; o <<= 1) part = fmaxf(part, __shfl_xor_sync(0xffffffffu, part, o));
+      if (t % (NT / 32) == 0) sh.part[t / (NT / 32)] = part;
+    }
+    auto join = [&](float& m, float& s, float& e, int width) {
+      float top_m = m;
 #pragma unroll
-    for (int k = 0; k < U; ++k) {
-      if (i + k * NT < c.nvec) {
-        float v[N];
-        Vec<T>::get(u[k], v);
-        float mx = v[0];
+      for (int o = width / 2; o > 0; o >>= 1) top_m = fmaxf(top_m, __shfl_xor_sync(0xffffffffu, top_m, o));
+      if (top_m != -INFINITY) {
+        const float d = m - top_m, f = ex2(d * L2E);
+        e = f * fmaf(fmaxf(d, LOWEST), s, e);
+        s *= f;
+      }
+      m = top_m;
 #pragma unroll
-        for (int q = 1; q < N; ++q) mx = fmaxf(mx, v[q]);
-        if (mx > r.m) r.raise(mx);
-        if (r.m != -INFINITY) {
+      for (int o = width / 2; o > 0; o >>= 1) {
+        s += __shfl_xor_sync(0xffffffffu, s, o);
+        e += __shfl_xor_sync(0xffffffffu, e, o);
+      }
+    };
+    join(r.m, r.s, r.e, 32);
+    if (G::WARPS > 1) {
+      if (lane == 0) { sh.m[warp] = r.m; sh.s[warp] = r.s; sh.e[warp] = r.e; }
+      if (t == 0) sh.n = 0;
+      G::sync();
+      r = Run{sh.m[lane % G::WARPS], sh.s[lane % G::WARPS], sh.e[lane % G::WARPS]};
+      join(r.m, r.s, r.e, G::WARPS);                          // every warp for itself, the same bits in all
+    } else {
+      if (t == 0) sh.n = 0;
+      G::sync();
+    }
+    const float ls = logf(r.s);
+    if (t == 0) {
+      logp[row] = target < 0 ? 0.f : target < V ? (xy - r.m) - ls : NAN;
+      entropy[row] = ls - r.e / r.s;
+      if (stats) stats[row] = make_float2(r.m, ls);
+    }
+    // ---- alternatives ----
+    if (TOP) {
+      const float v0 = sh.part[lane];                         // every warp ranks the 32 maxima
+      int rank0 = 0;
 #pragma unroll
-          for (int q = 0; q < N; ++q) r.add(v[q]);
-        } else {
+      for (int i = 0; i < 32; ++i) rank0 += ahead(__shfl_sync(0xffffffffu, v0, i), i, v0, lane);
+      const float bound = __shfl_sync(0xffffffffu, v0, __ffs(__ballot_sync(0xffffffffu, rank0 == top - 1)) - 1);
+      auto each_own = [&](auto f) {                           // this thread's entries, each with its index
+        if (t < c.head) f(Vec<T>::one(x[t]), t);
+        const uint4* body = reinterpret_cast<const uint4*>(x + c.head);
+#pragma unroll 4
+        for (int i = t; i < c.nvec; i += NT) {
+          float v[N];
+          Vec<T>::get(__ldg(body + i), v);
 #pragma unroll
-          for (int q = 0; q < N; ++q)
-            if (v[q] != v[q]) r.s = v[q];             // nothing but -inf and NaN so far
+          for (int k = 0; k < N; ++k) f(v[k], c.head + i * N + k);
+        }
+        if (c.tail0 + t < V) f(Vec<T>::one(x[c.tail0 + t]), c.tail0 + t);
+      };
+      auto offer = [&](float v, int i) {
+        if (!(v < bound)) {                                   // NaN goes in as well: it is ranked as the smallest
+          const int at = atomicAdd(&sh.n, 1);                 // the list's order does not matter: it is ranked
+          if (at < G::CAP) { sh.cv[at] = v == v ? v : -INFINITY; sh.ci[at] = i; }
+        }
+      };
+      if (NT == 32) {
+        if (!(own < bound)) each_own(offer);
+      } else {
+        // the warp looks at one such thread's entries together: one latency instead of one per vector
+        for (unsigned todo = __ballot_sync(0xffffffffu, !(own < bound)); todo; todo &= todo - 1) {
+          const int tt = warp * 32 + __ffs(todo) - 1;
+          const uint4* body = reinterpret_cast<const uint4*>(x + c.head);
+          for (int i = tt + NT * lane; i < c.nvec; i += NT * 32) {
+            float v[N];
+            Vec<T>::get(__ldg(body + i), v);
+#pragma unroll
+            for (int k = 0; k < N; ++k) offer(v[k], c.head + i * N + k);
+          }
+          if (lane == 0 && tt < c.head) offer(Vec<T>::one(x[tt]), tt);
+          if (lane == 1 && c.tail0 + tt < V) offer(Vec<T>::one(x[c.tail0 + tt]), c.tail0 + tt);
+        }
+      }
+      G::sync();
+      const int n = sh.n;
+      if (n <= G::CAP) {
+        for (int q = t; q < n; q += NT) {
+          const float v = sh.cv[q];
+          const int i = sh.ci[q];
+          int rank = 0;
+          for (int w = 0; w < n; ++w) rank += ahead(sh.cv[w], sh.ci[w], v, i);
+          if (rank < top) {
+            top_logp[row * top + rank] = (v - r.m) - ls;
+            top_ids[row * top + rank] = i;
+          }
+        }
+      } else {
+        // more ties than the list holds (a constant row, a row masked down to a few entries): one entry at a time, each the
+        // best behind the one before it
+        float pv = INFINITY;
+        int pi = -1;
+        for (int k = 0; k < top; ++k) {
+          float bv = -INFINITY;
+          int bi = V;
+          each_own([&](float v, int i) {
+            if (v != v) v = -INFINITY;
+            if (ahead(pv, pi, v, i) && ahead(v, i, bv, bi)) { bv = v; bi = i; }
+          });
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) {
+            const float v2 = __shfl_xor_sync(0xffffffffu, bv, o);
+            const int i2 = __shfl_xor_sync(0xffffffffu, bi, o);
+            if (ahead(v2, i2, bv, bi)) { bv = v2; bi = i2; }
+          }
+          G::sync();
+          if (lane == 0) { sh.cv[warp] = bv; sh.ci[warp] = bi; }
+          G::sync();
+          pv = sh.cv[0];
+          pi = sh.ci[0];
+          for (int w = 1; w < G::WARPS; ++w)
+            if (ahead(sh.cv[w], sh.ci[w], pv, pi)) { pv = sh.cv[w]; pi = sh.ci[w]; }
+          if (t == 0) {
+            top_logp[row * top + k] = (pv - r.m) - ls;
+            top_ids[row * top + k] = pi;
+          }
         }
       }
     }
-  }
-  // ---- the block's sums ----
-  __shared__ float sm[8], ss[8], se[8];
-  __shared__ float s_m, s_ls;
-  const float own = r.m;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float m2 = __shfl_xor_sync(0xffffffffu, r.m, o), s2 = __shfl_xor_sync(0xffffffffu, r.s, o),
-                e2 = __shfl_xor_sync(0xffffffffu, r.e, o);
-    // the same order of terms in both partners
-    const bool low = (lane & o) == 0;
-    Run z = low ? r : Run{m2, s2, e2};
-    const float ms = low ? m2 : r.m, sx = low ? s2 : r.s, ex = low ? e2 : r.e;
-    const bool dead = z.m == -INFINITY && ms == -INFINITY;
-    z.join(ms, sx, ex);
-    if (dead) z.s += sx;                              // NaN of a thread that saw nothing else
-    r = z;
-  }
-  if (lane == 0) { sm[warp] = r.m; ss[warp] = r.s; se[warp] = r.e; }
-  __shared__ float g_max[GROUPS];                     // maxima of the groups of 8 threads
-  if (TOP) {
-    float gm = own;
-    gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, 1));
-    gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, 2));
-    gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, 4));
-    if ((t & 7) == 0) g_max[t >> 3] = gm;
-  }
-  __shared__ float s_bound;
-  __shared__ int s_n;
-  __syncthreads();
-  if (t == 0) {
-    Run z{sm[0], ss[0], se[0]};
-#pragma unroll
-    for (int w = 1; w < NT / 32; ++w) {
-      const bool dead = z.m == -INFINITY && sm[w] == -INFINITY;
-      z.join(sm[w], ss[w], se[w]);
-      if (dead) z.s += ss[w];
-    }
-    const float ls = logf(z.s);
-    const long long y = tokens[row];
-    float lp = 0.f;
-    if (y >= 0) lp = y < V ? (Vec<T>::one(x[y]) - z.m) - ls : NAN;
-    logp[row] = lp;
-    entropy[row] = ls - z.e / z.s;
-    if (stats) stats[row] = make_float2(z.m, ls);
-    s_m = z.m;
-    s_ls = ls;
-    s_n = 0;
-  }
-  if (!TOP) return;
-  // ---- alternatives ----
-  __shared__ float cv[CAP];
-  __shared__ int ci[CAP];
-  if (warp == 1) {                                    // the top-th largest of the group maxima
-    const float v = g_max[lane];
-    int rank = 0;
-#pragma unroll
-    for (int i = 0; i < GROUPS; ++i) rank += ahead(g_max[i], i, v, lane);
-    if (rank == top - 1) s_bound = v;
-  }
-  __syncthreads();
-  const float bound = s_bound;
-  if (!(own < bound))
-    each_own(x, c, V, [&](float v, int i) {
-      if (!(v < bound)) {                             // NaN goes in as well: it is ranked as the smallest
-        const int at = atomicAdd(&s_n, 1);
-        if (at < CAP) { cv[at] = v == v ? v : -INFINITY; ci[at] = i; }
-      }
-    });
-  __syncthreads();
-  const int n = s_n;
-  if (n <= CAP) {
-    for (int a = t; a < n; a += NT) {
-      const float v = cv[a];
-      const int i = ci[a];
-      int rank = 0;
-      for (int b = 0; b < n; ++b) rank += ahead(cv[b], ci[b], v, i);
-      if (rank < top) {
-        top_logp[row * top + rank] = (v - s_m) - s_ls;
-        top_ids[row * top + rank] = i;
-      }
-    }
-    return;
-  }
-  // more ties than the list holds (a constant row, a row masked down to a few entries): one entry at a time, each the
-  // best behind the one before it
-  float pv = INFINITY;
-  int pi = -1;
-  for (int k = 0; k < top; ++k) {
-    float bv = -INFINITY;
-    int bi = V;
-    each_own(x, c, V, [&](float v, int i) {
-      if (v != v) v = -INFINITY;
-      if (ahead(pv, pi, v, i) && ahead(v, i, bv, bi)) { bv = v; bi = i; }
-    });
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const float v2 = __shfl_xor_sync(0xffffffffu, bv, o);
-      const int i2 = __shfl_xor_sync(0xffffffffu, bi, o);
-      if (ahead(v2, i2, bv, bi)) { bv = v2; bi = i2; }
-    }
-    __syncthreads();
-    if (lane == 0) { cv[warp] = bv; ci[warp] = bi; }
-    __syncthreads();
-    pv = cv[0];
-    pi = ci[0];
-    for (int w = 1; w < NT / 32; ++w)
-      if (ahead(cv[w], ci[w], pv, pi)) { pv = cv[w]; pi = ci[w]; }
-    if (t == 0) {
-      top_logp[row * top + k] = (pv - s_m) - s_ls;
-      top_ids[row * top + k] = pi;
-    }
+    if (next >= rows) return;
+    G::sync();                                                // the shared words are free
+    row = next;
+    x = xn;
+    c = cn;
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(NT) logprob_bwd_kernel(const T* __restrict__ logits, long long rs,
-                                                         const long long* __restrict__ tokens, int V,
+template <int NT, typename T>
+__global__ void __launch_bounds__(Group<NT>::BLOCK) logprob_bwd_kernel(const T* __restrict__ logits, long long rs,
+                                                         const long long* __restrict__ tokens, int rows, int V,
                                                          const float2* __restrict__ stats, const float* __restrict__ entropy,
                                                          const float* __restrict__ g_logp, const float* __restrict__ g_ent,
                                                          T* __restrict__ dx) {
   constexpr int N = Vec<T>::N;
-  const long long row = blockIdx.x;
+  const long long row = (long long)blockIdx.x * Group<NT>::ROWS + threadIdx.x / NT;
+  if (row >= rows) return;
   const T* x = logits + row * rs;
   T* out = dx + row * V;
-  const int t = threadIdx.x;
+  const int t = threadIdx.x % NT;
   const long long y = tokens[row];
   const float2 st = stats[row];
   const float gh = g_ent ? g_ent[row] : 0.f, gl = g_logp && y >= 0 ? (y < V ? g_logp[row] : NAN) : 0.f;
@@ -357,22 +446,40 @@ __global__ void __launch_bounds__(NT) logprob_bwd_kernel(const T* __restrict__ l
   }
 }
 
-template <typename T>
-int fwd(const void* x, long long rs, const long long* tok, long long rows, int V, int top, float* lp, float* ent, float2* st,
-        float* tlp, long long* tid, cudaStream_t s) {
-  if (top > 0)
-    logprob_fwd_kernel<T, true><<<(unsigned)rows, NT, 0, s>>>((const T*)x, rs, tok, V, top, lp, ent, st, tlp, tid);
-  else
-    logprob_fwd_kernel<T, false><<<(unsigned)rows, NT, 0, s>>>((const T*)x, rs, tok, V, top, lp, ent, st, tlp, tid);
+template <int NT, typename T>
+int fwd_nt(const T* x, long long rs, const long long* tok, int rows, int V, int top, float* lp, float* ent, float2* st, float* tlp,
+           long long* tid, int blocks, cudaStream_t s) {
+  using G = Group<NT>;
+  const int grid = min((rows + G::ROWS - 1) / G::ROWS, blocks);
+  if (top > 0) logprob_fwd_kernel<NT, T, true><<<grid, G::BLOCK, 0, s>>>(x, rs, tok, rows, V, top, lp, ent, st, tlp, tid);
+  else logprob_fwd_kernel<NT, T, false><<<grid, G::BLOCK, 0, s>>>(x, rs, tok, rows, V, top, lp, ent, st, tlp, tid);
   DMB_CHECK_LAUNCH();
   return 0;
 }
 template <typename T>
-int bwd(const void* x, long long rs, const long long* tok, long long rows, int V, const float2* st, const float* ent,
-        const float* gl, const float* gh, void* dx, cudaStream_t s) {
-  logprob_bwd_kernel<T><<<(unsigned)rows, NT, 0, s>>>((const T*)x, rs, tok, V, st, ent, gl, gh, (T*)dx);
+int fwd(const void* xv, long long rs, const long long* tok, int rows, int V, int top, float* lp, float* ent, float2* st,
+        float* tlp, long long* tid, cudaStream_t s) {
+  const T* x = (const T*)xv;
+  // blocks for 148 SMs: 4 of 256 threads, 1 of 1024 on each
+  if (V <= 2048) return fwd_nt<32>(x, rs, tok, rows, V, top, lp, ent, st, tlp, tid, 4 * 148, s);
+  if (rows <= 148) return fwd_nt<1024>(x, rs, tok, rows, V, top, lp, ent, st, tlp, tid, 148, s);
+  return fwd_nt<256>(x, rs, tok, rows, V, top, lp, ent, st, tlp, tid, 4 * 148, s);
+}
+template <int NT, typename T>
+int bwd_nt(const T* x, long long rs, const long long* tok, int rows, int V, const float2* st, const float* ent, const float* gl,
+           const float* gh, T* dx, cudaStream_t s) {
+  using G = Group<NT>;
+  logprob_bwd_kernel<NT, T><<<(rows + G::ROWS - 1) / G::ROWS, G::BLOCK, 0, s>>>(x, rs, tok, rows, V, st, ent, gl, gh, dx);
   DMB_CHECK_LAUNCH();
   return 0;
+}
+template <typename T>
+int bwd(const void* xv, long long rs, const long long* tok, int rows, int V, const float2* st, const float* ent,
+        const float* gl, const float* gh, void* dx, cudaStream_t s) {
+  const T* x = (const T*)xv;
+  if (V <= 2048) return bwd_nt<32>(x, rs, tok, rows, V, st, ent, gl, gh, (T*)dx, s);
+  if (rows <= 148) return bwd_nt<1024>(x, rs, tok, rows, V, st, ent, gl, gh, (T*)dx, s);
+  return bwd_nt<256>(x, rs, tok, rows, V, st, ent, gl, gh, (T*)dx, s);
 }
 
 }  // namespace
@@ -385,9 +492,9 @@ extern "C" int dmb_logprob_fwd(const void* x, long long rs, const long long* tok
   if (V <= 0 || rows > 0x7fffffffLL || top < 0 || top > MAX_TOP || top > V) return -1;
   cudaStream_t s = (cudaStream_t)stream;
   float2* st = (float2*)stats;
-  if (type == 0) return fwd<float>(x, rs, tokens, rows, V, top, logp, entropy, st, top_logp, top_ids, s);
-  if (type == 1) return fwd<bf16>(x, rs, tokens, rows, V, top, logp, entropy, st, top_logp, top_ids, s);
-  if (type == 2) return fwd<__half>(x, rs, tokens, rows, V, top, logp, entropy, st, top_logp, top_ids, s);
+  if (type == 0) return fwd<float>(x, rs, tokens, (int)rows, V, top, logp, entropy, st, top_logp, top_ids, s);
+  if (type == 1) return fwd<bf16>(x, rs, tokens, (int)rows, V, top, logp, entropy, st, top_logp, top_ids, s);
+  if (type == 2) return fwd<__half>(x, rs, tokens, (int)rows, V, top, logp, entropy, st, top_logp, top_ids, s);
   return -1;
 }
 // dx [rows, V] dense; g_logp / g_entropy fp32 [rows] or null (no gradient through that output)
@@ -398,8 +505,8 @@ extern "C" int dmb_logprob_bwd(const void* x, long long rs, const long long* tok
   if (V <= 0 || rows > 0x7fffffffLL) return -1;
   cudaStream_t s = (cudaStream_t)stream;
   const float2* st = (const float2*)stats;
-  if (type == 0) return bwd<float>(x, rs, tokens, rows, V, st, entropy, g_logp, g_entropy, dx, s);
-  if (type == 1) return bwd<bf16>(x, rs, tokens, rows, V, st, entropy, g_logp, g_entropy, dx, s);
-  if (type == 2) return bwd<__half>(x, rs, tokens, rows, V, st, entropy, g_logp, g_entropy, dx, s);
+  if (type == 0) return bwd<float>(x, rs, tokens, (int)rows, V, st, entropy, g_logp, g_entropy, dx, s);
+  if (type == 1) return bwd<bf16>(x, rs, tokens, (int)rows, V, st, entropy, g_logp, g_entropy, dx, s);
+  if (type == 2) return bwd<__half>(x, rs, tokens, (int)rows, V, st, entropy, g_logp, g_entropy, dx, s);
   return -1;
 }
