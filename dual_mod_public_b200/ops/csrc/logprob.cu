@@ -6,8 +6,8 @@
 // Both passes stream the row once with 16-byte loads and are bound by DRAM.  Forward: a group of threads per row (a warp, 256
 // or 1024 threads, see `fwd`), two sets of loads in flight per thread, running maximum and sums per thread (fp32; a thread adds
 // its part of the row, the rest is a tree), so nothing of the row is kept.  A block takes rows in turn and requests the next
-// row's first part before it joins the sums of the last.  Differences to the maximum are formed before they are scaled: a row
-// whose entries all are the type's lowest value is uniform, as it should be.
+// row's first part before it joins the sums of the last.  A row whose entries all are the type's lowest value is uniform, as it
+// should be.
 // Alternatives: the maxima of 32 parts of the row are entries of it, so the top-th largest of them bounds the top-th largest
 // entry from below; only threads whose own maximum reaches the bound look at their entries again (from L2), and what reaches
 // the bound, a few entries more than `top`, is ranked by (value, lower index first).
@@ -17,7 +17,7 @@
 namespace {
 
 constexpr int MAX_TOP = 32;
-constexpr float L2E = 1.4426950408889634f;
+constexpr float L2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 // exp of anything below this is zero in fp32; keeps 0 x (-inf) out of the sums
 constexpr float LOWEST = -200.f;
 
@@ -104,22 +104,31 @@ __device__ __forceinline__ Cut cut_row(const T* x, int V) {
   return {head, nvec, head + nvec * Vec<T>::N};
 }
 
-// running maximum, sum of exp(x - m) and sum of exp(x - m) (x - m)
+// Running maximum m, s = sum of 2^y and e = sum of 2^y y with y = x log2(e) - ref, ref the whole number above m log2(e): the
+// product and the difference are one rounding of a small value, and moving ref scales the sums by an exact power of two.
+// Where |m| is huge (a row of the type's lowest value, infinities) differences are formed first and ref is not used.
 struct Run {
-  float m, s, e;
-  __device__ __forceinline__ void raise(float top) {          // move the reference to `top` > m
-    const float d = m - top;                                  // -inf the first time
-    const float f = ex2(d * L2E);
-    e = f * fmaf(fmaxf(d, LOWEST), s, e);
-    s *= f;
+  float m, ref, s, e;
+  static __device__ __forceinline__ bool plain(float v) { return fabsf(v) < 1e30f; }
+  __device__ __forceinline__ void raise(float top) {          // `top` > m
+    if (plain(m) && plain(top)) {
+      const float r = ceilf(top * L2E), k = ref - r, f = ex2(k);
+      e = f * fmaf(k, s, e);
+      s *= f;
+      ref = r;
+    } else {                                                  // nothing so far, or nothing that counts beside `top` (NaN stays)
+      s *= 0.f;
+      e *= 0.f;
+      ref = plain(top) ? ceilf(top * L2E) : 0.f;
+    }
     m = top;
   }
   __device__ __forceinline__ void one(float v) {
     if (v > m) raise(v);
     if (v == -INFINITY) return;                               // adds nothing, also where m is -inf
-    const float d = v - m, p = ex2(d * L2E);
+    const float y = plain(m) ? fmaf(v, L2E, -ref) : (v - m) * L2E, p = ex2(y);
     s += p;
-    e = fmaf(p, fmaxf(d, LOWEST), e);
+    e = fmaf(p, fmaxf(y, LOWEST), e);
   }
   // K vectors at once; `live` of them count
   template <typename T, int K>
@@ -130,33 +139,30 @@ struct Run {
     for (int k = 0; k < K; ++k)
       if (k < live) top = fmaxf(top, Vec<T>::top(u[k]));
     if (top > m) raise(top);
-    const packed::f32x2 nm = packed::pair(-m, -m), l2 = packed::pair(L2E, L2E);
-    packed::f32x2 s2 = packed::pair(0.f, 0.f), e2 = packed::pair(0.f, 0.f);
+    if (plain(m)) {
+      float s0 = 0.f, s1 = 0.f, e0 = 0.f, e1 = 0.f;
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-      if (k < live) {
-        float v[N];
-        Vec<T>::get(u[k], v);
+      for (int k = 0; k < K; ++k)
+        if (k < live) {
+          float v[N];
+          Vec<T>::get(u[k], v);
 #pragma unroll
-        for (int i = 0; i < N; i += 2) {
-          const packed::f32x2 d = packed::add2(packed::pair(v[i], v[i + 1]), nm), y = packed::mul2(d, l2);
-          float y0, y1;
-          packed::split(y, y0, y1);
-          const packed::f32x2 p = packed::pair(ex2(y0), ex2(y1));
-          s2 = packed::add2(s2, p);
-          e2 = packed::fma2(p, d, e2);
+          for (int i = 0; i < N; i += 2) {
+            const float y0 = fmaf(v[i], L2E, -ref), y1 = fmaf(v[i + 1], L2E, -ref), p0 = ex2(y0), p1 = ex2(y1);
+            s0 += p0;
+            s1 += p1;
+            e0 = fmaf(p0, y0, e0);
+            e1 = fmaf(p1, y1, e1);
+          }
         }
+      if (e0 + e1 == e0 + e1) {
+        s += s0 + s1;
+        e += e0 + e1;
+        return;
       }
-    float s0, s1, e0, e1;
-    packed::split(s2, s0, s1);
-    packed::split(e2, e0, e1);
-    if (e0 + e1 == e0 + e1) {
-      s += s0 + s1;
-      e += e0 + e1;
-      return;
     }
 #pragma unroll 1
-    for (int k = 0; k < K; ++k) {                             // -inf among them (0 x inf above), or NaN: one by one
+    for (int k = 0; k < K; ++k) {                             // -inf among them (0 x inf above), NaN, huge values: one by one
       uint4 w = u[0];
 #pragma unroll
       for (int q = 1; q < K; ++q)
@@ -168,6 +174,12 @@ struct Run {
         if (k < live) one(v[i]);
     }
   }
+  // the sums relative to m itself, e in natural units
+  __device__ __forceinline__ void finish() {
+    const float t = plain(m) ? fmaf(m, L2E, -ref) : 0.f, f = ex2(-t);
+    e = f * LN2 * fmaf(-t, s, e);
+    s *= f;
+  }
 };
 
 __device__ __forceinline__ bool ahead(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
@@ -178,10 +190,11 @@ __device__ __forceinline__ uint4 load_stream(const uint4* p) {
   return v;
 }
 
-// A group of NT threads per row; blocks of max(NT, 256) threads.
+// A group of NT threads per row; a block is a group, or eight warps with a row each.
 template <int NT>
 struct Group {
-  static constexpr int BLOCK = NT < 256 ? 256 : NT, ROWS = BLOCK / NT, WARPS = NT / 32;
+  static constexpr int BLOCK = NT == 32 ? 256 : NT, ROWS = BLOCK / NT, WARPS = NT / 32;
+  static constexpr int BLOCKS = 1024 / BLOCK;                 // on an SM: 64 registers a thread
   static constexpr int CAP = NT == 32 ? 96 : 1024;            // candidates that a list holds
   static __device__ __forceinline__ void sync() {
     if (NT == 32) __syncwarp(); else __syncthreads();
@@ -196,7 +209,7 @@ struct Shared {                                               // of one group
 };
 
 template <int NT, typename T, bool TOP>
-__global__ void __launch_bounds__(Group<NT>::BLOCK, NT == 1024 ? 1 : 4)
+__global__ void __launch_bounds__(Group<NT>::BLOCK, Group<NT>::BLOCKS)
 logprob_fwd_kernel(const T* __restrict__ logits, long long rs, const long long* __restrict__ tokens, int rows, int V, int top,
                    float* __restrict__ logp, float* __restrict__ entropy, float2* __restrict__ stats,
                    float* __restrict__ top_logp, long long* __restrict__ top_ids) {
@@ -230,7 +243,7 @@ logprob_fwd_kernel(const T* __restrict__ logits, long long rs, const long long* 
   };
   fetch_first(x, c, row);
   for (;;) {
-    Run r{-INFINITY, 0.f, 0.f};
+    Run r{-INFINITY, 0.f, 0.f, 0.f};
     const long long target = y;
     if (t < c.head) r.one(Vec<T>::one(edge0));
     if (c.tail0 + t < V) r.one(Vec<T>::one(edge1));
@@ -274,12 +287,13 @@ logprob_fwd_kernel(const T* __restrict__ logits, long long rs, const long long* 
         e += __shfl_xor_sync(0xffffffffu, e, o);
       }
     };
+    r.finish();
     join(r.m, r.s, r.e, 32);
     if (G::WARPS > 1) {
       if (lane == 0) { sh.m[warp] = r.m; sh.s[warp] = r.s; sh.e[warp] = r.e; }
       if (t == 0) sh.n = 0;
       G::sync();
-      r = Run{sh.m[lane % G::WARPS], sh.s[lane % G::WARPS], sh.e[lane % G::WARPS]};
+      r = Run{sh.m[lane % G::WARPS], 0.f, sh.s[lane % G::WARPS], sh.e[lane % G::WARPS]};
       join(r.m, r.s, r.e, G::WARPS);                          // every warp for itself, the same bits in all
     } else {
       if (t == 0) sh.n = 0;
@@ -293,11 +307,14 @@ logprob_fwd_kernel(const T* __restrict__ logits, long long rs, const long long* 
     }
     // ---- alternatives ----
     if (TOP) {
-      const float v0 = sh.part[lane];                         // every warp ranks the 32 maxima
-      int rank0 = 0;
+      float bound = r.m;
+      if (top > 1) {
+        const float v0 = sh.part[lane];                       // every warp ranks the 32 maxima
+        int rank0 = 0;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) rank0 += ahead(__shfl_sync(0xffffffffu, v0, i), i, v0, lane);
-      const float bound = __shfl_sync(0xffffffffu, v0, __ffs(__ballot_sync(0xffffffffu, rank0 == top - 1)) - 1);
+        for (int i = 0; i < 32; ++i) rank0 += ahead(__shfl_sync(0xffffffffu, v0, i), i, v0, lane);
+        bound = __shfl_sync(0xffffffffu, v0, __ffs(__ballot_sync(0xffffffffu, rank0 == top - 1)) - 1);
+      }
       auto each_own = [&](auto f) {                           // this thread's entries, each with its index
         if (t < c.head) f(Vec<T>::one(x[t]), t);
         const uint4* body = reinterpret_cast<const uint4*>(x + c.head);
@@ -391,7 +408,7 @@ __global__ void __launch_bounds__(Group<NT>::BLOCK) logprob_bwd_kernel(const T* 
                                                          const long long* __restrict__ tokens, int rows, int V,
                                                          const float2* __restrict__ stats, const float* __restrict__ entropy,
                                                          const float* __restrict__ g_logp, const float* __restrict__ g_ent,
-                                                         T* __restrict__ dx) {
+                                                         T* __restrict__ dx, int part) {
   constexpr int N = Vec<T>::N;
   const long long row = (long long)blockIdx.x * Group<NT>::ROWS + threadIdx.x / NT;
   if (row >= rows) return;
@@ -409,24 +426,27 @@ __global__ void __launch_bounds__(Group<NT>::BLOCK) logprob_bwd_kernel(const T* 
   };
   // the output row is aligned like the input row or not: vectors where both are, else one by one
   const Cut c = cut_row(x, V);
+  const int v_begin = blockIdx.y * part, v_end = min(c.nvec, v_begin + part);        // this block's vectors
   const bool same = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
   auto single = [&](int i) {
     const float g = grad(Vec<T>::one(x[i]));
     out[i] = Vec<T>::from(i == yi ? g + gl : g);
   };
-  if (t < c.head) single(t);
-  if (c.tail0 + t < V) single(c.tail0 + t);
+  if (blockIdx.y == 0) {
+    if (t < c.head) single(t);
+    if (c.tail0 + t < V) single(c.tail0 + t);
+  }
   const uint4* body = reinterpret_cast<const uint4*>(x + c.head);
   constexpr int UB = 4;
-  for (int i = t; i < c.nvec; i += NT * UB) {
+  for (int i = v_begin + t; i < v_end; i += NT * UB) {
     uint4 u[UB];
 #pragma unroll
     for (int k = 0; k < UB; ++k)
-      if (i + k * NT < c.nvec) u[k] = __ldg(body + i + k * NT);
+      if (i + k * NT < v_end) u[k] = load_stream(body + i + k * NT);
 #pragma unroll
     for (int k = 0; k < UB; ++k) {
       const int j = i + k * NT;
-      if (j < c.nvec) {
+      if (j < v_end) {
         float v[N];
         Vec<T>::get(u[k], v);
         const int e0 = c.head + j * N;
@@ -446,30 +466,41 @@ __global__ void __launch_bounds__(Group<NT>::BLOCK) logprob_bwd_kernel(const T* 
   }
 }
 
+constexpr int SMS = 148;
+
 template <int NT, typename T>
 int fwd_nt(const T* x, long long rs, const long long* tok, int rows, int V, int top, float* lp, float* ent, float2* st, float* tlp,
-           long long* tid, int blocks, cudaStream_t s) {
+           long long* tid, cudaStream_t s) {
   using G = Group<NT>;
-  const int grid = min((rows + G::ROWS - 1) / G::ROWS, blocks);
+  // as many blocks as are resident (sharing the rows out evenly over fewer blocks was slower: 108 against 102 us)
+  const int grid = min((rows - 1) / G::ROWS + 1, SMS * G::BLOCKS);
   if (top > 0) logprob_fwd_kernel<NT, T, true><<<grid, G::BLOCK, 0, s>>>(x, rs, tok, rows, V, top, lp, ent, st, tlp, tid);
   else logprob_fwd_kernel<NT, T, false><<<grid, G::BLOCK, 0, s>>>(x, rs, tok, rows, V, top, lp, ent, st, tlp, tid);
   DMB_CHECK_LAUNCH();
   return 0;
 }
+// Threads per row.  Few threads: little to join per row; many: a row alone goes fast.  A warp where a row is short (16384 x 259:
+// 27 us against 420 with 256 threads); 1024 where every row has an SM to itself; between them as few as keep two rounds of
+// rows (8191 x 32000 bf16: 64 threads 102, 128 108, 256 113 us; 1021 x 50257 fp32: 128 61, 256 53 us).  Ranking alternatives
+// wants more of them (8191 x 32000, top 8: 64 176, 128 152, 256 172 us).
 template <typename T>
 int fwd(const void* xv, long long rs, const long long* tok, int rows, int V, int top, float* lp, float* ent, float2* st,
         float* tlp, long long* tid, cudaStream_t s) {
   const T* x = (const T*)xv;
-  // blocks for 148 SMs: 4 of 256 threads, 1 of 1024 on each
-  if (V <= 2048) return fwd_nt<32>(x, rs, tok, rows, V, top, lp, ent, st, tlp, tid, 4 * 148, s);
-  if (rows <= 148) return fwd_nt<1024>(x, rs, tok, rows, V, top, lp, ent, st, tlp, tid, 148, s);
-  return fwd_nt<256>(x, rs, tok, rows, V, top, lp, ent, st, tlp, tid, 4 * 148, s);
+  if (V <= 2048) return fwd_nt<32>(x, rs, tok, rows, V, top, lp, ent, st, tlp, tid, s);
+  if (rows <= SMS) return fwd_nt<1024>(x, rs, tok, rows, V, top, lp, ent, st, tlp, tid, s);
+  if (top <= 1 && rows >= 2 * 16 * SMS) return fwd_nt<64>(x, rs, tok, rows, V, top, lp, ent, st, tlp, tid, s);
+  if (rows >= 2 * 8 * SMS) return fwd_nt<128>(x, rs, tok, rows, V, top, lp, ent, st, tlp, tid, s);
+  return fwd_nt<256>(x, rs, tok, rows, V, top, lp, ent, st, tlp, tid, s);
 }
 template <int NT, typename T>
 int bwd_nt(const T* x, long long rs, const long long* tok, int rows, int V, const float2* st, const float* ent, const float* gl,
            const float* gh, T* dx, cudaStream_t s) {
   using G = Group<NT>;
-  logprob_bwd_kernel<NT, T><<<(rows + G::ROWS - 1) / G::ROWS, G::BLOCK, 0, s>>>(x, rs, tok, rows, V, st, ent, gl, gh, dx);
+  // few rows: a row in parts of 2048 vectors (1021 x 50257 fp32: 74 against 82 us); many: whole rows (8191 x 32000 bf16: 169
+  // against 178 us)
+  const int nvec = V / Vec<T>::N + 1, part = rows < 4 * 8 * SMS ? 2048 : nvec, parts = (nvec - 1) / part + 1;
+  logprob_bwd_kernel<NT, T><<<dim3((rows - 1) / G::ROWS + 1, parts), G::BLOCK, 0, s>>>(x, rs, tok, rows, V, st, ent, gl, gh, dx, part);
   DMB_CHECK_LAUNCH();
   return 0;
 }
@@ -478,7 +509,6 @@ int bwd(const void* xv, long long rs, const long long* tok, int rows, int V, con
         const float* gl, const float* gh, void* dx, cudaStream_t s) {
   const T* x = (const T*)xv;
   if (V <= 2048) return bwd_nt<32>(x, rs, tok, rows, V, st, ent, gl, gh, (T*)dx, s);
-  if (rows <= 148) return bwd_nt<1024>(x, rs, tok, rows, V, st, ent, gl, gh, (T*)dx, s);
   return bwd_nt<256>(x, rs, tok, rows, V, st, ent, gl, gh, (T*)dx, s);
 }
 

@@ -174,8 +174,10 @@ def test_logprobs_refusals():
             token_logprobs(*args, **kw)
 
 
-def test_cache_chunks_cover_the_cache():
+def test_cache_blocks():
+    """A power of two that the kernel takes, more of them for longer caches, one where the streams fill the device."""
     from dual_mod_public_b200.ops.cuda_ops import CudaOps
-    for B, Hkv, longest in [(1, 1, 0), (1, 1, 1), (1, 16, 2048), (64, 4, 8192), (300, 16, 100), (1, 1, 1 << 20)]:
-        chunk, splits = CudaOps.cache_chunks(B, Hkv, longest)
-        assert splits >= 1 and chunk >= 16 and chunk % 16 == 0 and chunk * splits >= longest and chunk * (splits - 1) <= max(0, longest - 1)
+    for streams in (1, 2, 16, 147, 148, 5000):
+        got = [CudaOps.cache_blocks(streams, n) for n in (0, 1, 256, 257, 2048, 5000, 1 << 20)]
+        assert got == sorted(got) and set(got) <= {1, 2, 4, 8, 16} and got[0] == 1 and got[-1] == 16
+    assert CudaOps.cache_blocks(148, 2048) == 1 and CudaOps.cache_blocks(16, 2048) == 8
