@@ -11,13 +11,16 @@
 // The price is that S and dP are formed twice (seven products of 128 x 128 x D per tile instead of five); one kernel would
 // have to add dQ tiles through memory in whatever order its CTAs run.
 //
-// Both: warps 0..7 do the elementwise work (warps w and w + 4 share the lanes 32 (w % 4) .. and take half of the columns
-// each), warp 8 issues the products, warp 9 loads.  The products of one step are issued in the order in which their operands
-// come free, so the tensor pipe works on (dV, next S) while the math warps form dS, and on (dK or dQ, next dP) while they
-// form the next P.  P and dS are rounded to bf16 (relative 2^-8 at most, as o was); everything else is fp32.
+// Both take the steps of the stream in turn on two warpgroups (warps 0..3 the even steps, 4..7 the odd ones; a thread owns a
+// whole row of a step's 128 x 128 scores), because the parts of a step depend on one another: product, 500 cycles until its
+// result is seen, exponentials, product.  While one warpgroup waits, the other computes.  Warp 8 issues all products in one
+// fixed order, warp 9 loads.  Tensor memory holds the accumulators and per warpgroup 128 columns for S, then dP, then dS; at
+// D = 64 another 64, so that dP can be formed while the exponentials run (dkv: P lies there; dq: dS, and the next S need not
+// wait for dQ).  At D = 128 the accumulators of dkv take the rest: dP follows the product that reads P.
+// P and dS are rounded to bf16 (relative 2^-8 at most, as o was); everything else is fp32.
 //
-// A first small kernel forms delta and scales lse to base 2 (+inf for rows without keys and for the padding of the last tile,
-// which makes their weights zero).
+// A first small kernel forms -delta and -lse in base 2 (-inf for rows without keys and for the padding of the last tile, which
+// makes their weights zero).
 #include "packed.cuh"
 
 using namespace packed;
@@ -25,8 +28,9 @@ using namespace packed;
 namespace {
 
 constexpr int NT = 384;
+constexpr int EMU = 2;                  // pairs of eight on the FMA pipe
 
-// aux: [2][Hq][Tp] fp32 (lse in base 2, delta), Tp = T rounded up to whole tiles
+// aux: [2][Hq][Tp] fp32 (-lse in base 2, -delta), Tp = T rounded up to whole tiles
 template <int LANES>
 __global__ void __launch_bounds__(256) packed_delta_kernel(const bf16* __restrict__ o, const bf16* __restrict__ go, long long g_rs,
                                                            long long g_hs, const float* __restrict__ lse, float* __restrict__ aux,
@@ -53,8 +57,8 @@ __global__ void __launch_bounds__(256) packed_delta_kernel(const bf16* __restric
   for (int i = LANES / 2; i > 0; i >>= 1) s += __shfl_xor_sync(0xffffffffu, s, i);
   if (sub == 0) {
     const float L = inside ? lse[(long long)h * T + row] : -INFINITY;
-    aux[(long long)h * Tp + row] = L == -INFINITY ? INFINITY : L * LOG2E;
-    aux[((long long)Hq + h) * Tp + row] = s;
+    aux[(long long)h * Tp + row] = L == -INFINITY ? -INFINITY : -L * LOG2E;
+    aux[((long long)Hq + h) * Tp + row] = -s;
   }
 }
 
@@ -99,13 +103,72 @@ __device__ __forceinline__ void store_row(uint32_t taddr, bf16* dst, int D, floa
 
 template <int DH>
 struct Cfg {
+  static constexpr bool SIDE = DH == 64;                   // 64 more columns per warpgroup
   static constexpr int TB = TILE * DH * 2;
-  static constexpr int ST = DH == 128 ? 2 : 4;             // ring stages, two tiles each
-  static constexpr int own_off = 0, ring_off = 2 * TB;     // the owner's two tiles, then the ring
-  static constexpr int aux_off = ring_off + ST * 2 * TB;   // dkv: per stage 128 lse and 128 delta
-  static constexpr int bar_off = aux_off + ST * 1024;
+  // rings of single tiles: A (dkv: queries, dq: keys) is read by the first and by the last product of a step, B by those between
+  static constexpr int NA = DH == 128 ? 3 : 4, NB = DH == 128 ? 2 : 4;
+  static constexpr int own_off = 0, a_off = 2 * TB, b_off = a_off + NA * TB;
+  // dkv: 128 -delta per tile of A and 128 -lse per tile of B, so each lies there until the math warps have read it
+  static constexpr int aux_off = b_off + NB * TB;
+  static constexpr int bar_off = aux_off + (NA + NB) * 512;
   static constexpr int total = bar_off + 256;
 };
+static_assert(Cfg<128>::total <= 227 * 1024 && Cfg<64>::total <= 227 * 1024, "shared memory");
+
+// 32 columns of P: exp2(s * scale + nl), nl (minus lse) the same for all columns or one per column.  Of every eight pairs EMU
+// are computed on the FMA pipe (packed.cuh).
+template <int EMU, typename NL>
+__device__ __forceinline__ void exponentials(uint32_t (&x)[32], float scale, NL nl) {
+  const f32x2 sc = pair(scale, scale);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const f32x2 y = fma2(pair(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), sc, nl(i));
+    float p0, p1;
+    if ((i * EMU) % 8 + EMU > 7) {
+      ex2_pair(y, p0, p1);
+    } else {
+      split(y, p0, p1);
+      p0 = ex2(p0);
+      p1 = ex2(p1);
+    }
+    x[2 * i] = __float_as_uint(p0);
+    x[2 * i + 1] = __float_as_uint(p1);
+  }
+}
+// columns outside [lo, hi] to zero; c0: the first of the 32 columns
+__device__ __forceinline__ void clear_hidden(uint32_t (&x)[32], int c0, int lo, int hi) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i)
+    if (c0 + i < lo || c0 + i > hi) x[i] = 0;
+}
+__device__ __forceinline__ void store_packed(uint32_t taddr, const uint32_t (&x)[32]) {
+  uint32_t w[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) w[i] = pack_bf16(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
+  tmem_st16(taddr, w);
+}
+// 32 columns of dS = P (dP - delta), from the dP in tensor memory
+template <typename ND>
+__device__ __forceinline__ void scale_weights(uint32_t (&x)[32], uint32_t taddr, ND nd) {
+  uint32_t d[32];
+  tmem_ld32(taddr, d);
+  tmem_ld_wait();
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const f32x2 t = add2(pair(__uint_as_float(d[2 * i]), __uint_as_float(d[2 * i + 1])), nd(i));
+    float s0, s1;
+    split(mul2(pair(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), t), s0, s1);
+    x[2 * i] = __float_as_uint(s0);
+    x[2 * i + 1] = __float_as_uint(s1);
+  }
+}
+// what a math warp has written to tensor memory is there for the products
+__device__ __forceinline__ void hand_over(uint32_t bar, int lane) {
+  tmem_st_wait();
+  tc_fence_before();
+  __syncwarp();
+  if (lane == 0) mbar_arrive(bar);
+}
 
 // ---------------------------------------------------------------------------------------------------------------------------
 template <int DH>
@@ -120,34 +183,41 @@ __global__ void __launch_bounds__(NT, 1) packed_dkv_kernel(
     return;
   }
   const uint32_t bar0 = base + C::bar_off;
-  // barriers: own, sfull, dpfull, pfull, dsfull, done, drained, qfull[ST], gfull[ST], empty[ST]
-  const uint32_t own = bar0, sfull = bar0 + 8, dpfull = bar0 + 16, pfull = bar0 + 24, dsfull = bar0 + 32, done = bar0 + 40,
-                 drained = bar0 + 48;
-  auto qfull = [&](int s) { return bar0 + 56 + 8u * s; };
-  auto gfull = [&](int s) { return bar0 + 56 + 8u * (C::ST + s); };
-  auto empty = [&](int s) { return bar0 + 56 + 8u * (2 * C::ST + s); };
+  // barriers: own, done, drained, sfull[2], sread[2], pfull[2], dpfull[2], dsfull[2], qfull[NA], qempty[NA], gfull[NB], gempty[NB]
+  const uint32_t own = bar0, done = bar0 + 8, drained = bar0 + 16;
+  auto sfull = [&](int a) { return bar0 + 24 + 8u * a; };
+  auto sread = [&](int a) { return bar0 + 40 + 8u * a; };
+  auto pfull = [&](int a) { return bar0 + 56 + 8u * a; };
+  auto dpfull = [&](int a) { return bar0 + 72 + 8u * a; };
+  auto dsfull = [&](int a) { return bar0 + 88 + 8u * a; };
+  auto qfull = [&](int i) { return bar0 + 104 + 8u * (i % C::NA); };
+  auto qempty = [&](int i) { return bar0 + 104 + 8u * (C::NA + i % C::NA); };
+  auto gfull = [&](int i) { return bar0 + 104 + 8u * (2 * C::NA + i % C::NB); };
+  auto gempty = [&](int i) { return bar0 + 104 + 8u * (2 * C::NA + C::NB + i % C::NB); };
+  auto qphase = [](int i) { return (uint32_t)(i / C::NA) & 1; };
+  auto gphase = [](int i) { return (uint32_t)(i / C::NB) & 1; };
   volatile uint32_t* tslot = reinterpret_cast<volatile uint32_t*>(smem + C::bar_off + 240);
   volatile int* serr = reinterpret_cast<volatile int*>(smem + C::bar_off + 248);
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   // the first keys of a long sequence are seen by the most queries: they come first
   const int kh = blockIdx.x % g.Hkv, kt = blockIdx.x / g.Hkv, key0 = kt * TILE;
   const int last = last_query(g.cu, g.nseq, g.window, g.T, min(g.T, key0 + TILE) - 1);
-  const int nq = uniform(max(kt, last / TILE)) - kt + 1, n_it = nq * g.group;         // query tiles kt .. kt + nq - 1 of each head
+  const int nq = uniform(max(kt, last / TILE)) - kt + 1, steps = nq * g.group;     // query tiles kt .. kt + nq - 1 of each head
 
   if (threadIdx.x == 0) {
     *serr = 0;
     mbar_init(own, 1);
-    mbar_init(sfull, 1);
-    mbar_init(dpfull, 1);
-    mbar_init(pfull, 8);
-    mbar_init(dsfull, 8);
     mbar_init(done, 1);
     mbar_init(drained, 1);
-    for (int s = 0; s < C::ST; ++s) {
-      mbar_init(qfull(s), 1);
-      mbar_init(gfull(s), 1);
-      mbar_init(empty(s), 1);
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(sfull(a), 1);
+      mbar_init(sread(a), 4);
+      mbar_init(pfull(a), 4);
+      mbar_init(dpfull(a), 1);
+      mbar_init(dsfull(a), 4);
     }
+    for (int i = 0; i < C::NA; ++i) { mbar_init(qfull(i), 1); mbar_init(qempty(i), 1); }
+    for (int i = 0; i < C::NB; ++i) { mbar_init(gfull(i), 1); mbar_init(gempty(i), 1); }
     fence_barrier_init();
   }
   if (warp == 8) tmem_alloc(tslot, 512);
@@ -155,10 +225,12 @@ __global__ void __launch_bounds__(NT, 1) packed_dkv_kernel(
   __syncthreads();
   tc_fence_after();
   const uint32_t tm = uniform(*tslot);
-  const uint32_t tS = tm, tdP = tm + TILE, tdV = tm + 2 * TILE, tdK = tdV + DH;
+  auto tX = [&](int a) { return tm + a * TILE; };                                   // S, dP, dS (and P where it has no side columns)
+  auto tP = [&](int a) { return C::SIDE ? tm + 2 * TILE + 2 * DH + a * 64 : tX(a); };
+  const uint32_t tdV = tm + 2 * TILE, tdK = tdV + DH;
   const uint32_t sK = base + C::own_off, sV = sK + C::TB;
-  auto sQ = [&](int s) { return base + C::ring_off + s * 2 * C::TB; };
-  auto sG = [&](int s) { return sQ(s) + C::TB; };
+  auto sQ = [&](int i) { return base + C::a_off + (i % C::NA) * C::TB; };
+  auto sG = [&](int i) { return base + C::b_off + (i % C::NB) * C::TB; };
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");          // 2 x 216 + 72 = 3 x 168
@@ -169,170 +241,181 @@ __global__ void __launch_bounds__(NT, 1) packed_dkv_kernel(
         load_tile<DH>(sV, &tmV, own, kh, key0);
       }
       int i = 0, qi = 0, h = kh * g.group;
-      for (; i < n_it && !*serr; ++i) {
-        const int s = i % C::ST, q0 = (kt + qi) * TILE;
+      for (; i < steps && !*serr; ++i) {
+        const int q0 = (kt + qi) * TILE;
         const float* ax = g.aux + (long long)h * g.Tp + q0;
-        const uint32_t sa = base + C::aux_off + s * 1024;
-        wait(empty(s), ((i / C::ST) & 1) ^ 1, serr);
+        const uint32_t aux = base + C::aux_off;
+        wait(qempty(i), qphase(i) ^ 1, serr);
         if (elect_one()) {
-          mbar_expect_tx(qfull(s), C::TB + 512);
-          load_tile<DH>(sQ(s), &tmQ, qfull(s), h, q0);
-          load_bulk(sa, ax, 512, qfull(s));
-          mbar_expect_tx(gfull(s), C::TB + 512);
-          load_tile<DH>(sG(s), &tmG, gfull(s), h, q0);
-          load_bulk(sa + 512, ax + (long long)g.Hq * g.Tp, 512, gfull(s));
+          mbar_expect_tx(qfull(i), C::TB + 512);
+          load_tile<DH>(sQ(i), &tmQ, qfull(i), h, q0);
+          load_bulk(aux + (i % C::NA) * 512, ax + (long long)g.Hq * g.Tp, 512, qfull(i));
+        }
+        wait(gempty(i), gphase(i) ^ 1, serr);
+        if (elect_one()) {
+          mbar_expect_tx(gfull(i), C::TB + 512);
+          load_tile<DH>(sG(i), &tmG, gfull(i), h, q0);
+          load_bulk(aux + (C::NA + i % C::NB) * 512, ax, 512, gfull(i));
         }
         if (++qi == nq) { qi = 0; ++h; }
       }
       if (*serr) {          // a wait ran out: let the copies in flight land before the CTA ends
         volatile int ignore = 0;
         mbar_wait(own, 0, &ignore);
-        for (int u = max(0, i - C::ST); u < i; ++u) {
-          mbar_wait(qfull(u % C::ST), (u / C::ST) & 1, &ignore);
-          mbar_wait(gfull(u % C::ST), (u / C::ST) & 1, &ignore);
-        }
+        for (int u = max(0, i - C::NA); u < i; ++u) mbar_wait(qfull(u), qphase(u), &ignore);
+        for (int u = max(0, i - C::NB); u < i; ++u) mbar_wait(gfull(u), gphase(u), &ignore);
       }
     } else if (warp == 8) {
       constexpr uint32_t idS = mma_desc<bf16>(TILE, TILE, 0, 0), idG = mma_desc<bf16>(TILE, DH, 0, 1);
       const int begin = max(0, __ldg(g.cu)), end = min(g.T, __ldg(g.cu + g.nseq));
-      auto padded = [&](int q0) { return q0 < begin || q0 + TILE > end; };
+      auto clean = [&](int off, int q0) {                // the padding rows of a tile that has just arrived
+        if (q0 < begin || q0 + TILE > end) blank_rows<DH>(smem + off, q0, begin, end, lane);
+      };
       auto scores = [&](int i, int q0) {                 // S^T = K Q_i^T
-        const int s = i % C::ST;
-        wait(qfull(s), (i / C::ST) & 1, serr);
-        if (padded(q0)) blank_rows<DH>(smem + C::ring_off + s * 2 * C::TB, q0, begin, end, lane);
+        wait(qfull(i), qphase(i), serr);
+        clean(C::a_off + (i % C::NA) * C::TB, q0);
         tc_fence_after();
         if (elect_one()) {
-          const uint64_t k = desc_dims(sK, 0), q = desc_dims(sQ(s), 0);
+          const uint64_t k = desc_dims(sK, 0), q = desc_dims(sQ(i), 0);
 #pragma unroll
-          for (int u = 0; u < DH / 16; ++u) umma_bf16(tS, k + dims_step(u), q + dims_step(u), idS, u != 0);
-          umma_commit(sfull);
+          for (int u = 0; u < DH / 16; ++u) umma_bf16(tX(i & 1), k + dims_step(u), q + dims_step(u), idS, u != 0);
+          umma_commit(sfull(i & 1));
         }
         __syncwarp();
       };
-      auto dscores = [&](int i, int q0) {                // dP^T = V dO_i^T
-        const int s = i % C::ST;
-        wait(gfull(s), (i / C::ST) & 1, serr);
-        if (padded(q0)) blank_rows<DH>(smem + C::ring_off + s * 2 * C::TB + C::TB, q0, begin, end, lane);
+      auto dscores = [&](int i, bool release) {          // dP^T = V dO_i^T
         tc_fence_after();
         if (elect_one()) {
-          const uint64_t v = desc_dims(sV, 0), go = desc_dims(sG(s), 0);
+          const uint64_t v = desc_dims(sV, 0), go = desc_dims(sG(i), 0);
 #pragma unroll
-          for (int u = 0; u < DH / 16; ++u) umma_bf16(tdP, v + dims_step(u), go + dims_step(u), idS, u != 0);
-          umma_commit(dpfull);
+          for (int u = 0; u < DH / 16; ++u) umma_bf16(tX(i & 1), v + dims_step(u), go + dims_step(u), idS, u != 0);
+          umma_commit(dpfull(i & 1));
+          if (release) umma_commit(gempty(i));
+        }
+        __syncwarp();
+      };
+      auto values = [&](int i, bool release) {           // dV += P^T dO_i
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t go = desc_rows(sG(i), 0);
+#pragma unroll
+          for (int u = 0; u < TILE / 16; ++u) umma_ts(tdV, tP(i & 1) + 8 * u, go + rows_step(u), idG, i > 0 || u != 0);
+          if (release) umma_commit(gempty(i));
+        }
+        __syncwarp();
+      };
+      auto keys = [&](int i) {                           // dK += dS^T Q_i
+        wait(dsfull(i & 1), (i >> 1) & 1, serr);
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t q = desc_rows(sQ(i), 0);
+#pragma unroll
+          for (int u = 0; u < TILE / 16; ++u) umma_ts(tdK, tX(i & 1) + 8 * u, q + rows_step(u), idG, i > 0 || u != 0);
+          umma_commit(qempty(i));
+          if (i + 1 == steps) umma_commit(done);
         }
         __syncwarp();
       };
       wait(own, 0, serr);
-      scores(0, key0);
-      dscores(0, key0);
-      int qi = 0;
-      for (int i = 0; i < n_it; ++i) {
-        const int s = i % C::ST;
-        if (++qi == nq) qi = 0;                          // of the next step
-        wait(pfull, i & 1, serr);
-        tc_fence_after();
-        if (elect_one()) {
-          const uint64_t go = desc_rows(sG(s), 0);
-#pragma unroll
-          for (int u = 0; u < TILE / 16; ++u)            // the halves of P^T lie behind each other's scores: 0 .. 31 and 64 .. 95
-            umma_ts(tdV, tS + (u / 4) * 64 + (u % 4) * 8, go + rows_step(u), idG, i > 0 || u != 0);
+      int q0 = key0, ahead0 = key0;                      // first rows of the query tiles of step i and of the next scores
+      auto next = [&](int v) { return v + TILE == key0 + nq * TILE ? key0 : v + TILE; };
+      scores(0, ahead0);
+      ahead0 = next(ahead0);
+      if (steps > 1) { scores(1, ahead0); ahead0 = next(ahead0); }
+      auto gradient_tile = [&](int i) {
+        wait(gfull(i), gphase(i), serr);
+        clean(C::b_off + (i % C::NB) * C::TB, q0);
+        q0 = next(q0);
+      };
+      auto finish = [&](int i) {                         // dS -> dK, and this warpgroup's next scores
+        keys(i);
+        if (i + 2 < steps) { scores(i + 2, ahead0); ahead0 = next(ahead0); }
+      };
+      if (C::SIDE) {
+        // S read -> dP in its place; the other warpgroup's last step; P -> dV
+        for (int i = 0; i < steps; ++i) {
+          gradient_tile(i);
+          wait(sread(i & 1), (i >> 1) & 1, serr);
+          dscores(i, false);
+          if (i > 0) finish(i - 1);
+          wait(pfull(i & 1), (i >> 1) & 1, serr);
+          values(i, true);
         }
-        __syncwarp();
-        if (i + 1 < n_it) scores(i + 1, key0 + qi * TILE);
-        wait(dsfull, i & 1, serr);
-        tc_fence_after();
-        if (elect_one()) {
-          const uint64_t q = desc_rows(sQ(s), 0);
-#pragma unroll
-          for (int u = 0; u < TILE / 16; ++u)
-            umma_ts(tdK, tdP + (u / 4) * 64 + (u % 4) * 8, q + rows_step(u), idG, i > 0 || u != 0);
-          umma_commit(empty(s));
-          if (i + 1 == n_it) umma_commit(done);
+        finish(steps - 1);
+      } else {
+        // P -> dV, and dP in its place behind it.  Between this and the end of the step its warpgroup needs the tensor pipe's
+        // latency and the time to form dS; in this order the other warpgroup's products fill it
+        auto begin_step = [&](int i) {
+          gradient_tile(i);
+          wait(pfull(i & 1), (i >> 1) & 1, serr);
+          values(i, false);
+          dscores(i, true);
+        };
+        for (int i = 0; i < steps; i += 2) {
+          begin_step(i);
+          if (i > 0) finish(i - 1);
+          finish(i);
+          if (i + 1 < steps) begin_step(i + 1);
         }
-        __syncwarp();
-        if (i + 1 < n_it) dscores(i + 1, key0 + qi * TILE);
+        if (!(steps & 1)) finish(steps - 1);
       }
       drain_products(drained, serr);
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-    const int half = warp >> 2, key = key0 + (warp & 3) * 32 + lane;
+    const int a = warp >> 2, key = key0 + (warp & 3) * 32 + lane;
     const uint32_t tl = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t x_addr = tX(a) + tl, p_addr = tP(a) + tl;
     const int hi = key < g.T ? last_query(g.cu, g.nseq, g.window, g.T, key) : key - 1;
     const int w_hi = __shfl_sync(0xffffffffu, hi, 0), w_key = key - lane + 31;        // hi ascends with the key
-    int qi = 0;
-    for (int i = 0; i < n_it; ++i) {
-      const int s = i % C::ST, q0 = (kt + qi) * TILE + half * 64;
-      if (++qi == nq) qi = 0;
-      const float4* lse = reinterpret_cast<const float4*>(smem + C::aux_off + s * 1024) + half * 16;
-      const float4* delta = lse + 32;
-      wait(sfull, i & 1, serr);
-      wait(qfull(s), (i / C::ST) & 1, serr);               // lse arrived with the queries
+    int qi = a % nq;
+    for (int i = a; i < steps; i += 2) {
+      const uint32_t ph = (i >> 1) & 1;
+      const int q0 = (kt + qi) * TILE;
+      qi = (qi + 2) % nq;
+      const ulonglong2* ndelta = reinterpret_cast<const ulonglong2*>(smem + C::aux_off + (i % C::NA) * 512);
+      const ulonglong2* nlse = reinterpret_cast<const ulonglong2*>(smem + C::aux_off + (C::NA + i % C::NB) * 512);
+      wait(sfull(a), ph, serr);
+      wait(qfull(i), qphase(i), serr);                     // delta arrived with the queries
+      wait(gfull(i), gphase(i), serr);                     // and lse with the output's gradient
       tc_fence_after();
-      uint32_t x[2][32];
-      tmem_ld32(tS + tl + half * 64, x[0]);
-      tmem_ld32(tS + tl + half * 64 + 32, x[1]);
-      tmem_ld_wait();
-      float p[64];
+      uint32_t x[4][32];
 #pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        const float4 L = lse[c];
-        p[4 * c] = exp2f(fmaf(__uint_as_float(x[c >> 3][(4 * c) & 31]), g.scale_log2, -L.x));
-        p[4 * c + 1] = exp2f(fmaf(__uint_as_float(x[c >> 3][(4 * c + 1) & 31]), g.scale_log2, -L.y));
-        p[4 * c + 2] = exp2f(fmaf(__uint_as_float(x[c >> 3][(4 * c + 2) & 31]), g.scale_log2, -L.z));
-        p[4 * c + 3] = exp2f(fmaf(__uint_as_float(x[c >> 3][(4 * c + 3) & 31]), g.scale_log2, -L.w));
+      for (int c = 0; c < 4; ++c) tmem_ld32(x_addr + 32 * c, x[c]);
+      tmem_ld_wait();
+      if (C::SIDE) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(sread(a));
       }
-      const bool mask = q0 < w_key || q0 + 63 > w_hi;
+      const bool mask = q0 < w_key || q0 + TILE - 1 > w_hi;
       const int c_lo = key - q0, c_hi = hi - q0;
-      if (mask) {
 #pragma unroll
-        for (int c = 0; c < 64; ++c)
-          if (c < c_lo || c > c_hi) p[c] = 0.f;
+      for (int c = 0; c < 4; ++c) {
+        auto nl = [&](int u) { const ulonglong2 v = nlse[8 * c + (u >> 1)]; return (u & 1) ? v.y : v.x; };
+        if (mask) {
+          exponentials<0>(x[c], g.scale_log2, nl);
+          clear_hidden(x[c], 32 * c, c_lo, c_hi);
+        } else {
+          exponentials<EMU>(x[c], g.scale_log2, nl);
+        }
+        store_packed(p_addr + 16 * c, x[c]);
       }
-      {
-        uint32_t w[32];
-#pragma unroll
-        for (int c = 0; c < 32; ++c) w[c] = pack_bf16(p[2 * c], p[2 * c + 1]);
-        tmem_st32(tS + tl + half * 64, w);
-      }
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(pfull);
-      wait(dpfull, i & 1, serr);
-      wait(gfull(s), (i / C::ST) & 1, serr);
+      hand_over(pfull(a), lane);
+      wait(dpfull(a), ph, serr);
       tc_fence_after();
-      tmem_ld32(tdP + tl + half * 64, x[0]);
-      tmem_ld32(tdP + tl + half * 64 + 32, x[1]);
-      tmem_ld_wait();
 #pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        const float4 d = delta[c];
-        p[4 * c] *= __uint_as_float(x[c >> 3][(4 * c) & 31]) - d.x;
-        p[4 * c + 1] *= __uint_as_float(x[c >> 3][(4 * c + 1) & 31]) - d.y;
-        p[4 * c + 2] *= __uint_as_float(x[c >> 3][(4 * c + 2) & 31]) - d.z;
-        p[4 * c + 3] *= __uint_as_float(x[c >> 3][(4 * c + 3) & 31]) - d.w;
+      for (int c = 0; c < 4; ++c) {
+        scale_weights(x[c], x_addr + 32 * c, [&](int u) { const ulonglong2 v = ndelta[8 * c + (u >> 1)]; return (u & 1) ? v.y : v.x; });
+        if (mask) clear_hidden(x[c], 32 * c, c_lo, c_hi);  // 0 x (what a padding row's product left) is not zero
+        store_packed(x_addr + 16 * c, x[c]);               // into columns whose dP has been read
       }
-      if (mask) {                                          // 0 x (what a padding row's product left) is not zero
-#pragma unroll
-        for (int c = 0; c < 64; ++c)
-          if (c < c_lo || c > c_hi) p[c] = 0.f;
-      }
-      {
-        uint32_t w[32];
-#pragma unroll
-        for (int c = 0; c < 32; ++c) w[c] = pack_bf16(p[2 * c], p[2 * c + 1]);
-        tmem_st32(tdP + tl + half * 64, w);
-      }
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(dsfull);
+      hand_over(dsfull(a), lane);
     }
     wait(done, 0, serr);
     tc_fence_after();
     const long long off = ((long long)key * g.Hkv + kh) * g.D;
-    if (half == 0) store_row<DH>(tdV + tl, dv + off, g.D, 1.f, key < g.T);
+    if (a == 0) store_row<DH>(tdV + tl, dv + off, g.D, 1.f, key < g.T);
     else store_row<DH>(tdK + tl, dk + off, g.D, g.scale, key < g.T);
   }
   tc_fence_before();
@@ -355,32 +438,39 @@ __global__ void __launch_bounds__(NT, 1) packed_dq_kernel(
     return;
   }
   const uint32_t bar0 = base + C::bar_off;
-  // barriers: own, sfull, dpfull, sread, dsfull, done, drained, kfull[ST], vfull[ST], empty[ST]
-  const uint32_t own = bar0, sfull = bar0 + 8, dpfull = bar0 + 16, sread = bar0 + 24, dsfull = bar0 + 32, done = bar0 + 40,
-                 drained = bar0 + 48;
-  auto kfull = [&](int s) { return bar0 + 56 + 8u * s; };
-  auto vfull = [&](int s) { return bar0 + 56 + 8u * (C::ST + s); };
-  auto empty = [&](int s) { return bar0 + 56 + 8u * (2 * C::ST + s); };
+  // barriers: own, done, drained, sfull[2], sread[2], dqdone[2], dpfull[2], dsfull[2], kfull[NA], kempty[NA], vfull[NB], vempty[NB]
+  const uint32_t own = bar0, done = bar0 + 8, drained = bar0 + 16;
+  auto sfull = [&](int a) { return bar0 + 24 + 8u * a; };
+  auto sread = [&](int a) { return bar0 + 40 + 8u * a; };
+  auto dqdone = [&](int a) { return bar0 + 56 + 8u * a; };
+  auto dpfull = [&](int a) { return bar0 + 72 + 8u * a; };
+  auto dsfull = [&](int a) { return bar0 + 88 + 8u * a; };
+  auto kfull = [&](int i) { return bar0 + 104 + 8u * (i % C::NA); };
+  auto kempty = [&](int i) { return bar0 + 104 + 8u * (C::NA + i % C::NA); };
+  auto vfull = [&](int i) { return bar0 + 104 + 8u * (2 * C::NA + i % C::NB); };
+  auto vempty = [&](int i) { return bar0 + 104 + 8u * (2 * C::NA + C::NB + i % C::NB); };
+  auto kphase = [](int i) { return (uint32_t)(i / C::NA) & 1; };
+  auto vphase = [](int i) { return (uint32_t)(i / C::NB) & 1; };
   volatile uint32_t* tslot = reinterpret_cast<volatile uint32_t*>(smem + C::bar_off + 240);
   volatile int* serr = reinterpret_cast<volatile int*>(smem + C::bar_off + 248);
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int h = blockIdx.x % g.Hq, qt = g.tiles - 1 - blockIdx.x / g.Hq, row0 = qt * TILE;
-  const int kb0 = uniform(min(qt, first_key(g.cu, g.nseq, g.window, row0) / TILE)), n_it = qt - kb0 + 1;
+  const int kb0 = uniform(min(qt, first_key(g.cu, g.nseq, g.window, row0) / TILE)), steps = qt - kb0 + 1;
 
   if (threadIdx.x == 0) {
     *serr = 0;
     mbar_init(own, 1);
-    mbar_init(sfull, 1);
-    mbar_init(dpfull, 1);
-    mbar_init(sread, 8);
-    mbar_init(dsfull, 8);
     mbar_init(done, 1);
     mbar_init(drained, 1);
-    for (int s = 0; s < C::ST; ++s) {
-      mbar_init(kfull(s), 1);
-      mbar_init(vfull(s), 1);
-      mbar_init(empty(s), 1);
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(sfull(a), 1);
+      mbar_init(sread(a), 4);
+      mbar_init(dqdone(a), 1);
+      mbar_init(dpfull(a), 1);
+      mbar_init(dsfull(a), 4);
     }
+    for (int i = 0; i < C::NA; ++i) { mbar_init(kfull(i), 1); mbar_init(kempty(i), 1); }
+    for (int i = 0; i < C::NB; ++i) { mbar_init(vfull(i), 1); mbar_init(vempty(i), 1); }
     fence_barrier_init();
   }
   if (warp == 8) tmem_alloc(tslot, 512);
@@ -388,10 +478,12 @@ __global__ void __launch_bounds__(NT, 1) packed_dq_kernel(
   __syncthreads();
   tc_fence_after();
   const uint32_t tm = uniform(*tslot);
-  const uint32_t tS = tm, tdP = tm + TILE, tdQ = tm + 2 * TILE;
+  auto tX = [&](int a) { return tm + a * TILE; };                                   // S, then dP
+  auto tDS = [&](int a) { return C::SIDE ? tm + 2 * TILE + DH + a * 64 : tX(a); };
+  const uint32_t tdQ = tm + 2 * TILE;
   const uint32_t sQ = base + C::own_off, sG = sQ + C::TB;
-  auto sK = [&](int s) { return base + C::ring_off + s * 2 * C::TB; };
-  auto sV = [&](int s) { return sK(s) + C::TB; };
+  auto sK = [&](int i) { return base + C::a_off + (i % C::NA) * C::TB; };
+  auto sV = [&](int i) { return base + C::b_off + (i % C::NB) * C::TB; };
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
@@ -403,124 +495,125 @@ __global__ void __launch_bounds__(NT, 1) packed_dq_kernel(
         load_tile<DH>(sG, &tmG, own, h, row0);
       }
       int i = 0;
-      for (; i < n_it && !*serr; ++i) {
-        const int s = i % C::ST, k0 = (kb0 + i) * TILE;
-        wait(empty(s), ((i / C::ST) & 1) ^ 1, serr);
+      for (; i < steps && !*serr; ++i) {
+        const int k0 = (kb0 + i) * TILE;
+        wait(kempty(i), kphase(i) ^ 1, serr);
         if (elect_one()) {
-          mbar_expect_tx(kfull(s), C::TB);
-          load_tile<DH>(sK(s), &tmK, kfull(s), kh, k0);
-          mbar_expect_tx(vfull(s), C::TB);
-          load_tile<DH>(sV(s), &tmV, vfull(s), kh, k0);
+          mbar_expect_tx(kfull(i), C::TB);
+          load_tile<DH>(sK(i), &tmK, kfull(i), kh, k0);
+        }
+        wait(vempty(i), vphase(i) ^ 1, serr);
+        if (elect_one()) {
+          mbar_expect_tx(vfull(i), C::TB);
+          load_tile<DH>(sV(i), &tmV, vfull(i), kh, k0);
         }
       }
       if (*serr) {
         volatile int ignore = 0;
         mbar_wait(own, 0, &ignore);
-        for (int u = max(0, i - C::ST); u < i; ++u) {
-          mbar_wait(kfull(u % C::ST), (u / C::ST) & 1, &ignore);
-          mbar_wait(vfull(u % C::ST), (u / C::ST) & 1, &ignore);
-        }
+        for (int u = max(0, i - C::NA); u < i; ++u) mbar_wait(kfull(u), kphase(u), &ignore);
+        for (int u = max(0, i - C::NB); u < i; ++u) mbar_wait(vfull(u), vphase(u), &ignore);
       }
     } else if (warp == 8) {
       constexpr uint32_t idS = mma_desc<bf16>(TILE, TILE, 0, 0), idG = mma_desc<bf16>(TILE, DH, 0, 1);
       const int begin = max(0, __ldg(g.cu)), end = min(g.T, __ldg(g.cu + g.nseq));
       auto scores = [&](int i) {                         // S = Q K_i^T
-        const int s = i % C::ST, k0 = (kb0 + i) * TILE;
-        wait(kfull(s), (i / C::ST) & 1, serr);
-        if (k0 < begin || k0 + TILE > end) blank_rows<DH>(smem + C::ring_off + s * 2 * C::TB, k0, begin, end, lane);
+        const int k0 = (kb0 + i) * TILE;
+        wait(kfull(i), kphase(i), serr);
+        if (k0 < begin || k0 + TILE > end) blank_rows<DH>(smem + C::a_off + (i % C::NA) * C::TB, k0, begin, end, lane);
         tc_fence_after();
         if (elect_one()) {
-          const uint64_t q = desc_dims(sQ, 0), k = desc_dims(sK(s), 0);
+          const uint64_t q = desc_dims(sQ, 0), k = desc_dims(sK(i), 0);
 #pragma unroll
-          for (int u = 0; u < DH / 16; ++u) umma_bf16(tS, q + dims_step(u), k + dims_step(u), idS, u != 0);
-          umma_commit(sfull);
+          for (int u = 0; u < DH / 16; ++u) umma_bf16(tX(i & 1), q + dims_step(u), k + dims_step(u), idS, u != 0);
+          umma_commit(sfull(i & 1));
         }
         __syncwarp();
       };
-      auto dscores = [&](int i) {                        // dP = dO V_i^T
-        const int s = i % C::ST;
-        wait(vfull(s), (i / C::ST) & 1, serr);
+      auto dscores = [&](int i) {                        // dP = dO V_i^T, once S has been read
+        wait(vfull(i), vphase(i), serr);
+        wait(sread(i & 1), (i >> 1) & 1, serr);
         tc_fence_after();
         if (elect_one()) {
-          const uint64_t go = desc_dims(sG, 0), v = desc_dims(sV(s), 0);
+          const uint64_t go = desc_dims(sG, 0), v = desc_dims(sV(i), 0);
 #pragma unroll
-          for (int u = 0; u < DH / 16; ++u) umma_bf16(tdP, go + dims_step(u), v + dims_step(u), idS, u != 0);
-          umma_commit(dpfull);
+          for (int u = 0; u < DH / 16; ++u) umma_bf16(tX(i & 1), go + dims_step(u), v + dims_step(u), idS, u != 0);
+          umma_commit(dpfull(i & 1));
+          umma_commit(vempty(i));
+        }
+        __syncwarp();
+      };
+      auto queries = [&](int i) {                        // dQ += dS K_i
+        if (elect_one()) {
+          const uint64_t k = desc_rows(sK(i), 0);
+#pragma unroll
+          for (int u = 0; u < TILE / 16; ++u) umma_ts(tdQ, tDS(i & 1) + 8 * u, k + rows_step(u), idG, i > 0 || u != 0);
+          umma_commit(kempty(i));
+          if (C::SIDE) umma_commit(dqdone(i & 1));
+          if (i + 1 == steps) umma_commit(done);
         }
         __syncwarp();
       };
       wait(own, 0, serr);
       scores(0);
-      dscores(0);
-      for (int i = 0; i < n_it; ++i) {
-        const int s = i % C::ST;
-        if (i + 1 < n_it) {
-          wait(sread, i & 1, serr);
-          scores(i + 1);
+      if (steps > 1) scores(1);
+      for (int i = 0; i < steps; ++i) {
+        dscores(i);
+        if (i > 0) {                                     // the other warpgroup's dS -> dQ and its next scores
+          wait(dsfull((i - 1) & 1), ((i - 1) >> 1) & 1, serr);
+          tc_fence_after();
+          if (C::SIDE && i + 1 < steps) scores(i + 1);
+          queries(i - 1);
+          if (!C::SIDE && i + 1 < steps) scores(i + 1);
         }
-        wait(dsfull, i & 1, serr);
-        tc_fence_after();
-        if (elect_one()) {
-          const uint64_t k = desc_rows(sK(s), 0);
-#pragma unroll
-          for (int u = 0; u < TILE / 16; ++u)
-            umma_ts(tdQ, tdP + (u / 4) * 64 + (u % 4) * 8, k + rows_step(u), idG, i > 0 || u != 0);
-          umma_commit(empty(s));
-          if (i + 1 == n_it) umma_commit(done);
-        }
-        __syncwarp();
-        if (i + 1 < n_it) dscores(i + 1);
       }
+      wait(dsfull((steps - 1) & 1), ((steps - 1) >> 1) & 1, serr);
+      tc_fence_after();
+      queries(steps - 1);
       drain_products(drained, serr);
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-    const int half = warp >> 2, row = row0 + (warp & 3) * 32 + lane;
+    const int a = warp >> 2, row = row0 + (warp & 3) * 32 + lane;
     const uint32_t tl = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t x_addr = tX(a) + tl, ds_addr = tDS(a) + tl;
     const int lo = row < g.T ? first_key(g.cu, g.nseq, g.window, row) : row + 1;
     const int w_lo = __shfl_sync(0xffffffffu, lo, 31), w_row = row - lane;
-    const float L = g.aux[(long long)h * g.Tp + row], delta = g.aux[((long long)g.Hq + h) * g.Tp + row];
-    for (int i = 0; i < n_it; ++i) {
-      const int k0 = (kb0 + i) * TILE + half * 64;
-      wait(sfull, i & 1, serr);
+    const float L = g.aux[(long long)h * g.Tp + row], D = g.aux[((long long)g.Hq + h) * g.Tp + row];
+    const f32x2 nl = pair(L, L), nd = pair(D, D);
+    for (int i = a; i < steps; i += 2) {
+      const uint32_t ph = (i >> 1) & 1;
+      const int k0 = (kb0 + i) * TILE;
+      wait(sfull(a), ph, serr);
       tc_fence_after();
-      uint32_t x[2][32];
-      tmem_ld32(tS + tl + half * 64, x[0]);
-      tmem_ld32(tS + tl + half * 64 + 32, x[1]);
+      uint32_t x[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld32(x_addr + 32 * c, x[c]);
       tmem_ld_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(sread);
-      float p[64];
+      if (lane == 0) mbar_arrive(sread(a));
+      const bool mask = k0 < w_lo || k0 + TILE - 1 > w_row;
+      const int c_lo = lo - k0, c_hi = row - k0;
 #pragma unroll
-      for (int c = 0; c < 64; ++c) p[c] = exp2f(fmaf(__uint_as_float(x[c >> 5][c & 31]), g.scale_log2, -L));
-      wait(dpfull, i & 1, serr);
+      for (int c = 0; c < 4; ++c) {
+        if (mask) exponentials<0>(x[c], g.scale_log2, [&](int) { return nl; });
+        else exponentials<EMU>(x[c], g.scale_log2, [&](int) { return nl; });
+      }
+      wait(dpfull(a), ph, serr);
+      if (C::SIDE && i >= 2) wait(dqdone(a), ((i >> 1) - 1) & 1, serr);               // the last dS of this warpgroup has been read
       tc_fence_after();
-      tmem_ld32(tdP + tl + half * 64, x[0]);
-      tmem_ld32(tdP + tl + half * 64 + 32, x[1]);
-      tmem_ld_wait();
 #pragma unroll
-      for (int c = 0; c < 64; ++c) p[c] *= __uint_as_float(x[c >> 5][c & 31]) - delta;
-      if (k0 < w_lo || k0 + 63 > w_row) {
-        const int c_lo = lo - k0, c_hi = row - k0;
-#pragma unroll
-        for (int c = 0; c < 64; ++c)
-          if (c < c_lo || c > c_hi) p[c] = 0.f;
+      for (int c = 0; c < 4; ++c) {
+        scale_weights(x[c], x_addr + 32 * c, [&](int) { return nd; });
+        if (mask) clear_hidden(x[c], 32 * c, c_lo, c_hi);
+        store_packed(ds_addr + 16 * c, x[c]);              // where there are no side columns: into some whose dP has been read
       }
-      {
-        uint32_t w[32];
-#pragma unroll
-        for (int c = 0; c < 32; ++c) w[c] = pack_bf16(p[2 * c], p[2 * c + 1]);
-        tmem_st32(tdP + tl + half * 64, w);
-      }
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(dsfull);
+      hand_over(dsfull(a), lane);
     }
     wait(done, 0, serr);
     tc_fence_after();
-    if (half == 0) store_row<DH>(tdQ + tl, dq + ((long long)row * g.Hq + h) * g.D, g.D, g.scale, row < g.T);
+    if (a == 0) store_row<DH>(tdQ + tl, dq + ((long long)row * g.Hq + h) * g.D, g.D, g.scale, row < g.T);
   }
   tc_fence_before();
   __syncthreads();
