@@ -14,9 +14,10 @@
 // Both take the steps of the stream in turn on two warpgroups (warps 0..3 the even steps, 4..7 the odd ones; a thread owns a
 // whole row of a step's 128 x 128 scores), because the parts of a step depend on one another: product, 500 cycles until its
 // result is seen, exponentials, product.  While one warpgroup waits, the other computes.  Warp 8 issues all products in one
-// fixed order, warp 9 loads.  Tensor memory holds the accumulators and per warpgroup 128 columns for S, then dP, then dS; at
-// D = 64 another 64, so that dP can be formed while the exponentials run (dkv: P lies there; dq: dS, and the next S need not
-// wait for dQ).  At D = 128 the accumulators of dkv take the rest: dP follows the product that reads P.
+// fixed order, warp 9 loads.  Tensor memory holds the accumulators and per warpgroup 128 columns for S, then dP, and 64 for the
+// 16-bit operands (dkv: P, then dS; dq: dS): dP is formed while the exponentials run, and the next S as soon as dP has been
+// read.  At D = 128 the accumulators of dkv leave no such columns: P and dS overwrite S and dP, dP follows the product that
+// reads P, and the next S the one that reads dS.
 // P and dS are rounded to bf16 (relative 2^-8 at most, as o was); everything else is fp32.
 //
 // A first small kernel forms -delta and -lse in base 2 (-inf for rows without keys and for the padding of the last tile, which
@@ -103,7 +104,7 @@ __device__ __forceinline__ void store_row(uint32_t taddr, bf16* dst, int D, floa
 
 template <int DH>
 struct Cfg {
-  static constexpr bool SIDE = DH == 64;                   // 64 more columns per warpgroup
+  static constexpr bool SIDE = DH == 64;                   // dkv: columns for the 16-bit operands
   static constexpr int TB = TILE * DH * 2;
   // rings of single tiles: A (dkv: queries, dq: keys) is read by the first and by the last product of a step, B by those between
   static constexpr int NA = DH == 128 ? 3 : 4, NB = DH == 128 ? 2 : 4;
@@ -111,28 +112,42 @@ struct Cfg {
   // dkv: 128 -delta per tile of A and 128 -lse per tile of B, so each lies there until the math warps have read it
   static constexpr int aux_off = b_off + NB * TB;
   static constexpr int bar_off = aux_off + (NA + NB) * 512;
-  static constexpr int total = bar_off + 256;
+  static constexpr int total = bar_off + 304;
 };
 static_assert(Cfg<128>::total <= 227 * 1024 && Cfg<64>::total <= 227 * 1024, "shared memory");
 
-// 32 columns of P: exp2(s * scale + nl), nl (minus lse) the same for all columns or one per column.  Of every eight pairs EMU
-// are computed on the FMA pipe (packed.cuh).
-template <int EMU, typename NL>
-__device__ __forceinline__ void exponentials(uint32_t (&x)[32], float scale, NL nl) {
+// P = exp2(s * scale + nl) in place, nl = -lse.  Of every eight pairs EMU are computed on the FMA pipe (packed.cuh).
+template <int EMU>
+__device__ __forceinline__ void exponential_pair(uint32_t& a, uint32_t& b, f32x2 sc, f32x2 nl, int i) {
+  const f32x2 y = fma2(pair(__uint_as_float(a), __uint_as_float(b)), sc, nl);
+  float p0, p1;
+  if ((i * EMU) % 8 + EMU > 7) {
+    ex2_pair(y, p0, p1);
+  } else {
+    split(y, p0, p1);
+    p0 = ex2(p0);
+    p1 = ex2(p1);
+  }
+  a = __float_as_uint(p0);
+  b = __float_as_uint(p1);
+}
+// a row per thread, 32 of its columns
+template <int EMU>
+__device__ __forceinline__ void exponentials(uint32_t (&x)[32], float scale, f32x2 nl) {
   const f32x2 sc = pair(scale, scale);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const f32x2 y = fma2(pair(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), sc, nl(i));
-    float p0, p1;
-    if ((i * EMU) % 8 + EMU > 7) {
-      ex2_pair(y, p0, p1);
-    } else {
-      split(y, p0, p1);
-      p0 = ex2(p0);
-      p1 = ex2(p1);
-    }
-    x[2 * i] = __float_as_uint(p0);
-    x[2 * i + 1] = __float_as_uint(p1);
+  for (int i = 0; i < 16; ++i) exponential_pair<EMU>(x[2 * i], x[2 * i + 1], sc, nl, i);
+}
+// fragments of 32 rows and 128 columns; nl: this thread's pair of every 8 columns
+template <int EMU>
+__device__ __forceinline__ void exponentials(uint32_t (&x)[2][64], float scale, const f32x2* nl) {
+  const f32x2 sc = pair(scale, scale);
+#pragma unroll
+  for (int u = 0; u < 16; ++u) {
+    const f32x2 n = nl[4 * u];
+#pragma unroll
+    for (int v = 0; v < 4; ++v)
+      exponential_pair<EMU>(x[v >> 1][4 * u + 2 * (v & 1)], x[v >> 1][4 * u + 2 * (v & 1) + 1], sc, n, 4 * u + v);
   }
 }
 // columns outside [lo, hi] to zero; c0: the first of the 32 columns
@@ -147,20 +162,18 @@ __device__ __forceinline__ void store_packed(uint32_t taddr, const uint32_t (&x)
   for (int i = 0; i < 16; ++i) w[i] = pack_bf16(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
   tmem_st16(taddr, w);
 }
-// 32 columns of dS = P (dP - delta), from the dP in tensor memory
-template <typename ND>
-__device__ __forceinline__ void scale_weights(uint32_t (&x)[32], uint32_t taddr, ND nd) {
-  uint32_t d[32];
-  tmem_ld32(taddr, d);
-  tmem_ld_wait();
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const f32x2 t = add2(pair(__uint_as_float(d[2 * i]), __uint_as_float(d[2 * i + 1])), nd(i));
-    float s0, s1;
-    split(mul2(pair(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), t), s0, s1);
-    x[2 * i] = __float_as_uint(s0);
-    x[2 * i + 1] = __float_as_uint(s1);
-  }
+// dS = P (dP - delta) in place, nd = -delta
+__device__ __forceinline__ void scale_pair(uint32_t& a, uint32_t& b, uint32_t d0, uint32_t d1, f32x2 nd) {
+  float s0, s1;
+  split(mul2(pair(__uint_as_float(a), __uint_as_float(b)), add2(pair(__uint_as_float(d0), __uint_as_float(d1)), nd)), s0, s1);
+  a = __float_as_uint(s0);
+  b = __float_as_uint(s1);
+}
+// a math warp has read what it wanted of tensor memory
+__device__ __forceinline__ void release(uint32_t bar, int lane) {
+  tc_fence_before();
+  __syncwarp();
+  if (lane == 0) mbar_arrive(bar);
 }
 // what a math warp has written to tensor memory is there for the products
 __device__ __forceinline__ void hand_over(uint32_t bar, int lane) {
@@ -183,21 +196,24 @@ __global__ void __launch_bounds__(NT, 1) packed_dkv_kernel(
     return;
   }
   const uint32_t bar0 = base + C::bar_off;
-  // barriers: own, done, drained, sfull[2], sread[2], pfull[2], dpfull[2], dsfull[2], qfull[NA], qempty[NA], gfull[NB], gempty[NB]
+  // barriers: own, done, drained, sfull[2], sread[2], pfull[2], dpfull[2], dsfull[2], dpread[2], dvdone[2], dkdone[2], then the rings'
   const uint32_t own = bar0, done = bar0 + 8, drained = bar0 + 16;
   auto sfull = [&](int a) { return bar0 + 24 + 8u * a; };
   auto sread = [&](int a) { return bar0 + 40 + 8u * a; };
   auto pfull = [&](int a) { return bar0 + 56 + 8u * a; };
   auto dpfull = [&](int a) { return bar0 + 72 + 8u * a; };
   auto dsfull = [&](int a) { return bar0 + 88 + 8u * a; };
-  auto qfull = [&](int i) { return bar0 + 104 + 8u * (i % C::NA); };
-  auto qempty = [&](int i) { return bar0 + 104 + 8u * (C::NA + i % C::NA); };
-  auto gfull = [&](int i) { return bar0 + 104 + 8u * (2 * C::NA + i % C::NB); };
-  auto gempty = [&](int i) { return bar0 + 104 + 8u * (2 * C::NA + C::NB + i % C::NB); };
+  auto dpread = [&](int a) { return bar0 + 104 + 8u * a; };
+  auto dvdone = [&](int a) { return bar0 + 120 + 8u * a; };
+  auto dkdone = [&](int a) { return bar0 + 136 + 8u * a; };
+  auto qfull = [&](int i) { return bar0 + 152 + 8u * (i % C::NA); };
+  auto qempty = [&](int i) { return bar0 + 152 + 8u * (C::NA + i % C::NA); };
+  auto gfull = [&](int i) { return bar0 + 152 + 8u * (2 * C::NA + i % C::NB); };
+  auto gempty = [&](int i) { return bar0 + 152 + 8u * (2 * C::NA + C::NB + i % C::NB); };
   auto qphase = [](int i) { return (uint32_t)(i / C::NA) & 1; };
   auto gphase = [](int i) { return (uint32_t)(i / C::NB) & 1; };
-  volatile uint32_t* tslot = reinterpret_cast<volatile uint32_t*>(smem + C::bar_off + 240);
-  volatile int* serr = reinterpret_cast<volatile int*>(smem + C::bar_off + 248);
+  volatile uint32_t* tslot = reinterpret_cast<volatile uint32_t*>(smem + C::bar_off + 280);
+  volatile int* serr = reinterpret_cast<volatile int*>(smem + C::bar_off + 288);
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   // the first keys of a long sequence are seen by the most queries: they come first
   const int kh = blockIdx.x % g.Hkv, kt = blockIdx.x / g.Hkv, key0 = kt * TILE;
@@ -215,6 +231,9 @@ __global__ void __launch_bounds__(NT, 1) packed_dkv_kernel(
       mbar_init(pfull(a), 4);
       mbar_init(dpfull(a), 1);
       mbar_init(dsfull(a), 4);
+      mbar_init(dpread(a), 4);
+      mbar_init(dvdone(a), 1);
+      mbar_init(dkdone(a), 1);
     }
     for (int i = 0; i < C::NA; ++i) { mbar_init(qfull(i), 1); mbar_init(qempty(i), 1); }
     for (int i = 0; i < C::NB; ++i) { mbar_init(gfull(i), 1); mbar_init(gempty(i), 1); }
@@ -225,7 +244,8 @@ __global__ void __launch_bounds__(NT, 1) packed_dkv_kernel(
   __syncthreads();
   tc_fence_after();
   const uint32_t tm = uniform(*tslot);
-  auto tX = [&](int a) { return tm + a * TILE; };                                   // S, dP, dS (and P where it has no side columns)
+  auto tX = [&](int a) { return tm + a * TILE; };                                   // S, then dP
+  // P, then dS
   auto tP = [&](int a) { return C::SIDE ? tm + 2 * TILE + 2 * DH + a * 64 : tX(a); };
   const uint32_t tdV = tm + 2 * TILE, tdK = tdV + DH;
   const uint32_t sK = base + C::own_off, sV = sK + C::TB;
@@ -301,6 +321,7 @@ __global__ void __launch_bounds__(NT, 1) packed_dkv_kernel(
 #pragma unroll
           for (int u = 0; u < TILE / 16; ++u) umma_ts(tdV, tP(i & 1) + 8 * u, go + rows_step(u), idG, i > 0 || u != 0);
           if (release) umma_commit(gempty(i));
+          if (C::SIDE) umma_commit(dvdone(i & 1));
         }
         __syncwarp();
       };
@@ -310,8 +331,9 @@ __global__ void __launch_bounds__(NT, 1) packed_dkv_kernel(
         if (elect_one()) {
           const uint64_t q = desc_rows(sQ(i), 0);
 #pragma unroll
-          for (int u = 0; u < TILE / 16; ++u) umma_ts(tdK, tX(i & 1) + 8 * u, q + rows_step(u), idG, i > 0 || u != 0);
+          for (int u = 0; u < TILE / 16; ++u) umma_ts(tdK, tP(i & 1) + 8 * u, q + rows_step(u), idG, i > 0 || u != 0);
           umma_commit(qempty(i));
+          if (C::SIDE) umma_commit(dkdone(i & 1));
           if (i + 1 == steps) umma_commit(done);
         }
         __syncwarp();
@@ -327,24 +349,31 @@ __global__ void __launch_bounds__(NT, 1) packed_dkv_kernel(
         clean(C::b_off + (i % C::NB) * C::TB, q0);
         q0 = next(q0);
       };
-      auto finish = [&](int i) {                         // dS -> dK, and this warpgroup's next scores
-        keys(i);
+      auto next_scores = [&](int i) {                    // of the warpgroup of step i
         if (i + 2 < steps) { scores(i + 2, ahead0); ahead0 = next(ahead0); }
       };
       if (C::SIDE) {
-        // S read -> dP in its place; the other warpgroup's last step; P -> dV
+        // S read -> dP in its place; the other warpgroup's dP read -> its next S, and its dS -> dK; P -> dV
         for (int i = 0; i < steps; ++i) {
           gradient_tile(i);
           wait(sread(i & 1), (i >> 1) & 1, serr);
           dscores(i, false);
-          if (i > 0) finish(i - 1);
+          if (i > 0) {
+            wait(dpread((i - 1) & 1), ((i - 1) >> 1) & 1, serr);
+            next_scores(i - 1);
+            keys(i - 1);
+          }
           wait(pfull(i & 1), (i >> 1) & 1, serr);
           values(i, true);
         }
-        finish(steps - 1);
+        keys(steps - 1);
       } else {
         // P -> dV, and dP in its place behind it.  Between this and the end of the step its warpgroup needs the tensor pipe's
         // latency and the time to form dS; in this order the other warpgroup's products fill it
+        auto finish = [&](int i) {
+          keys(i);
+          next_scores(i);
+        };
         auto begin_step = [&](int i) {
           gradient_tile(i);
           wait(pfull(i & 1), (i >> 1) & 1, serr);
@@ -363,60 +392,98 @@ __global__ void __launch_bounds__(NT, 1) packed_dkv_kernel(
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-    const int a = warp >> 2, key = key0 + (warp & 3) * 32 + lane;
-    const uint32_t tl = (uint32_t)((warp & 3) * 32) << 16;
+    // Scores are read as MMA fragments (16 lanes x 256 bits): a thread holds four of its warp's 32 keys and every fourth pair of
+    // queries, so it wants lse and delta of 32 queries instead of 128.  With a key per thread, handing every value of both to
+    // every thread took as much of shared memory's bandwidth as two of the products (D = 128: 3000 cycles a step).
+    const int a = warp >> 2, t4 = lane & 3, first = key0 + (warp & 3) * 32, own_key = first + lane;
+    const uint32_t tl = (uint32_t)((warp & 3) * 32) << 16, lower = 16u << 16;
     const uint32_t x_addr = tX(a) + tl, p_addr = tP(a) + tl;
-    const int hi = key < g.T ? last_query(g.cu, g.nseq, g.window, g.T, key) : key - 1;
-    const int w_hi = __shfl_sync(0xffffffffu, hi, 0), w_key = key - lane + 31;        // hi ascends with the key
+    const int own_hi = own_key < g.T ? last_query(g.cu, g.nseq, g.window, g.T, own_key) : own_key - 1;
+    const int w_hi = __shfl_sync(0xffffffffu, own_hi, 0), w_key = first + 31;         // hi ascends with the key
+    int hi[2][2];                                                                     // of key first + 16 h + 8 e + lane / 4
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) hi[h][e] = __shfl_sync(0xffffffffu, own_hi, 16 * h + 8 * e + (lane >> 2));
     int qi = a % nq;
     for (int i = a; i < steps; i += 2) {
       const uint32_t ph = (i >> 1) & 1;
       const int q0 = (kt + qi) * TILE;
       qi = (qi + 2) % nq;
-      const ulonglong2* ndelta = reinterpret_cast<const ulonglong2*>(smem + C::aux_off + (i % C::NA) * 512);
-      const ulonglong2* nlse = reinterpret_cast<const ulonglong2*>(smem + C::aux_off + (C::NA + i % C::NB) * 512);
+      const f32x2* ndelta = reinterpret_cast<const f32x2*>(smem + C::aux_off + (i % C::NA) * 512) + t4;
+      const f32x2* nlse = reinterpret_cast<const f32x2*>(smem + C::aux_off + (C::NA + i % C::NB) * 512) + t4;
       wait(sfull(a), ph, serr);
       wait(qfull(i), qphase(i), serr);                     // delta arrived with the queries
       wait(gfull(i), gphase(i), serr);                     // and lse with the output's gradient
       tc_fence_after();
-      uint32_t x[4][32];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(x_addr + 32 * c, x[c]);
+      uint32_t x[2][64];
+      tmem_ld_16x256b_x16(x_addr, x[0]);
+      tmem_ld_16x256b_x16(x_addr + lower, x[1]);
       tmem_ld_wait();
-      if (C::SIDE) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(sread(a));
-      }
+      if (C::SIDE) release(sread(a), lane);
       const bool mask = q0 < w_key || q0 + TILE - 1 > w_hi;
-      const int c_lo = key - q0, c_hi = hi - q0;
+      auto clear = [&]() {                                 // queries that do not see the key
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        auto nl = [&](int u) { const ulonglong2 v = nlse[8 * c + (u >> 1)]; return (u & 1) ? v.y : v.x; };
-        if (mask) {
-          exponentials<0>(x[c], g.scale_log2, nl);
-          clear_hidden(x[c], 32 * c, c_lo, c_hi);
-        } else {
-          exponentials<EMU>(x[c], g.scale_log2, nl);
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int lo_c = first + 16 * h + 8 * e + (lane >> 2) - q0 - 2 * t4, hi_c = hi[h][e] - q0 - 2 * t4;
+#pragma unroll
+            for (int u = 0; u < 16; ++u)
+#pragma unroll
+              for (int w = 0; w < 2; ++w)
+                if (8 * u + w < lo_c || 8 * u + w > hi_c) x[h][4 * u + 2 * e + w] = 0;
+          }
+      };
+      auto store = [&]() {                                 // as the 16-bit operand of the next product
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t w[32];
+#pragma unroll
+          for (int u = 0; u < 32; ++u) w[u] = pack_bf16(__uint_as_float(x[h][2 * u]), __uint_as_float(x[h][2 * u + 1]));
+          tmem_st_16x128b_x16(p_addr + h * lower, w);
         }
-        store_packed(p_addr + 16 * c, x[c]);
+      };
+      if (mask) {
+        exponentials<0>(x, g.scale_log2, nlse);
+        clear();
+      } else {
+        exponentials<EMU>(x, g.scale_log2, nlse);
       }
+      if (C::SIDE && i >= 2) {                             // the product has read this warpgroup's last dS
+        wait(dkdone(a), ((i >> 1) - 1) & 1, serr);
+        tc_fence_after();
+      }
+      store();
       hand_over(pfull(a), lane);
       wait(dpfull(a), ph, serr);
       tc_fence_after();
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        scale_weights(x[c], x_addr + 32 * c, [&](int u) { const ulonglong2 v = ndelta[8 * c + (u >> 1)]; return (u & 1) ? v.y : v.x; });
-        if (mask) clear_hidden(x[c], 32 * c, c_lo, c_hi);  // 0 x (what a padding row's product left) is not zero
-        store_packed(x_addr + 16 * c, x[c]);               // into columns whose dP has been read
+      for (int h = 0; h < 2; ++h) {
+        uint32_t d[64];
+        tmem_ld_16x256b_x16(x_addr + h * lower, d);
+        tmem_ld_wait();
+        if (C::SIDE && h) release(dpread(a), lane);
+#pragma unroll
+        for (int u = 0; u < 16; ++u) {
+          const f32x2 nd = ndelta[4 * u];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) scale_pair(x[h][4 * u + 2 * e], x[h][4 * u + 2 * e + 1], d[4 * u + 2 * e], d[4 * u + 2 * e + 1], nd);
+        }
       }
+      if (mask) clear();                                   // 0 x (what a padding row's product left) is not zero
+      if (C::SIDE) {                                       // the product has read P
+        wait(dvdone(a), ph, serr);
+        tc_fence_after();
+      }
+      store();
       hand_over(dsfull(a), lane);
     }
     wait(done, 0, serr);
     tc_fence_after();
-    const long long off = ((long long)key * g.Hkv + kh) * g.D;
-    if (a == 0) store_row<DH>(tdV + tl, dv + off, g.D, 1.f, key < g.T);
-    else store_row<DH>(tdK + tl, dk + off, g.D, g.scale, key < g.T);
+    const long long off = ((long long)own_key * g.Hkv + kh) * g.D;
+    if (a == 0) store_row<DH>(tdV + tl, dv + off, g.D, 1.f, own_key < g.T);
+    else store_row<DH>(tdK + tl, dk + off, g.D, g.scale, own_key < g.T);
   }
   tc_fence_before();
   __syncthreads();
@@ -438,21 +505,22 @@ __global__ void __launch_bounds__(NT, 1) packed_dq_kernel(
     return;
   }
   const uint32_t bar0 = base + C::bar_off;
-  // barriers: own, done, drained, sfull[2], sread[2], dqdone[2], dpfull[2], dsfull[2], kfull[NA], kempty[NA], vfull[NB], vempty[NB]
+  // barriers: own, done, drained, sfull[2], sread[2], dqdone[2], dpfull[2], dsfull[2], dpread[2], then the rings'
   const uint32_t own = bar0, done = bar0 + 8, drained = bar0 + 16;
   auto sfull = [&](int a) { return bar0 + 24 + 8u * a; };
   auto sread = [&](int a) { return bar0 + 40 + 8u * a; };
   auto dqdone = [&](int a) { return bar0 + 56 + 8u * a; };
   auto dpfull = [&](int a) { return bar0 + 72 + 8u * a; };
   auto dsfull = [&](int a) { return bar0 + 88 + 8u * a; };
-  auto kfull = [&](int i) { return bar0 + 104 + 8u * (i % C::NA); };
-  auto kempty = [&](int i) { return bar0 + 104 + 8u * (C::NA + i % C::NA); };
-  auto vfull = [&](int i) { return bar0 + 104 + 8u * (2 * C::NA + i % C::NB); };
-  auto vempty = [&](int i) { return bar0 + 104 + 8u * (2 * C::NA + C::NB + i % C::NB); };
+  auto dpread = [&](int a) { return bar0 + 104 + 8u * a; };
+  auto kfull = [&](int i) { return bar0 + 120 + 8u * (i % C::NA); };
+  auto kempty = [&](int i) { return bar0 + 120 + 8u * (C::NA + i % C::NA); };
+  auto vfull = [&](int i) { return bar0 + 120 + 8u * (2 * C::NA + i % C::NB); };
+  auto vempty = [&](int i) { return bar0 + 120 + 8u * (2 * C::NA + C::NB + i % C::NB); };
   auto kphase = [](int i) { return (uint32_t)(i / C::NA) & 1; };
   auto vphase = [](int i) { return (uint32_t)(i / C::NB) & 1; };
-  volatile uint32_t* tslot = reinterpret_cast<volatile uint32_t*>(smem + C::bar_off + 240);
-  volatile int* serr = reinterpret_cast<volatile int*>(smem + C::bar_off + 248);
+  volatile uint32_t* tslot = reinterpret_cast<volatile uint32_t*>(smem + C::bar_off + 280);
+  volatile int* serr = reinterpret_cast<volatile int*>(smem + C::bar_off + 288);
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int h = blockIdx.x % g.Hq, qt = g.tiles - 1 - blockIdx.x / g.Hq, row0 = qt * TILE;
   const int kb0 = uniform(min(qt, first_key(g.cu, g.nseq, g.window, row0) / TILE)), steps = qt - kb0 + 1;
@@ -468,6 +536,7 @@ __global__ void __launch_bounds__(NT, 1) packed_dq_kernel(
       mbar_init(dqdone(a), 1);
       mbar_init(dpfull(a), 1);
       mbar_init(dsfull(a), 4);
+      mbar_init(dpread(a), 4);
     }
     for (int i = 0; i < C::NA; ++i) { mbar_init(kfull(i), 1); mbar_init(kempty(i), 1); }
     for (int i = 0; i < C::NB; ++i) { mbar_init(vfull(i), 1); mbar_init(vempty(i), 1); }
@@ -479,7 +548,7 @@ __global__ void __launch_bounds__(NT, 1) packed_dq_kernel(
   tc_fence_after();
   const uint32_t tm = uniform(*tslot);
   auto tX = [&](int a) { return tm + a * TILE; };                                   // S, then dP
-  auto tDS = [&](int a) { return C::SIDE ? tm + 2 * TILE + DH + a * 64 : tX(a); };
+  auto tDS = [&](int a) { return tm + 2 * TILE + DH + a * 64; };
   const uint32_t tdQ = tm + 2 * TILE;
   const uint32_t sQ = base + C::own_off, sG = sQ + C::TB;
   auto sK = [&](int i) { return base + C::a_off + (i % C::NA) * C::TB; };
@@ -544,12 +613,14 @@ __global__ void __launch_bounds__(NT, 1) packed_dq_kernel(
         __syncwarp();
       };
       auto queries = [&](int i) {                        // dQ += dS K_i
+        wait(dsfull(i & 1), (i >> 1) & 1, serr);
+        tc_fence_after();
         if (elect_one()) {
           const uint64_t k = desc_rows(sK(i), 0);
 #pragma unroll
           for (int u = 0; u < TILE / 16; ++u) umma_ts(tdQ, tDS(i & 1) + 8 * u, k + rows_step(u), idG, i > 0 || u != 0);
           umma_commit(kempty(i));
-          if (C::SIDE) umma_commit(dqdone(i & 1));
+          umma_commit(dqdone(i & 1));
           if (i + 1 == steps) umma_commit(done);
         }
         __syncwarp();
@@ -559,16 +630,12 @@ __global__ void __launch_bounds__(NT, 1) packed_dq_kernel(
       if (steps > 1) scores(1);
       for (int i = 0; i < steps; ++i) {
         dscores(i);
-        if (i > 0) {                                     // the other warpgroup's dS -> dQ and its next scores
-          wait(dsfull((i - 1) & 1), ((i - 1) >> 1) & 1, serr);
-          tc_fence_after();
-          if (C::SIDE && i + 1 < steps) scores(i + 1);
+        if (i > 0) {                                     // the other warpgroup's dP read -> its next S, and its dS -> dQ
+          wait(dpread((i - 1) & 1), ((i - 1) >> 1) & 1, serr);
+          if (i + 1 < steps) scores(i + 1);
           queries(i - 1);
-          if (!C::SIDE && i + 1 < steps) scores(i + 1);
         }
       }
-      wait(dsfull((steps - 1) & 1), ((steps - 1) >> 1) & 1, serr);
-      tc_fence_after();
       queries(steps - 1);
       drain_products(drained, serr);
     }
@@ -590,25 +657,37 @@ __global__ void __launch_bounds__(NT, 1) packed_dq_kernel(
 #pragma unroll
       for (int c = 0; c < 4; ++c) tmem_ld32(x_addr + 32 * c, x[c]);
       tmem_ld_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(sread(a));
+      release(sread(a), lane);
       const bool mask = k0 < w_lo || k0 + TILE - 1 > w_row;
       const int c_lo = lo - k0, c_hi = row - k0;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        if (mask) exponentials<0>(x[c], g.scale_log2, [&](int) { return nl; });
-        else exponentials<EMU>(x[c], g.scale_log2, [&](int) { return nl; });
+        if (mask) exponentials<0>(x[c], g.scale_log2, nl);
+        else exponentials<EMU>(x[c], g.scale_log2, nl);
       }
       wait(dpfull(a), ph, serr);
-      if (C::SIDE && i >= 2) wait(dqdone(a), ((i >> 1) - 1) & 1, serr);               // the last dS of this warpgroup has been read
       tc_fence_after();
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        scale_weights(x[c], x_addr + 32 * c, [&](int) { return nd; });
-        if (mask) clear_hidden(x[c], 32 * c, c_lo, c_hi);
-        store_packed(ds_addr + 16 * c, x[c]);              // where there are no side columns: into some whose dP has been read
+      for (int half = 0; half < 2; ++half) {
+        uint32_t d[2][32];
+        tmem_ld32(x_addr + 64 * half, d[0]);
+        tmem_ld32(x_addr + 64 * half + 32, d[1]);
+        tmem_ld_wait();
+        if (half) release(dpread(a), lane);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int c = 2 * half + u;
+#pragma unroll
+          for (int w = 0; w < 32; w += 2) scale_pair(x[c][w], x[c][w + 1], d[u][w], d[u][w + 1], nd);
+          if (mask) clear_hidden(x[c], 32 * c, c_lo, c_hi);  // 0 x (what a padding row's product left) is not zero
+        }
       }
+      if (i >= 2) {                                        // the last dS of this warpgroup has been read
+        wait(dqdone(a), ((i >> 1) - 1) & 1, serr);
+        tc_fence_after();
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) store_packed(ds_addr + 16 * c, x[c]);
       hand_over(dsfull(a), lane);
     }
     wait(done, 0, serr);
