@@ -29,7 +29,6 @@ using namespace packed;
 namespace {
 
 constexpr int NT = 384;
-constexpr int EMU = 2;                  // pairs of eight on the FMA pipe
 
 // aux: [2][Hq][Tp] fp32 (-lse in base 2, -delta), Tp = T rounded up to whole tiles
 template <int LANES>
@@ -116,38 +115,29 @@ struct Cfg {
 };
 static_assert(Cfg<128>::total <= 227 * 1024 && Cfg<64>::total <= 227 * 1024, "shared memory");
 
-// P = exp2(s * scale + nl) in place, nl = -lse.  Of every eight pairs EMU are computed on the FMA pipe (packed.cuh).
-template <int EMU>
-__device__ __forceinline__ void exponential_pair(uint32_t& a, uint32_t& b, f32x2 sc, f32x2 nl, int i) {
-  const f32x2 y = fma2(pair(__uint_as_float(a), __uint_as_float(b)), sc, nl);
-  float p0, p1;
-  if ((i * EMU) % 8 + EMU > 7) {
-    ex2_pair(y, p0, p1);
-  } else {
-    split(y, p0, p1);
-    p0 = ex2(p0);
-    p1 = ex2(p1);
-  }
-  a = __float_as_uint(p0);
-  b = __float_as_uint(p1);
+// P = exp2(s * scale + nl) in place, nl = -lse.  All on the special-function unit: a share of them on the FMA pipe as in the
+// forward pass was slower here (8192 x 16 heads of 64: none 517, one of eight pairs 525, two 534 us; half a row per thread and
+// twice the warps 551 us).
+__device__ __forceinline__ void exponential_pair(uint32_t& a, uint32_t& b, f32x2 sc, f32x2 nl) {
+  float y0, y1;
+  split(fma2(pair(__uint_as_float(a), __uint_as_float(b)), sc, nl), y0, y1);
+  a = __float_as_uint(ex2(y0));
+  b = __float_as_uint(ex2(y1));
 }
 // a row per thread, 32 of its columns
-template <int EMU>
 __device__ __forceinline__ void exponentials(uint32_t (&x)[32], float scale, f32x2 nl) {
   const f32x2 sc = pair(scale, scale);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) exponential_pair<EMU>(x[2 * i], x[2 * i + 1], sc, nl, i);
+  for (int i = 0; i < 16; ++i) exponential_pair(x[2 * i], x[2 * i + 1], sc, nl);
 }
 // fragments of 32 rows and 128 columns; nl: this thread's pair of every 8 columns
-template <int EMU>
 __device__ __forceinline__ void exponentials(uint32_t (&x)[2][64], float scale, const f32x2* nl) {
   const f32x2 sc = pair(scale, scale);
 #pragma unroll
   for (int u = 0; u < 16; ++u) {
     const f32x2 n = nl[4 * u];
 #pragma unroll
-    for (int v = 0; v < 4; ++v)
-      exponential_pair<EMU>(x[v >> 1][4 * u + 2 * (v & 1)], x[v >> 1][4 * u + 2 * (v & 1) + 1], sc, n, 4 * u + v);
+    for (int v = 0; v < 4; ++v) exponential_pair(x[v >> 1][4 * u + 2 * (v & 1)], x[v >> 1][4 * u + 2 * (v & 1) + 1], sc, n);
   }
 }
 // columns outside [lo, hi] to zero; c0: the first of the 32 columns
@@ -444,11 +434,11 @@ __global__ void __launch_bounds__(NT, 1) packed_dkv_kernel(
           tmem_st_16x128b_x16(p_addr + h * lower, w);
         }
       };
-      if (mask) {
-        exponentials<0>(x, g.scale_log2, nlse);
+      if (mask) {                                          // two branches with the same exponentials: see packed_dq_kernel
+        exponentials(x, g.scale_log2, nlse);
         clear();
       } else {
-        exponentials<EMU>(x, g.scale_log2, nlse);
+        exponentials(x, g.scale_log2, nlse);
       }
       if (C::SIDE && i >= 2) {                             // the product has read this warpgroup's last dS
         wait(dkdone(a), ((i >> 1) - 1) & 1, serr);
@@ -662,8 +652,10 @@ __global__ void __launch_bounds__(NT, 1) packed_dq_kernel(
       const int c_lo = lo - k0, c_hi = row - k0;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        if (mask) exponentials<0>(x[c], g.scale_log2, nl);
-        else exponentials<EMU>(x[c], g.scale_log2, nl);
+        // The exponentials belong before the wait for dP, which they hide.  Only results that come out of a branch stay there:
+        // without one the compiler moves them to their use behind the wait (8192 x 16 heads of 64: dq 293 against 237 us).
+        if (mask) exponentials(x[c], g.scale_log2, nl);
+        else exponentials(x[c], g.scale_log2, nl);
       }
       wait(dpfull(a), ph, serr);
       tc_fence_after();

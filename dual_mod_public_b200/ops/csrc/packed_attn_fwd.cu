@@ -37,8 +37,9 @@ constexpr float LAG = 8.f;              // octaves
 template <int DH>
 struct Cfg {
   static constexpr bool TURNS = DH == 128;                 // one S for both tiles
-  // pairs of eight on the FMA pipe; 8192 rows, 16 heads: D = 64 1: 188.0, 2: 188.7, 3: 196.2 us; D = 128 1: 223.9, 2: 229.9, 3: 232.8
-  static constexpr int EMU = DH == 64 ? 2 : 1;
+  // pairs of eight on the FMA pipe; 8192 rows, 16 heads: D = 64 1: 188.0, 2: 186.4, 3: 196.2 us; D = 128 0: 226.4, 1: 230.6,
+  // 2: 229.9, 3: 232.8
+  static constexpr int EMU = DH == 64 ? 2 : 0;
   static constexpr int S_STEP = TURNS ? 0 : TILE;          // tensor memory columns: S, P, O
   static constexpr int P_OFF = TURNS ? TILE : 2 * TILE + 2 * DH, O_OFF = 2 * TILE;
   static constexpr int TB = TILE * DH * 2;                 // one tile
