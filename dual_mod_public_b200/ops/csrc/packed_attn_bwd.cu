@@ -3,7 +3,8 @@
 //   p_ij = exp(s_ij - lse_i),  delta_i = do_i . o_i,  ds_ij = p_ij (do_i . v_j - delta_i)
 //   dv_j = sum_i p_ij do_i,   dk_j = scale sum_i ds_ij q_i,   dq_i = scale sum_j ds_ij k_j
 //
-// Two kernels, each owning what it writes, so nothing is accumulated through memory and results do not depend on any order:
+// Two kinds of CTA in one launch, each owning what it writes, so nothing is accumulated through memory and results do not depend
+// on any order:
 //   dkv   a CTA per (key head, 128 keys); streams the query tiles (of all heads of the group) that see the keys.  Scores are
 //         formed transposed, S^T = K Q^T and dP^T = V dO^T: a key per lane of tensor memory, so P^T and dS^T are written
 //         back there as the A operands of dV += P^T dO and dK += dS^T Q
@@ -29,36 +30,47 @@ using namespace packed;
 namespace {
 
 constexpr int NT = 384;
+constexpr int MORE = 4;
 
 // aux: [2][Hq][Tp] fp32 (-lse in base 2, -delta), Tp = T rounded up to whole tiles
 template <int LANES>
 __global__ void __launch_bounds__(256) packed_delta_kernel(const bf16* __restrict__ o, const bf16* __restrict__ go, long long g_rs,
                                                            long long g_hs, const float* __restrict__ lse, float* __restrict__ aux,
                                                            const int* __restrict__ cu, int nseq, int T, int Tp, int Hq, int D) {
-  const long long w = ((long long)blockIdx.x * 256 + threadIdx.x) / LANES;      // (row, head), LANES threads of 8 dims each
-  const int sub = threadIdx.x % LANES;
-  const long long row = w / Hq;
-  const int h = (int)(w - row * Hq);
-  if (row >= Tp) return;                                                        // whole groups leave together
-  float s = 0.f;
-  const bool inside = row < T && row >= __ldg(cu) && row < __ldg(cu + nseq);    // padding rows may hold anything
-  if (inside && sub * 8 < D) {
-    const uint4 a = *reinterpret_cast<const uint4*>(o + (row * Hq + h) * D + sub * 8);
-    const uint4 b = *reinterpret_cast<const uint4*>(go + row * g_rs + h * g_hs + sub * 8);
-    const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+  // a group of LANES threads (8 dims each) takes MORE consecutive (row, head) pairs, whose loads are in flight together
+  const long long w0 = ((long long)blockIdx.x * 256 + threadIdx.x) / LANES * MORE;
+  const int sub = threadIdx.x % LANES, begin = __ldg(cu), end = __ldg(cu + nseq);
+  uint4 a[MORE], b[MORE];
+  int row[MORE], h[MORE];
+  bool inside[MORE];
+#pragma unroll
+  for (int k = 0; k < MORE; ++k) {
+    row[k] = (int)((w0 + k) / Hq);                        // below Tp: the grid is exact
+    h[k] = (int)(w0 + k - (long long)row[k] * Hq);
+    inside[k] = row[k] < T && row[k] >= begin && row[k] < end;                  // padding rows may hold anything
+    a[k] = b[k] = make_uint4(0, 0, 0, 0);
+    if (inside[k] && sub * 8 < D) {
+      a[k] = *reinterpret_cast<const uint4*>(o + ((long long)row[k] * Hq + h[k]) * D + sub * 8);
+      b[k] = *reinterpret_cast<const uint4*>(go + row[k] * g_rs + h[k] * g_hs + sub * 8);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < MORE; ++k) {
+    const uint32_t x[4] = {a[k].x, a[k].y, a[k].z, a[k].w}, y[4] = {b[k].x, b[k].y, b[k].z, b[k].w};
+    float s = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float2 p = unpack_bf16(x[i]), q = unpack_bf16(y[i]);
       s = fmaf(p.x, q.x, s);
       s = fmaf(p.y, q.y, s);
     }
-  }
 #pragma unroll
-  for (int i = LANES / 2; i > 0; i >>= 1) s += __shfl_xor_sync(0xffffffffu, s, i);
-  if (sub == 0) {
-    const float L = inside ? lse[(long long)h * T + row] : -INFINITY;
-    aux[(long long)h * Tp + row] = L == -INFINITY ? -INFINITY : -L * LOG2E;
-    aux[((long long)Hq + h) * Tp + row] = -s;
+    for (int i = LANES / 2; i > 0; i >>= 1) s += __shfl_xor_sync(0xffffffffu, s, i);
+    if (sub == 0) {
+      const float L = inside[k] ? lse[(long long)h[k] * T + row[k]] : -INFINITY;
+      aux[(long long)h[k] * Tp + row[k]] = L == -INFINITY ? -INFINITY : -L * LOG2E;
+      aux[((long long)Hq + h[k]) * Tp + row[k]] = -s;
+    }
   }
 }
 
@@ -175,9 +187,9 @@ __device__ __forceinline__ void hand_over(uint32_t bar, int lane) {
 
 // ---------------------------------------------------------------------------------------------------------------------------
 template <int DH>
-__global__ void __launch_bounds__(NT, 1) packed_dkv_kernel(
-    const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-    const __grid_constant__ CUtensorMap tmG, bf16* __restrict__ dk, bf16* __restrict__ dv, const Geo g, int* __restrict__ gerr) {
+__device__ __forceinline__ void keys_and_values(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CUtensorMap& tmV,
+                                                const CUtensorMap& tmG, bf16* __restrict__ dk, bf16* __restrict__ dv, const Geo& g,
+                                                int block, int* __restrict__ gerr) {
   using C = Cfg<DH>;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t base = smem_u32(smem);
@@ -206,28 +218,47 @@ __global__ void __launch_bounds__(NT, 1) packed_dkv_kernel(
   volatile int* serr = reinterpret_cast<volatile int*>(smem + C::bar_off + 288);
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   // the first keys of a long sequence are seen by the most queries: they come first
-  const int kh = blockIdx.x % g.Hkv, kt = blockIdx.x / g.Hkv, key0 = kt * TILE;
-  const int last = last_query(g.cu, g.nseq, g.window, g.T, min(g.T, key0 + TILE) - 1);
-  const int nq = uniform(max(kt, last / TILE)) - kt + 1, steps = nq * g.group;     // query tiles kt .. kt + nq - 1 of each head
-
-  if (threadIdx.x == 0) {
-    *serr = 0;
-    mbar_init(own, 1);
-    mbar_init(done, 1);
-    mbar_init(drained, 1);
-    for (int a = 0; a < 2; ++a) {
-      mbar_init(sfull(a), 1);
-      mbar_init(sread(a), 4);
-      mbar_init(pfull(a), 4);
-      mbar_init(dpfull(a), 1);
-      mbar_init(dsfull(a), 4);
-      mbar_init(dpread(a), 4);
-      mbar_init(dvdone(a), 1);
-      mbar_init(dkdone(a), 1);
+  const int kh = block % g.Hkv, kt = block / g.Hkv, key0 = kt * TILE;
+  const uint32_t sK = base + C::own_off, sV = sK + C::TB;
+  auto sQ = [&](int i) { return base + C::a_off + (i % C::NA) * C::TB; };
+  auto sG = [&](int i) { return base + C::b_off + (i % C::NB) * C::TB; };
+  auto load_queries = [&](int i, int h, int q0) {
+    mbar_expect_tx(qfull(i), C::TB + 512);
+    load_tile<DH>(sQ(i), &tmQ, qfull(i), h, q0);
+    load_bulk(base + C::aux_off + (i % C::NA) * 512, g.aux + (long long)(g.Hq + h) * g.Tp + q0, 512, qfull(i));
+  };
+  auto load_gradients = [&](int i, int h, int q0) {
+    mbar_expect_tx(gfull(i), C::TB + 512);
+    load_tile<DH>(sG(i), &tmG, gfull(i), h, q0);
+    load_bulk(base + C::aux_off + (C::NA + i % C::NB) * 512, g.aux + (long long)h * g.Tp + q0, 512, gfull(i));
+  };
+  if (warp == 9) {
+    if (elect_one()) {
+      *serr = 0;
+      mbar_init(own, 1);
+      mbar_init(done, 1);
+      mbar_init(drained, 1);
+      for (int a = 0; a < 2; ++a) {
+        mbar_init(sfull(a), 1);
+        mbar_init(sread(a), 4);
+        mbar_init(pfull(a), 4);
+        mbar_init(dpfull(a), 1);
+        mbar_init(dsfull(a), 4);
+        mbar_init(dpread(a), 4);
+        mbar_init(dvdone(a), 1);
+        mbar_init(dkdone(a), 1);
+      }
+      for (int i = 0; i < C::NA; ++i) { mbar_init(qfull(i), 1); mbar_init(qempty(i), 1); }
+      for (int i = 0; i < C::NB; ++i) { mbar_init(gfull(i), 1); mbar_init(gempty(i), 1); }
+      fence_barrier_init();
+      // what does not depend on the sequences: the keys and the queries of their own tile
+      mbar_expect_tx(own, 2 * C::TB);
+      load_tile<DH>(sK, &tmK, own, kh, key0);
+      load_queries(0, kh * g.group, key0);
+      load_tile<DH>(sV, &tmV, own, kh, key0);
+      load_gradients(0, kh * g.group, key0);
     }
-    for (int i = 0; i < C::NA; ++i) { mbar_init(qfull(i), 1); mbar_init(qempty(i), 1); }
-    for (int i = 0; i < C::NB; ++i) { mbar_init(gfull(i), 1); mbar_init(gempty(i), 1); }
-    fence_barrier_init();
+    __syncwarp();
   }
   if (warp == 8) tmem_alloc(tslot, 512);
   tc_fence_before();
@@ -238,35 +269,19 @@ __global__ void __launch_bounds__(NT, 1) packed_dkv_kernel(
   // P, then dS
   auto tP = [&](int a) { return C::SIDE ? tm + 2 * TILE + 2 * DH + a * 64 : tX(a); };
   const uint32_t tdV = tm + 2 * TILE, tdK = tdV + DH;
-  const uint32_t sK = base + C::own_off, sV = sK + C::TB;
-  auto sQ = [&](int i) { return base + C::a_off + (i % C::NA) * C::TB; };
-  auto sG = [&](int i) { return base + C::b_off + (i % C::NB) * C::TB; };
+  const int last = last_query(g.cu, g.nseq, g.window, g.T, min(g.T, key0 + TILE) - 1);
+  const int nq = uniform(max(kt, last / TILE)) - kt + 1, steps = nq * g.group;     // query tiles kt .. kt + nq - 1 of each head
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");          // 2 x 216 + 72 = 3 x 168
     if (warp == 9) {
-      if (elect_one()) {
-        mbar_expect_tx(own, 2 * C::TB);
-        load_tile<DH>(sK, &tmK, own, kh, key0);
-        load_tile<DH>(sV, &tmV, own, kh, key0);
-      }
-      int i = 0, qi = 0, h = kh * g.group;
+      int i = 1, qi = nq == 1 ? 0 : 1, h = kh * g.group + (nq == 1);        // step 0 is on its way
       for (; i < steps && !*serr; ++i) {
         const int q0 = (kt + qi) * TILE;
-        const float* ax = g.aux + (long long)h * g.Tp + q0;
-        const uint32_t aux = base + C::aux_off;
         wait(qempty(i), qphase(i) ^ 1, serr);
-        if (elect_one()) {
-          mbar_expect_tx(qfull(i), C::TB + 512);
-          load_tile<DH>(sQ(i), &tmQ, qfull(i), h, q0);
-          load_bulk(aux + (i % C::NA) * 512, ax + (long long)g.Hq * g.Tp, 512, qfull(i));
-        }
+        if (elect_one()) load_queries(i, h, q0);
         wait(gempty(i), gphase(i) ^ 1, serr);
-        if (elect_one()) {
-          mbar_expect_tx(gfull(i), C::TB + 512);
-          load_tile<DH>(sG(i), &tmG, gfull(i), h, q0);
-          load_bulk(aux + (C::NA + i % C::NB) * 512, ax, 512, gfull(i));
-        }
+        if (elect_one()) load_gradients(i, h, q0);
         if (++qi == nq) { qi = 0; ++h; }
       }
       if (*serr) {          // a wait ran out: let the copies in flight land before the CTA ends
@@ -434,7 +449,7 @@ __global__ void __launch_bounds__(NT, 1) packed_dkv_kernel(
           tmem_st_16x128b_x16(p_addr + h * lower, w);
         }
       };
-      if (mask) {                                          // two branches with the same exponentials: see packed_dq_kernel
+      if (mask) {                                          // two branches with the same exponentials: see queries_only
         exponentials(x, g.scale_log2, nlse);
         clear();
       } else {
@@ -484,9 +499,9 @@ __global__ void __launch_bounds__(NT, 1) packed_dkv_kernel(
 
 // ---------------------------------------------------------------------------------------------------------------------------
 template <int DH>
-__global__ void __launch_bounds__(NT, 1) packed_dq_kernel(
-    const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-    const __grid_constant__ CUtensorMap tmG, bf16* __restrict__ dq, const Geo g, int* __restrict__ gerr) {
+__device__ __forceinline__ void queries_only(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CUtensorMap& tmV,
+                                             const CUtensorMap& tmG, bf16* __restrict__ dq, const Geo& g, int block,
+                                             int* __restrict__ gerr) {
   using C = Cfg<DH>;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t base = smem_u32(smem);
@@ -512,25 +527,43 @@ __global__ void __launch_bounds__(NT, 1) packed_dq_kernel(
   volatile uint32_t* tslot = reinterpret_cast<volatile uint32_t*>(smem + C::bar_off + 280);
   volatile int* serr = reinterpret_cast<volatile int*>(smem + C::bar_off + 288);
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int h = blockIdx.x % g.Hq, qt = g.tiles - 1 - blockIdx.x / g.Hq, row0 = qt * TILE;
-  const int kb0 = uniform(min(qt, first_key(g.cu, g.nseq, g.window, row0) / TILE)), steps = qt - kb0 + 1;
-
-  if (threadIdx.x == 0) {
-    *serr = 0;
-    mbar_init(own, 1);
-    mbar_init(done, 1);
-    mbar_init(drained, 1);
-    for (int a = 0; a < 2; ++a) {
-      mbar_init(sfull(a), 1);
-      mbar_init(sread(a), 4);
-      mbar_init(dqdone(a), 1);
-      mbar_init(dpfull(a), 1);
-      mbar_init(dsfull(a), 4);
-      mbar_init(dpread(a), 4);
+  const int h = block % g.Hq, qt = g.tiles - 1 - block / g.Hq, row0 = qt * TILE;
+  const uint32_t sQ = base + C::own_off, sG = sQ + C::TB;
+  auto sK = [&](int i) { return base + C::a_off + (i % C::NA) * C::TB; };
+  auto sV = [&](int i) { return base + C::b_off + (i % C::NB) * C::TB; };
+  const int kh = h / g.group;                              // key blocks from the diagonal down
+  auto load_keys = [&](int i) {
+    mbar_expect_tx(kfull(i), C::TB);
+    load_tile<DH>(sK(i), &tmK, kfull(i), kh, (qt - i) * TILE);
+  };
+  auto load_values = [&](int i) {
+    mbar_expect_tx(vfull(i), C::TB);
+    load_tile<DH>(sV(i), &tmV, vfull(i), kh, (qt - i) * TILE);
+  };
+  if (warp == 9) {
+    if (elect_one()) {
+      *serr = 0;
+      mbar_init(own, 1);
+      mbar_init(done, 1);
+      mbar_init(drained, 1);
+      for (int a = 0; a < 2; ++a) {
+        mbar_init(sfull(a), 1);
+        mbar_init(sread(a), 4);
+        mbar_init(dqdone(a), 1);
+        mbar_init(dpfull(a), 1);
+        mbar_init(dsfull(a), 4);
+        mbar_init(dpread(a), 4);
+      }
+      for (int i = 0; i < C::NA; ++i) { mbar_init(kfull(i), 1); mbar_init(kempty(i), 1); }
+      for (int i = 0; i < C::NB; ++i) { mbar_init(vfull(i), 1); mbar_init(vempty(i), 1); }
+      fence_barrier_init();
+      mbar_expect_tx(own, 2 * C::TB);
+      load_tile<DH>(sQ, &tmQ, own, h, row0);
+      load_keys(0);
+      load_tile<DH>(sG, &tmG, own, h, row0);
+      load_values(0);
     }
-    for (int i = 0; i < C::NA; ++i) { mbar_init(kfull(i), 1); mbar_init(kempty(i), 1); }
-    for (int i = 0; i < C::NB; ++i) { mbar_init(vfull(i), 1); mbar_init(vempty(i), 1); }
-    fence_barrier_init();
+    __syncwarp();
   }
   if (warp == 8) tmem_alloc(tslot, 512);
   tc_fence_before();
@@ -540,32 +573,17 @@ __global__ void __launch_bounds__(NT, 1) packed_dq_kernel(
   auto tX = [&](int a) { return tm + a * TILE; };                                   // S, then dP
   auto tDS = [&](int a) { return tm + 2 * TILE + DH + a * 64; };
   const uint32_t tdQ = tm + 2 * TILE;
-  const uint32_t sQ = base + C::own_off, sG = sQ + C::TB;
-  auto sK = [&](int i) { return base + C::a_off + (i % C::NA) * C::TB; };
-  auto sV = [&](int i) { return base + C::b_off + (i % C::NB) * C::TB; };
+  const int steps = qt - uniform(min(qt, first_key(g.cu, g.nseq, g.window, row0) / TILE)) + 1;
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 9) {
-      const int kh = h / g.group;
-      if (elect_one()) {
-        mbar_expect_tx(own, 2 * C::TB);
-        load_tile<DH>(sQ, &tmQ, own, h, row0);
-        load_tile<DH>(sG, &tmG, own, h, row0);
-      }
-      int i = 0;
+      int i = 1;                                           // step 0 is on its way
       for (; i < steps && !*serr; ++i) {
-        const int k0 = (kb0 + i) * TILE;
         wait(kempty(i), kphase(i) ^ 1, serr);
-        if (elect_one()) {
-          mbar_expect_tx(kfull(i), C::TB);
-          load_tile<DH>(sK(i), &tmK, kfull(i), kh, k0);
-        }
+        if (elect_one()) load_keys(i);
         wait(vempty(i), vphase(i) ^ 1, serr);
-        if (elect_one()) {
-          mbar_expect_tx(vfull(i), C::TB);
-          load_tile<DH>(sV(i), &tmV, vfull(i), kh, k0);
-        }
+        if (elect_one()) load_values(i);
       }
       if (*serr) {
         volatile int ignore = 0;
@@ -577,7 +595,7 @@ __global__ void __launch_bounds__(NT, 1) packed_dq_kernel(
       constexpr uint32_t idS = mma_desc<bf16>(TILE, TILE, 0, 0), idG = mma_desc<bf16>(TILE, DH, 0, 1);
       const int begin = max(0, __ldg(g.cu)), end = min(g.T, __ldg(g.cu + g.nseq));
       auto scores = [&](int i) {                         // S = Q K_i^T
-        const int k0 = (kb0 + i) * TILE;
+        const int k0 = (qt - i) * TILE;
         wait(kfull(i), kphase(i), serr);
         if (k0 < begin || k0 + TILE > end) blank_rows<DH>(smem + C::a_off + (i % C::NA) * C::TB, k0, begin, end, lane);
         tc_fence_after();
@@ -640,7 +658,7 @@ __global__ void __launch_bounds__(NT, 1) packed_dq_kernel(
     const f32x2 nl = pair(L, L), nd = pair(D, D);
     for (int i = a; i < steps; i += 2) {
       const uint32_t ph = (i >> 1) & 1;
-      const int k0 = (kb0 + i) * TILE;
+      const int k0 = (qt - i) * TILE;
       wait(sfull(a), ph, serr);
       tc_fence_after();
       uint32_t x[4][32];
@@ -693,15 +711,23 @@ __global__ void __launch_bounds__(NT, 1) packed_dq_kernel(
   if (threadIdx.x == 0 && *serr) atomicExch(gerr, 1);
 }
 
+// One launch for both: the dkv blocks, which have more to do, come first, and dq blocks fill the SMs that they leave.
+template <int DH>
+__global__ void __launch_bounds__(NT, 1) packed_bwd_kernel(
+    const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+    const __grid_constant__ CUtensorMap tmG, bf16* __restrict__ dq, bf16* __restrict__ dk, bf16* __restrict__ dv,
+    const __grid_constant__ Geo g, int* __restrict__ gerr) {
+  const int n = g.tiles * g.Hkv, block = blockIdx.x;
+  if (block < n) keys_and_values<DH>(tmQ, tmK, tmV, tmG, dk, dv, g, block, gerr);
+  else queries_only<DH>(tmQ, tmK, tmV, tmG, dq, g, block - n, gerr);
+}
+
 template <int DH>
 int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mg, bf16* dq, bf16* dk, bf16* dv,
            const Geo& g, int* err, cudaStream_t st) {
-  cudaError_t e = cudaFuncSetAttribute(packed_dkv_kernel<DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<DH>::total);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(packed_dq_kernel<DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<DH>::total);
+  cudaError_t e = cudaFuncSetAttribute(packed_bwd_kernel<DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<DH>::total);
   if (e != cudaSuccess) return (int)e;
-  packed_dkv_kernel<DH><<<(unsigned)(g.tiles * g.Hkv), NT, Cfg<DH>::total, st>>>(mq, mk, mv, mg, dk, dv, g, err);
-  DMB_CHECK_LAUNCH();
-  packed_dq_kernel<DH><<<(unsigned)(g.tiles * g.Hq), NT, Cfg<DH>::total, st>>>(mq, mk, mv, mg, dq, g, err);
+  packed_bwd_kernel<DH><<<(unsigned)(g.tiles * (g.Hkv + g.Hq)), NT, Cfg<DH>::total, st>>>(mq, mk, mv, mg, dq, dk, dv, g, err);
   DMB_CHECK_LAUNCH();
   return 0;
 }
@@ -724,17 +750,17 @@ extern "C" int dmb_packed_attn_bwd(const void* go, long long g_rs, long long g_h
   if (rc == 0) rc = make_map_rows(&mg, go, D, Hq, T, g_rs, g_hs);
   if (rc) return rc;
   const int tiles = (int)(((long long)T + TILE - 1) / TILE);
-  if ((long long)tiles * Hq > 0x7fffffffLL) return -1;
+  if ((long long)tiles * (Hq + Hkv) > 0x7fffffffLL) return -1;
   const Geo g{cu, aux, nseq, T, tiles * TILE, Hq, Hkv, Hq / Hkv, D, window, tiles, scale, scale * LOG2E};
   cudaStream_t st = (cudaStream_t)stream;
   const long long rows = (long long)g.Tp * Hq;
-  if (D <= 64) {
-    packed_delta_kernel<8><<<(unsigned)((rows * 8 + 255) / 256), 256, 0, st>>>((const bf16*)o, (const bf16*)go, g_rs, g_hs, lse, aux,
-                                                                                cu, nseq, T, g.Tp, Hq, D);
-  } else {
-    packed_delta_kernel<16><<<(unsigned)((rows * 16 + 255) / 256), 256, 0, st>>>((const bf16*)o, (const bf16*)go, g_rs, g_hs, lse, aux,
-                                                                                  cu, nseq, T, g.Tp, Hq, D);
-  }
+  // rows is a multiple of 128, so with 8 or 16 threads for 4 of them every block is full
+  if (D <= 64)
+    packed_delta_kernel<8><<<(unsigned)(rows / MORE * 8 / 256), 256, 0, st>>>((const bf16*)o, (const bf16*)go, g_rs, g_hs, lse, aux, cu,
+                                                                               nseq, T, g.Tp, Hq, D);
+  else
+    packed_delta_kernel<16><<<(unsigned)(rows / MORE * 16 / 256), 256, 0, st>>>((const bf16*)o, (const bf16*)go, g_rs, g_hs, lse, aux, cu,
+                                                                                 nseq, T, g.Tp, Hq, D);
   DMB_CHECK_LAUNCH();
   return D <= 64 ? launch<64>(mq, mk, mv, mg, (bf16*)dq, (bf16*)dk, (bf16*)dv, g, err, st)
                  : launch<128>(mq, mk, mv, mg, (bf16*)dq, (bf16*)dk, (bf16*)dv, g, err, st);

@@ -105,37 +105,48 @@ __global__ void __launch_bounds__(NT, 1) packed_fwd_kernel(
   // the longest rows of a long sequence first
   const int h = blockIdx.x % g.Hq, two = g.pairs - 1 - blockIdx.x / g.Hq;
   const int row0 = two * 2 * TILE;
-  // key blocks [first, last) of a tile; blocks are aligned to 128 rows, so the last one of a tile is its diagonal.  A first
-  // row without keys starts at itself: its tile's later rows begin no earlier.
-  auto first_block = [&](int a) {
-    const int r = row0 + a * TILE;
-    return r < g.T ? first_key(g.cu, g.nseq, g.window, r) / TILE : 0;
-  };
+  // key blocks [first, last) of a tile; blocks are aligned to 128 rows, so the last one of a tile is its diagonal.  They are
+  // taken from the diagonal down: the first copies then wait for nothing that has to be looked up.
   auto last_block = [&](int a) { return row0 + a * TILE < g.T ? row0 / TILE + a + 1 : 0; };
-  const int first0 = uniform(first_block(0)), first1 = uniform(first_block(1)), last0 = last_block(0), last1 = last_block(1);
-  const int B1 = max(last0, last1), B0 = last1 ? min(first0, first1) : first0;
-
-  if (threadIdx.x == 0) {
-    *serr = 0;
-    mbar_init(qfull, 1);
-    for (int a = 0; a < 2; ++a) {
-      mbar_init(sfull(a), 1);
-      mbar_init(sread(a), 4);
-      mbar_init(pfull(a), 4);
-      mbar_init(pvdone(a), 1);
+  const int last0 = last_block(0), last1 = last_block(1), B1 = max(last0, last1), kh = h / g.group;
+  if (warp == 10) {
+    if (elect_one()) {
+      *serr = 0;
+      mbar_init(qfull, 1);
+      for (int a = 0; a < 2; ++a) {
+        mbar_init(sfull(a), 1);
+        mbar_init(sread(a), 4);
+        mbar_init(pfull(a), 4);
+        mbar_init(pvdone(a), 1);
+      }
+      mbar_init(drained, C::TURNS ? 1 : 2);
+      for (int s = 0; s < C::SLOTS; ++s) {
+        mbar_init(full(s), 1);
+        mbar_init(empty(s), C::TURNS ? 1 : 2);     // one release per issuing warp
+      }
+      fence_barrier_init();
+      mbar_expect_tx(qfull, 2 * C::TB);
+      load_tile<DH>(base + C::q_off, &tmQ, qfull, h, row0);
+      load_tile<DH>(base + C::q_off + C::TB, &tmQ, qfull, h, row0 + TILE);         // rows past the end read as zero
+      for (int i = 0; i < 2; ++i) {
+        mbar_expect_tx(full(i), C::TB);
+        load_tile<DH>(base + C::ring_off + i * C::TB, i ? &tmV : &tmK, full(i), kh, (B1 - 1) * TILE);
+      }
     }
-    mbar_init(drained, C::TURNS ? 1 : 2);
-    for (int s = 0; s < C::SLOTS; ++s) {
-      mbar_init(full(s), 1);
-      mbar_init(empty(s), C::TURNS ? 1 : 2);     // one release per issuing warp
-    }
-    fence_barrier_init();
+    __syncwarp();
   }
   if (warp == 8) tmem_alloc(tslot, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tm = uniform(*tslot);
+  // A first row without keys starts at itself: its tile's later rows begin no earlier.
+  auto first_block = [&](int a) {
+    const int r = row0 + a * TILE;
+    return r < g.T ? first_key(g.cu, g.nseq, g.window, r) / TILE : 0;
+  };
+  const int first0 = uniform(first_block(0)), first1 = uniform(first_block(1));
+  const int B0 = last1 ? min(first0, first1) : first0;
   auto tS = [&](int a) { return tm + a * C::S_STEP; };
   auto tP = [&](int a) { return tm + C::P_OFF + a * (TILE / 2); };
   auto tO = [&](int a) { return tm + C::O_OFF + a * DH; };
@@ -145,19 +156,14 @@ __global__ void __launch_bounds__(NT, 1) packed_fwd_kernel(
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 10) {
       // ---------------- TMA loads: K and V of a block in turn ----------------
-      const int kh = h / g.group, n = 2 * (B1 - B0);
-      if (elect_one()) {
-        mbar_expect_tx(qfull, 2 * C::TB);
-        load_tile<DH>(base + C::q_off, &tmQ, qfull, h, row0);
-        load_tile<DH>(base + C::q_off + C::TB, &tmQ, qfull, h, row0 + TILE);   // rows past the end read as zero
-      }
-      int i = 0;
+      const int n = 2 * (B1 - B0);
+      int i = 2;                                                    // the first block is on its way
       for (; i < n && !*serr; ++i) {
         const int s = i % C::SLOTS;
         wait(empty(s), ((i / C::SLOTS) & 1) ^ 1, serr);
         if (elect_one()) {
           mbar_expect_tx(full(s), C::TB);
-          load_tile<DH>(base + C::ring_off + s * C::TB, (i & 1) ? &tmV : &tmK, full(s), kh, (B0 + (i >> 1)) * TILE);
+          load_tile<DH>(base + C::ring_off + s * C::TB, (i & 1) ? &tmV : &tmK, full(s), kh, (B1 - 1 - (i >> 1)) * TILE);
         }
       }
       if (*serr) {        // a wait ran out: let the copies in flight land before the CTA ends
@@ -171,7 +177,7 @@ __global__ void __launch_bounds__(NT, 1) packed_fwd_kernel(
       const int begin = max(0, __ldg(g.cu)), end = min(g.T, __ldg(g.cu + g.nseq));
       auto slot_full = [&](int i) { wait(full(i % C::SLOTS), (i / C::SLOTS) & 1, serr); };
       auto scores = [&](int a, int j, bool release) {               // S = Q K_j^T into columns that are free
-        const int i = 2 * (j - B0), s = i % C::SLOTS;
+        const int i = 2 * (B1 - 1 - j), s = i % C::SLOTS;
         slot_full(i);
         tc_fence_after();
         if (elect_one()) {
@@ -184,7 +190,7 @@ __global__ void __launch_bounds__(NT, 1) packed_fwd_kernel(
         __syncwarp();
       };
       auto values = [&](int a, int j, int n, bool release) {        // O += P V_j, n-th block of the tile
-        const int i = 2 * (j - B0) + 1, s = i % C::SLOTS;
+        const int i = 2 * (B1 - 1 - j) + 1, s = i % C::SLOTS;
         slot_full(i);
         if (j * TILE < begin || (j + 1) * TILE > end) blank_rows<DH>(smem + C::ring_off + s * C::TB, j * TILE, begin, end, lane);
         const uint64_t v = desc_rows(base + C::ring_off + s * C::TB, 0);
@@ -206,37 +212,37 @@ __global__ void __launch_bounds__(NT, 1) packed_fwd_kernel(
         auto turn = [&](int a, int j) {
           if (before >= 0) wait(sread(before), phase & 1, serr);
           before = a;
-          phase = j - (a ? first1 : first0);
+          phase = (a ? last1 : last0) - 1 - j;
           scores(a, j, a == 1 || !has(1, j));
         };
-        if (has(0, B0)) turn(0, B0);
-        if (has(1, B0)) turn(1, B0);
-        for (int j = B0; j < B1; ++j) {
-          if (has(0, j + 1)) turn(0, j + 1);
-          if (has(0, j)) values(0, j, j - first0, !has(1, j));
-          if (has(1, j + 1)) turn(1, j + 1);
-          if (has(1, j)) values(1, j, j - first1, true);
+        if (has(0, B1 - 1)) turn(0, B1 - 1);
+        if (has(1, B1 - 1)) turn(1, B1 - 1);
+        for (int j = B1 - 1; j >= B0; --j) {
+          if (has(0, j - 1)) turn(0, j - 1);
+          if (has(0, j)) values(0, j, last0 - 1 - j, !has(1, j));
+          if (has(1, j - 1)) turn(1, j - 1);
+          if (has(1, j)) values(1, j, last1 - 1 - j, true);
         }
       } else {
         // a warp per tile; the next scores go behind the softmax's read of the last ones
         const int a = warp - 8, b0 = a ? first1 : first0, b1 = a ? last1 : last0;
         auto skip = [&](int j) {                                    // a block of the other tile only
-          for (int i = 2 * (j - B0); i < 2 * (j - B0) + 2; ++i) {
+          for (int i = 2 * (B1 - 1 - j); i < 2 * (B1 - 1 - j) + 2; ++i) {
             slot_full(i);
             if (elect_one()) mbar_arrive(empty(i % C::SLOTS));
             __syncwarp();
           }
         };
-        for (int j = B0; j < (b1 > b0 ? b0 : B1); ++j) skip(j);
-        if (b1 > b0) scores(a, b0, true);
-        for (int j = b0, n = 0; j < b1; ++j, ++n) {
-          if (j + 1 < b1) {
+        for (int j = B1 - 1; j >= (b1 > b0 ? b1 : B0); --j) skip(j);
+        if (b1 > b0) scores(a, b1 - 1, true);
+        for (int j = b1 - 1, n = 0; j >= b0; --j, ++n) {
+          if (j > b0) {
             wait(sread(a), n & 1, serr);
-            scores(a, j + 1, true);
+            scores(a, j - 1, true);
           }
           values(a, j, n, true);
         }
-        for (int j = max(b1, B0); b1 > b0 && j < B1; ++j) skip(j);
+        for (int j = b0 - 1; b1 > b0 && j >= B0; --j) skip(j);
       }
       drain_products(drained, serr);
     }
@@ -251,7 +257,7 @@ __global__ void __launch_bounds__(NT, 1) packed_fwd_kernel(
     const int w_lo = __shfl_sync(0xffffffffu, lo, 31), w_row = row - lane;          // lo ascends with the row
     float m = -INFINITY, l = 0.f;
     int n = 0;
-    for (int j = b0; j < b1; ++j, ++n) {
+    for (int j = b1 - 1; j >= b0; --j, ++n) {
       wait(sfull(a), n & 1, serr);
       tc_fence_after();
       uint32_t x[4][32];
