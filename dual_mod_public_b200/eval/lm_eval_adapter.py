@@ -16,6 +16,9 @@ tuples or objects with `.args`.
   generation   greedy through the static-tape `GraphDecoder` (one graph launch per token) on a GPU,
                through `decode_step` otherwise; prompts longer than the context keep head + tail
                (`GEN_TRUNC=head`) or the tail
+  packed       `packed=True` (attn_mode "vanilla"): requests of different lengths without padding.  Scoring packs rows up
+               to `packed_tokens` into one forward pass and forms logits only where a continuation token is scored;
+               generation batches prompts of any lengths (`eval.packed_decode.PackedDecoder`)
   cache        `EVAL_GEN_CACHE=<jsonl>`: finished generations are appended and served on restart;
                `EVAL_CACHE_ONLY=1` answers uncached requests with "<UNCACHED>"
   ranks        under torchrun the harness shards requests by `rank / world_size` (exposed as properties)
@@ -34,6 +37,7 @@ import os
 import torch
 import torch.nn.functional as F
 
+from ..ops import token_logprobs
 from ..utils.checkpoint import load_checkpoint, model_from_checkpoint
 
 try:                                                     # optional dependency
@@ -79,7 +83,7 @@ def trunc_keep_head(toks, cap):
 
 class DualModEval(_Base):
     def __init__(self, ckpt, tokenizer=None, batch_rows=16, device=None, max_length=2048, ctx_len=None,
-                 engine_K=0, engine_chunk=64, model=None, gen_rows=8):
+                 engine_K=0, engine_chunk=64, model=None, gen_rows=8, packed=False, packed_tokens=16384):
         if _Base is not object:
             super().__init__()
         self.dev = device or ("cuda" if torch.cuda.is_available() else "cpu")
@@ -100,6 +104,9 @@ class DualModEval(_Base):
         self.bos = self.tok.bos_token_id if self.tok.bos_token_id is not None else 1
         self.batch_rows, self.engine_K, self.engine_chunk = batch_rows, engine_K, engine_chunk
         self.gen_rows = gen_rows
+        if packed and cfg.attn_mode != "vanilla":
+            raise ValueError("packed=True is for attn_mode 'vanilla'")
+        self.packed, self.packed_tokens = packed, packed_tokens
         self.len_quant = int(os.environ.get("EVAL_LEN_QUANT", "64"))
         self._engines = {}
         self._rank, self._world_size = 0, 1
@@ -185,6 +192,8 @@ class DualModEval(_Base):
     def _score_rows(self, rows):
         """rows: list of (tokens, n_continuation).  Returns [(sum logprob of the continuation, greedy?)] in
         the given order; batches are formed inside length buckets."""
+        if self.packed:
+            return self._score_packed(rows)
         order = sorted(range(len(rows)), key=lambda i: len(rows[i][0]))
         out = [None] * len(rows)
         q = self.len_quant
@@ -206,6 +215,39 @@ class DualModEval(_Base):
                 lp = logp[r, pos]
                 out[i] = (lp.gather(1, tgt[:, None]).sum().item(), bool((lp.argmax(-1) == tgt).all()))
         return out
+
+    @torch.no_grad()
+    def _score_packed(self, rows):
+        """`_score_rows` without padding: rows packed up to `packed_tokens` per forward pass."""
+        out, batch, held = [None] * len(rows), [], 0
+        for i, (toks, n_c) in enumerate(rows):
+            toks = toks[-self.max_length:]
+            if batch and held + len(toks) > self.packed_tokens:
+                self._score_pack(batch, out)
+                batch, held = [], 0
+            batch.append((i, toks, min(n_c, len(toks) - 1)))
+            held += len(toks)
+        if batch:
+            self._score_pack(batch, out)
+        return out
+
+    def _score_pack(self, batch, out):
+        edges, where, targets = [0], [], []
+        for _, toks, n_c in batch:
+            end = edges[-1] + len(toks)
+            where += range(end - n_c - 1, end - 1)               # the row before a token predicts it
+            targets += toks[len(toks) - n_c:]
+            edges.append(end)
+        idx = torch.tensor([t for _, toks, _ in batch for t in toks], device=self.dev)
+        rows, y = torch.tensor(where, device=self.dev, dtype=torch.long), torch.tensor(targets, device=self.dev, dtype=torch.long)
+        with self._amp():
+            logits = self.model(idx, cu_seqlens=edges, logit_rows=rows)[0]
+        r = token_logprobs(logits, y, top=1)
+        logp, greedy = r.logp.double().tolist(), (r.top_ids[:, 0] == y).tolist()
+        at = 0
+        for i, _, n_c in batch:
+            out[i] = (sum(logp[at:at + n_c]), all(greedy[at:at + n_c]))
+            at += n_c
 
     def loglikelihood(self, requests):
         rows = []
@@ -247,7 +289,10 @@ class DualModEval(_Base):
         """Greedy continuations of prompts of ONE length (so a single position serves the whole batch) ->
         texts.  On a GPU: the static-tape `GraphDecoder` at a fixed batch of `gen_rows` rows (short batches are
         filled with copies of the last row, so one recorded graph serves every batch); on CPU: `decode_step`.
-        The budget is capped at half the context, so a short context still keeps a prompt."""
+        The budget is capped at half the context, so a short context still keeps a prompt.  With `packed=True` the
+        prompts may have any lengths (`PackedDecoder`)."""
+        if self.packed:
+            return self._greedy_packed(prompts, max_new, stop_strs)
         n, eos = len(prompts), self.tok.eos_token_id
         x = torch.tensor(prompts, dtype=torch.long, device=self.dev)
         plen = x.shape[1]
@@ -281,6 +326,18 @@ class DualModEval(_Base):
                 logits = self.model.decode_step(nxt[:, None], plen + j, caches)
         return [self._cut(t, stop_strs) for t in toks]
 
+    def _greedy_packed(self, prompts, max_new, stop_strs):
+        from .packed_decode import PackedDecoder
+        rows = max(self.gen_rows, len(prompts))
+        P = min(-(-(max(map(len, prompts)) + max_new) // 256) * 256, self.model.cfg.max_seq_len)
+        key = ("packed", rows, P)
+        if key not in self._engines:
+            dec = PackedDecoder(self.model, rows, P)
+            self._engines[key] = dec.capture() if torch.device(self.dev).type == "cuda" else dec
+        stop = (lambda ids: any(s in self.tok.decode(ids) for s in stop_strs)) if stop_strs else None
+        ids, _ = self._engines[key].generate(prompts, max_new, eos_id=self.tok.eos_token_id, stop_fn=stop)
+        return [self._cut(t, stop_strs) for t in ids]
+
     def _greedy(self, prompt_ids, max_new, stop_strs):
         max_new = min(max_new, max(1, self.max_length // 2))
         ids = trunc_keep_head(prompt_ids, max(1, self.max_length - max_new))
@@ -288,7 +345,8 @@ class DualModEval(_Base):
 
     def generate_until(self, requests):
         """Greedy generation.  Requests are grouped by (prompt length in tokens, stop strings, budget): rows of
-        one group share their position counter, so they decode as one batch of up to `gen_rows` rows."""
+        one group share their position counter, so they decode as one batch of up to `gen_rows` rows (with
+        `packed=True` prompts of any lengths do)."""
         from collections import defaultdict
         out, groups = [None] * len(requests), defaultdict(list)
         for i, req in enumerate(requests):
@@ -305,7 +363,7 @@ class DualModEval(_Base):
             else:
                 max_new = min(max_new, max(1, self.max_length // 2))
                 ids = trunc_keep_head([self.bos] + self.tok_encode(prompt), max(1, self.max_length - max_new))
-                groups[(len(ids), until, max_new)].append((i, key, ids))
+                groups[(0 if self.packed else len(ids), until, max_new)].append((i, key, ids))
         for (_, until, max_new), items in sorted(groups.items(), key=lambda kv: kv[0][0]):
             for b0 in range(0, len(items), self.gen_rows):
                 part = items[b0:b0 + self.gen_rows]

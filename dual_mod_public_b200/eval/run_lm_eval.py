@@ -38,6 +38,7 @@ def parse_args(argv=None):
     a("--tokenizer", default="bytes", help="tokenizer folder, or 'bytes'")
     a("--num_fewshot", type=int, default=None)
     a("--ctx_len", type=int, default=None, help="evaluate at a longer context than trained (RoPE tables rebuilt)")
+    a("--packed", action="store_true", help="score and generate without padding (attn_mode vanilla only)")
     a("--engine_K", type=int, default=0, help="> 0: likelihood and generation through the training engine at this K")
     a("--engine", default="wave3d", choices=["wave3d", "wavescan"])
     a("--T_eval", type=int, default=2048)
@@ -58,9 +59,11 @@ def build_lm(args):
     common = dict(tokenizer=args.tokenizer, batch_rows=args.batch_rows, device=args.device or None,
                   ctx_len=args.ctx_len)
     if args.engine_K:
+        if args.packed:
+            raise SystemExit("--packed and --engine_K exclude each other")
         return WavefrontEval(args.ckpt, args.engine_K, T_eval=args.T_eval, engine=args.engine, gen_rows=args.gen_rows,
                              engine_kwargs=json.loads(args.engine_kwargs), **common)
-    return DualModEval(args.ckpt, max_length=args.ctx_len or args.T_eval, **common)
+    return DualModEval(args.ckpt, max_length=args.ctx_len or args.T_eval, packed=args.packed, **common)
 
 
 def out_name(args, step):

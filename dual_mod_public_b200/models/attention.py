@@ -24,6 +24,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from ..config import DualModConfig
+from ..ops.packed import packed_attention
 from .layers import LoRAGate, LoRALinear, RMSNorm, head_rms
 from .rope import apply_rope
 
@@ -251,9 +252,13 @@ class DualModAttention(nn.Module):
         return kpp, vpp
 
     # ---- full-sequence paths ----------------------------------------------------------------
-    def forward(self, xhat, cos, sin, collect=None):
-        """x̂ [B,T,d] (already normed) -> W_O o, the residual contribution."""
+    def forward(self, xhat, cos, sin, collect=None, cu_seqlens=None):
+        """x̂ [B,T,d] (already normed) -> W_O o, the residual contribution.  With `cu_seqlens` (vanilla only) x̂ is
+        [T,d], sequences packed one behind the other, cos / sin hold the angles of every row [T, dh/2] and `cu_seqlens` is
+        (the table of `packed_attention`, the position of every row in its sequence)."""
         mode = self.cfg.attn_mode
+        if cu_seqlens is not None:
+            return self._forward_packed(xhat, cos, sin, cu_seqlens)
         if mode == "vanilla":
             return self._forward_vanilla(xhat, cos, sin)
         if mode == "sequential":
@@ -295,6 +300,27 @@ class DualModAttention(nn.Module):
         else:
             o = F.scaled_dot_product_attention(q, k, v, is_causal=True, enable_gqa=gqa)
         return self.wo(o.transpose(1, 2).reshape(B, T, self.d_attn))
+
+    def _packed_qkv(self, xhat, cos, sin):
+        """x̂ [T,d], the angles of every row [T, dh/2] -> rotated q [T,h,dh], rotated k and v [T,h_kv,dh]."""
+        heads = lambda x: x.view(x.shape[0], -1, self.head_dim)
+        c, s = cos[:, None], sin[:, None]
+        return apply_rope(heads(self.wq(xhat)), c, s), apply_rope(heads(self.wk(xhat)), c, s), heads(self.project_v(xhat))
+
+    def _logn_queries(self, q, pos):
+        """q [T,h,dh] times the log-n factor of its row (position `pos`, which sees pos + 1 keys): the scores' factor."""
+        ref = self.cfg.attn_logn_ref or 0
+        if ref <= 1:
+            return q
+        f = ((pos + 1).float().log() / math.log(ref)).clamp_min(0.0)
+        return (q.float() * f[:, None, None]).to(q.dtype)
+
+    def _forward_packed(self, xhat, cos, sin, rows):
+        """`_forward_vanilla` for packed sequences; `rows` = (cu_seqlens, position of every row)."""
+        cu, pos = rows
+        q, k, v = self._packed_qkv(xhat, cos, sin)
+        o = packed_attention(self._logn_queries(q, pos), k, v, cu, window=self.cfg.local_window or 0, scale=self.scale)
+        return self.wo(o.reshape(xhat.shape[0], self.d_attn))
 
     def _read_with_raw_diagonal(self, q_r, k_self_r, v_raw, K, V):
         """Causal read over a full-sequence tape (K, V) where every position's own

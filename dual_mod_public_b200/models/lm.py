@@ -15,6 +15,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from ..config import DualModConfig
+from ..ops.packed import token_logprobs
 from .attention import DualModAttention
 from .init import init_dualmod_lm
 from .layers import RMSNorm, SwiGLU
@@ -31,8 +32,8 @@ class Block(nn.Module):
         self.mlp_norm = RMSNorm(cfg.d_model)
         self.mlp = SwiGLU(cfg.d_model, cfg.mlp_hidden)
 
-    def forward(self, x, cos, sin, collect=None):
-        x = x + self.attn(self.attn_norm(x), cos, sin, collect=collect)
+    def forward(self, x, cos, sin, collect=None, cu_seqlens=None):
+        x = x + self.attn(self.attn_norm(x), cos, sin, collect=collect, cu_seqlens=cu_seqlens)
         return x + self.mlp(self.mlp_norm(x))
 
     def decode_step(self, x_j, pos, cache, cos, sin):
@@ -70,9 +71,15 @@ class DualModLM(nn.Module):
         self.rope_cos, self.rope_sin = cos, sin
         self.cfg.max_seq_len = max_seq_len
 
-    def forward(self, idx=None, targets=None, inputs_embeds=None, collect=None):
+    def forward(self, idx=None, targets=None, inputs_embeds=None, collect=None, cu_seqlens=None, logit_rows=None):
         """(logits [B,T,V], loss or None).  `collect`: optional list of per-layer
-        dicts that receive telemetry tensors."""
+        dicts that receive telemetry tensors.
+
+        `cu_seqlens` (attn_mode "vanilla"): idx / targets are [T] (or [1,T]), sequences of any lengths packed one behind
+        the other, sequence s being the rows [cu_seqlens[s], cu_seqlens[s+1]); no row sees another sequence and positions
+        restart with each.  Returns logits [T,V] (of the rows `logit_rows` only, where given: int64 [n], targets [n])."""
+        if cu_seqlens is not None:
+            return self._forward_packed(idx, targets, inputs_embeds, cu_seqlens, logit_rows)
         x = self.tok_emb(idx) if inputs_embeds is None else inputs_embeds
         T = x.shape[1]
         assert T <= self.cfg.max_seq_len, "sequence longer than the RoPE table"
@@ -84,6 +91,40 @@ class DualModLM(nn.Module):
         if targets is not None:
             loss = F.cross_entropy(logits.float().view(-1, logits.shape[-1]),
                                    targets.reshape(-1), ignore_index=-1)
+        return logits, loss
+
+    def packed_rows(self, cu_seqlens, T, device):
+        """(table, position of every row, cos, sin) of T packed rows.  A table that the host holds (a list, a tensor on CPU)
+        is checked; one on the device is taken as it is, and positions beyond the RoPE table keep its last angle."""
+        longest = None
+        if not (isinstance(cu_seqlens, torch.Tensor) and cu_seqlens.is_cuda):
+            cu_seqlens = torch.as_tensor(cu_seqlens, dtype=torch.int32)
+            gaps = cu_seqlens.diff()
+            if cu_seqlens.dim() != 1 or len(gaps) == 0 or cu_seqlens[0] < 0 or gaps.min() < 0 or cu_seqlens[-1] > T:
+                raise ValueError(f"cu_seqlens have to ascend within [0, {T}]")
+            longest = int(gaps.max())
+        if longest is not None and longest > self.cfg.max_seq_len:
+            raise ValueError(f"a sequence of {longest} tokens is longer than the RoPE table ({self.cfg.max_seq_len})")
+        cu = cu_seqlens.to(device=device, dtype=torch.int32)
+        row = torch.arange(T, device=device, dtype=torch.int32)
+        start = cu[(torch.searchsorted(cu, row, right=True) - 1).clamp_min(0)]
+        pos = (row - start).clamp(0, self.cfg.max_seq_len - 1).long()
+        return cu, pos, self.rope_cos[pos], self.rope_sin[pos]
+
+    def _forward_packed(self, idx, targets, inputs_embeds, cu_seqlens, logit_rows):
+        if self.cfg.attn_mode != "vanilla":
+            raise ValueError("packed sequences are for attn_mode 'vanilla'")
+        x = self.tok_emb(idx.reshape(-1)) if inputs_embeds is None else inputs_embeds.reshape(-1, self.cfg.d_model)
+        cu, pos, cos, sin = self.packed_rows(cu_seqlens, x.shape[0], x.device)
+        for blk in self.blocks:
+            x = blk(x, cos, sin, cu_seqlens=(cu, pos))
+        if logit_rows is not None:
+            x = x[logit_rows]
+        logits = self.lm_head(self.norm_f(x))
+        loss = None
+        if targets is not None:
+            targets = targets.reshape(-1)
+            loss = -token_logprobs(logits, targets).logp.sum() / (targets >= 0).sum()
         return logits, loss
 
     # ---- incremental decode ----------------------------------------------------------

@@ -8,6 +8,9 @@
   --arch gdn       gated delta-rule network (`models.baselines.build_gdn`)
   --arch fbt | looped | rdepth | lstm   the small-scale baselines of the formal-language harness
 
+  --packed_docs --eos_id 2   (vanilla, ematch) rows are streams of documents that end with that token: attention and positions
+                   stay inside a document (`ops.packed_attention`, loss by `ops.token_logprobs`)
+
 Same AdamW(0.9, 0.95), weight decay on matrices only, warm-up + cosine, clip 1.0, EMA outlier batch skip
 with non-finite always skipped (`governors.SkipRule`), as the Dual-Mod arm.  Micro-batch accumulation
 runs under `no_sync()` so the gradient all-reduce happens once per optimizer step.  Checkpoints carry
@@ -60,6 +63,15 @@ def build_arch(arch, shape, vocab, T):
     raise ValueError(arch)
 
 
+def document_edges(x, eos_id):
+    """cu_seqlens (int32, on x's device) of the documents in rows x [B, T] laid one behind the other: a document ends with
+    `eos_id` or with its row."""
+    ends = x == eos_id
+    ends[:, -1] = True
+    last = ends.reshape(-1).nonzero().squeeze(-1) + 1
+    return torch.cat((last.new_zeros(1), last)).to(torch.int32)
+
+
 def logits_of(model, x):
     out = model(x)
     return out[0] if isinstance(out, tuple) else out
@@ -88,7 +100,13 @@ def main(argv=None):
     a("--seed", type=int, default=1337)
     a("--device", default="")
     a("--log_every", type=int, default=10)
+    a("--packed_docs", action="store_true", help="attend within documents only (vanilla, ematch)")
+    a("--eos_id", type=int, default=-1, help="the token that ends a document (--packed_docs)")
     args = ap.parse_args(argv)
+    if args.packed_docs and args.arch not in ("vanilla", "ematch"):
+        ap.error("--packed_docs is for --arch vanilla or ematch")
+    if args.packed_docs and args.eos_id < 0:
+        ap.error("--packed_docs needs --eos_id")
     world, rank = int(os.environ.get("WORLD_SIZE", 1)), int(os.environ.get("RANK", 0))
     local = int(os.environ.get("LOCAL_RANK", 0))
     cuda = torch.cuda.is_available() and args.device != "cpu"
@@ -131,8 +149,12 @@ def main(argv=None):
             hold = net.no_sync() if world > 1 and i < accum - 1 else contextlib.nullcontext()
             with hold:
                 with torch.autocast(dev.type, dtype=torch.bfloat16, enabled=cuda):
-                    lg = logits_of(net, x)
-                loss = F.cross_entropy(lg.float().view(-1, lg.shape[-1]), y.reshape(-1)) / accum
+                    if args.packed_docs:
+                        loss = net(x.reshape(-1), targets=y.reshape(-1), cu_seqlens=document_edges(x, args.eos_id))[1] / accum
+                    else:
+                        lg = logits_of(net, x)
+                if not args.packed_docs:
+                    loss = F.cross_entropy(lg.float().view(-1, lg.shape[-1]), y.reshape(-1)) / accum
                 loss.backward()
             loss_acc += loss.item()
         gn = torch.nn.utils.clip_grad_norm_(params, 1.0).item()
