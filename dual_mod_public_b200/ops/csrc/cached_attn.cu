@@ -255,8 +255,10 @@ template <typename T, int DH>
 int launch(const void* q, const void* k, const void* v, const int* lengths, void* o, int B, int Hkv, int blocks, const Geo& g,
            cudaStream_t st) {
   auto kern = cached_kernel<T, DH>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<DH>::smem);
-  if (e == cudaSuccess && blocks > 8) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  static std::atomic<unsigned long long> set{0};
+  if (int rc = packed::allow_smem(kern, Cfg<DH>::smem, set)) return rc;
+  cudaError_t e = cudaSuccess;
+  if (blocks > 8) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e != cudaSuccess) return (int)e;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;

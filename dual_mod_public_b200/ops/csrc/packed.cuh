@@ -3,6 +3,8 @@
 #pragma once
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "tc05.cuh"
 
 namespace packed {
@@ -266,6 +268,18 @@ inline int bind_context() {
   int d = 0;
   cudaError_t e = cudaGetDevice(&d);
   if (e == cudaSuccess) e = cudaSetDevice(d);
+  return (int)e;
+}
+
+// dynamic shared memory of a kernel, set once per device (`set`: a bit per device, one word per kernel)
+template <typename K>
+inline int allow_smem(K kernel, int bytes, std::atomic<unsigned long long>& set) {
+  int d = 0;
+  cudaError_t e = cudaGetDevice(&d);
+  if (e != cudaSuccess) return (int)e;
+  if (d < 64 && (set.load(std::memory_order_relaxed) >> d & 1)) return 0;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && d < 64) set.fetch_or(1ull << d, std::memory_order_relaxed);
   return (int)e;
 }
 

@@ -725,8 +725,8 @@ __global__ void __launch_bounds__(NT, 1) packed_bwd_kernel(
 template <int DH>
 int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mg, bf16* dq, bf16* dk, bf16* dv,
            const Geo& g, int* err, cudaStream_t st) {
-  cudaError_t e = cudaFuncSetAttribute(packed_bwd_kernel<DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<DH>::total);
-  if (e != cudaSuccess) return (int)e;
+  static std::atomic<unsigned long long> set{0};
+  if (int rc = allow_smem(packed_bwd_kernel<DH>, Cfg<DH>::total, set)) return rc;
   packed_bwd_kernel<DH><<<(unsigned)(g.tiles * (g.Hkv + g.Hq)), NT, Cfg<DH>::total, st>>>(mq, mk, mv, mg, dq, dk, dv, g, err);
   DMB_CHECK_LAUNCH();
   return 0;

@@ -372,8 +372,8 @@ template <typename T, int DH>
 int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, void* o, float* lse, const Geo& g, int* err,
            cudaStream_t st) {
   auto kern = packed_fwd_kernel<T, DH>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<DH>::total);
-  if (e != cudaSuccess) return (int)e;
+  static std::atomic<unsigned long long> set{0};
+  if (int rc = allow_smem(kern, Cfg<DH>::total, set)) return rc;
   kern<<<dim3((unsigned)((long long)g.Hq * g.pairs)), NT, Cfg<DH>::total, st>>>(mq, mk, mv, (T*)o, lse, g, err);
   DMB_CHECK_LAUNCH();
   return 0;

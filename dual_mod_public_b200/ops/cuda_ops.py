@@ -9,6 +9,7 @@ stay correct.  `launches` counts kernel launches issued by this table.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 
 import torch
@@ -111,6 +112,43 @@ def _dense_tail(t: torch.Tensor, n_tail: int) -> bool:
             return False
         exp *= t.shape[-i]
     return True
+
+
+try:                                                     # half of torch.empty's time per call
+    from torch._C._dynamo.guards import _empty_strided_cuda
+except ImportError:
+    def _empty_strided_cuda(size, stride, dtype):
+        return torch.empty_strided(size, stride, dtype=dtype, device="cuda")
+
+
+def _raw_stream(index):
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
+
+
+def _here(method):
+    """The method with the table's device as the current one: allocations, tensor maps and launches go there."""
+    @functools.wraps(method)
+    def call(self, *args, **kw):
+        index = self._index
+        if index is None:
+            index = self._index = torch.cuda.current_device() if self.device.index is None else self.device.index
+        if torch.cuda.current_device() == index:
+            return method(self, *args, **kw)
+        with torch.cuda.device(index):
+            return method(self, *args, **kw)
+    return call
+
+
+def _empty(dtype, *size):
+    """Contiguous and uninitialised, on the current device."""
+    stride, n = [], 1
+    for k in reversed(size):
+        stride.append(n)
+        n *= k if k > 1 else 1
+    return _empty_strided_cuda(size, tuple(stride[::-1]), dtype)
 
 
 class CudaOps(TorchOps):
@@ -1030,16 +1068,8 @@ class CudaOps(TorchOps):
     # ---- packed sequences (ops/packed.py) ---------------------------------------------------
     # The smallest of these calls take the device a few microseconds, so what the host does per call is kept short.
     def _launch(self, fn, what, *args):
-        """fn(*args, stream) on this table's device and its current stream."""
-        index = self._index
-        if index is None:
-            index = self._index = torch.cuda.current_device() if self.device.index is None else self.device.index
-        stream = torch._C._cuda_getCurrentRawStream(index)
-        if torch.cuda.current_device() == index:
-            rc = fn(*args, stream)
-        else:
-            with torch.cuda.device(index):
-                rc = fn(*args, stream)
+        """fn(*args, stream) on the current device, which is this table's (`_here`), and its current stream."""
+        rc = fn(*args, _raw_stream(self._index))
         if rc != 0:
             raise RuntimeError(f"{what} failed with code {rc}")
         self.launches += 1
@@ -1076,20 +1106,22 @@ class CudaOps(TorchOps):
         D = q.shape[-1]
         return (q.dtype is BF16 or q.dtype is F16) and D <= 128 and not D & 7
 
+    @_here
     def packed_attn_fwd(self, q, k, v, cu, window, scale, need_lse=True):
         if not self._packed_ok(q):
             self._fell_back("packed_attn_fwd")
             return super().packed_attn_fwd(q, k, v, cu, window, scale, need_lse)
         (q, qs), (k, ks), (v, vs) = self._rows16(q), self._rows16(k), self._rows16(v)
         T, Hq, D = q.shape
-        o = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
-        lse = torch.empty((Hq, T), dtype=F32, device=q.device) if need_lse else None
+        o = _empty(q.dtype, T, Hq, D)
+        lse = _empty(F32, Hq, T) if need_lse else None
         if T:
             self._launch(self.lib.dmb_packed_attn_fwd, "packed_attn_fwd", q.data_ptr(), *qs, k.data_ptr(), *ks, v.data_ptr(),
                          *vs, cu.data_ptr(), cu.shape[0] - 1, o.data_ptr(), lse.data_ptr() if need_lse else None, T, Hq,
                          k.shape[1], D, window, scale, q.dtype is F16, self._tc_err_ptr)
         return o, lse
 
+    @_here
     def packed_attn_bwd(self, do, q, k, v, o, lse, cu, window, scale):
         # dS = P (dP - delta) has no natural scale: in fp16 it underflows where the gradient does, so fp16 takes fp32 math
         if not self._packed_ok(q) or q.dtype is not BF16 or do.dtype is not BF16:
@@ -1098,17 +1130,15 @@ class CudaOps(TorchOps):
         (do, gs), (q, qs), (k, ks), (v, vs) = self._rows16(do), self._rows16(q), self._rows16(k), self._rows16(v)
         T, Hq, D = q.shape
         Hkv = k.shape[1]
-        dev = q.device
-        dq = torch.empty((T, Hq, D), dtype=BF16, device=dev)
-        dk = torch.empty((T, Hkv, D), dtype=BF16, device=dev)
-        dv = torch.empty((T, Hkv, D), dtype=BF16, device=dev)
+        dq, dk, dv = _empty(BF16, T, Hq, D), _empty(BF16, T, Hkv, D), _empty(BF16, T, Hkv, D)
         if T:
-            aux = torch.empty(2 * Hq * (-(-T // 128) * 128), dtype=F32, device=dev)
+            aux = _empty(F32, 2 * Hq * (-(-T // 128) * 128))
             self._launch(self.lib.dmb_packed_attn_bwd, "packed_attn_bwd", do.data_ptr(), *gs, q.data_ptr(), *qs, k.data_ptr(),
                          *ks, v.data_ptr(), *vs, o.data_ptr(), lse.data_ptr(), cu.data_ptr(), cu.shape[0] - 1, aux.data_ptr(),
                          dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), T, Hq, Hkv, D, window, scale, self._tc_err_ptr)
         return dq, dk, dv
 
+    @_here
     def cached_attn(self, q, k, v, lengths, window, scale):
         if not self._packed_ok(q):
             self._fell_back("cached_attn")
@@ -1116,7 +1146,7 @@ class CudaOps(TorchOps):
         (q, qs), (k, ks), (v, vs) = self._rows16(q), self._rows16(k), self._rows16(v)
         B, Hq, D = q.shape
         P, Hkv = k.shape[1], k.shape[2]
-        o = torch.empty((B, Hq, D), dtype=q.dtype, device=q.device)
+        o = _empty(q.dtype, B, Hq, D)
         if B == 0:
             return o
         blocks = self.cache_blocks(B * Hkv, min(P, window) if window else P)
@@ -1138,18 +1168,16 @@ class CudaOps(TorchOps):
 
     _LOGIT_TYPES = {F32: 0, BF16: 1, F16: 2}
 
+    @_here
     def token_logprobs_fwd(self, x, tokens, top, need_stats=True):
         if x.stride(1) != 1 and x.shape[1] != 1:
             x = x.contiguous()
         N, V = x.shape
-        dev = x.device
-        logp = torch.empty(N, dtype=F32, device=dev)
-        entropy = torch.empty(N, dtype=F32, device=dev)
-        stats = torch.empty((N, 2), dtype=F32, device=dev) if need_stats else None
+        logp, entropy = _empty(F32, N), _empty(F32, N)
+        stats = _empty(F32, N, 2) if need_stats else None
         top_logp = top_ids = None
         if top:
-            top_logp = torch.empty((N, top), dtype=F32, device=dev)
-            top_ids = torch.empty((N, top), dtype=torch.int64, device=dev)
+            top_logp, top_ids = _empty(F32, N, top), _empty(torch.int64, N, top)
         if N:
             self._launch(self.lib.dmb_logprob_fwd, "token_logprobs_fwd", x.data_ptr(), x.stride(0), tokens.data_ptr(), N, V,
                          self._LOGIT_TYPES[x.dtype], top, logp.data_ptr(), entropy.data_ptr(),
@@ -1157,11 +1185,12 @@ class CudaOps(TorchOps):
                          top_ids.data_ptr() if top else None)
         return logp, entropy, stats, top_logp, top_ids
 
+    @_here
     def token_logprobs_bwd(self, x, tokens, stats, entropy, g_logp, g_entropy):
         if x.stride(1) != 1 and x.shape[1] != 1:
             x = x.contiguous()
         N, V = x.shape
-        dx = torch.empty((N, V), dtype=x.dtype, device=x.device)
+        dx = _empty(x.dtype, N, V)
         if N:
             gl, gh = (None if g is None else g.float().contiguous() for g in (g_logp, g_entropy))
             self._launch(self.lib.dmb_logprob_bwd, "token_logprobs_bwd", x.data_ptr(), x.stride(0), tokens.data_ptr(), N, V,
