@@ -45,6 +45,14 @@ __device__ __forceinline__ int last_query(const int* __restrict__ cu, int n, int
   return hi;
 }
 
+// bits i of 32 columns c0 + i that lie in [lo, hi].  Masks are applied as tests of constant bits of such a word, which the
+// hardware turns into predicates seven at a time: one select per element instead of two comparisons and a select (half of the
+// blocks of documents of some hundred tokens hold a border; 8192 rows of eleven, 16 heads of 64, forward: 60 against 53 us).
+__device__ __forceinline__ uint32_t range_bits(int c0, int lo, int hi) {
+  const int a = max(lo - c0, 0), b = min(hi - c0, 31);
+  return a > b ? 0u : (0xffffffffu >> (31 - b)) & (0xffffffffu << a);
+}
+
 // ---- waits and issue --------------------------------------------------------------------------------------------------
 // A wait of a whole warp, bounded like mbar_wait: when it runs out it raises *err, and every later wait of the block returns
 // at once, so the roles run to their ends on whatever lies in shared and tensor memory (all addresses stay in range) and the

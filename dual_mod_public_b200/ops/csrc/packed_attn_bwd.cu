@@ -154,9 +154,9 @@ __device__ __forceinline__ void exponentials(uint32_t (&x)[2][64], float scale, 
 }
 // columns outside [lo, hi] to zero; c0: the first of the 32 columns
 __device__ __forceinline__ void clear_hidden(uint32_t (&x)[32], int c0, int lo, int hi) {
+  const uint32_t seen = range_bits(c0, lo, hi);
 #pragma unroll
-  for (int i = 0; i < 32; ++i)
-    if (c0 + i < lo || c0 + i > hi) x[i] = 0;
+  for (int i = 0; i < 32; ++i) x[i] = seen & (1u << i) ? x[i] : 0u;
 }
 __device__ __forceinline__ void store_packed(uint32_t taddr, const uint32_t (&x)[32]) {
   uint32_t w[16];
@@ -434,10 +434,16 @@ __device__ __forceinline__ void keys_and_values(const CUtensorMap& tmQ, const CU
           for (int e = 0; e < 2; ++e) {
             const int lo_c = first + 16 * h + 8 * e + (lane >> 2) - q0 - 2 * t4, hi_c = hi[h][e] - q0 - 2 * t4;
 #pragma unroll
-            for (int u = 0; u < 16; ++u)
+            for (int c = 0; c < 4; ++c) {
+              const uint32_t seen = range_bits(32 * c, lo_c, hi_c);
 #pragma unroll
-              for (int w = 0; w < 2; ++w)
-                if (8 * u + w < lo_c || 8 * u + w > hi_c) x[h][4 * u + 2 * e + w] = 0;
+              for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                  uint32_t& v = x[h][16 * c + 4 * u + 2 * e + w];
+                  v = seen & (1u << (8 * u + w)) ? v : 0u;
+                }
+            }
           }
       };
       auto store = [&]() {                                 // as the 16-bit operand of the next product

@@ -6,16 +6,15 @@
 // head h / (Hq / Hkv).  A tile is 128 consecutive packed rows whatever sequences they belong to, so short sequences cost no
 // padding: the keys a tile needs are one contiguous range, and each row masks to its own part of it.
 //
-// One CTA per (head, pair of query tiles), 256 rows; key blocks of 128 stream through a shared-memory ring and serve both:
-//   warps 0..3   softmax of tile 0: every thread owns one row = one lane of tensor memory
-//   warps 4..7   softmax of tile 1
-//   warps 8, 9   S = Q K^T, and O += P V with P in tensor memory
-//   warp 10      TMA loads
+// D = 128: one CTA per (head, pair of query tiles) on an SM; D = 64: one CTA per (head, query tile), two of them on an SM, which
+// start and end independently of one another (tensor memory, 512 columns, holds two tiles either way).  Key blocks of 128
+// stream through a shared-memory ring.  Per tile
+//   four softmax warps (a thread owns a row = a lane of tensor memory), and per CTA
+//   one warp that issues S = Q K^T, and O += P V with P in tensor memory, and one for the TMA loads.
 // Scores stay in tensor memory only until the softmax has read them into registers, and P has columns of its own, so the next
-// scores are formed while the exponentials of the last ones run.  D = 64: both tiles have 128 columns for S (512 columns: 2 x
-// (128 S + 64 P + 64 O)).  D = 128: they take turns with one S (128 + 2 x (64 P + 128 O)).  The turns cost little, since S is
-// held for a product, its latency and one read, and they keep the two tiles half a block apart: one tile's exponentials run
-// while the tensor pipe works for the other.
+// scores are formed while the exponentials of the last ones run.  D = 64: 128 columns S, 64 P, 64 O.  D = 128: the two tiles
+// take turns with one S (128 + 2 x (64 P + 128 O)).  The turns cost little, since S is held for a product, its latency and one
+// read, and they keep the two tiles half a block apart: one tile's exponentials run while the tensor pipe works for the other.
 //
 // What bounds: 128 x 128 exponentials take 1024 cycles of the special-function unit, as long as the products at D = 128 and
 // twice as long at D = 64.  So of every eight pairs EMU are computed by a polynomial on the FMA pipe (packed.cuh), in blocks
@@ -31,27 +30,28 @@ using namespace packed;
 
 namespace {
 
-constexpr int NT = 384;                 // two softmax warpgroups, one for issue and loads (one of its warps idles)
 constexpr float LAG = 8.f;              // octaves
 
 template <int DH>
 struct Cfg {
-  static constexpr bool TURNS = DH == 128;                 // one S for both tiles
+  static constexpr int TILES = DH == 128 ? 2 : 1;
+  static constexpr bool TURNS = TILES == 2;                // one S for both tiles
+  static constexpr int NT = (TILES + 1) * 128, ISSUE = TILES * 4, LOAD = ISSUE + 1;      // threads; the issuing and loading warps
+  static constexpr int COLS = TILES * 256;                 // tensor memory
   // pairs of eight on the FMA pipe; 8192 rows, 16 heads: D = 64 1: 188.0, 2: 186.4, 3: 196.2 us; D = 128 0: 226.4, 1: 230.6,
   // 2: 229.9, 3: 232.8
   static constexpr int EMU = DH == 64 ? 2 : 0;
-  static constexpr int S_STEP = TURNS ? 0 : TILE;          // tensor memory columns: S, P, O
-  static constexpr int P_OFF = TURNS ? TILE : 2 * TILE + 2 * DH, O_OFF = 2 * TILE;
+  static constexpr int P_OFF = TILE, O_OFF = TILE + TILES * 64;        // S, then P and O of each tile
   static constexpr int TB = TILE * DH * 2;                 // one tile
-  static constexpr int SLOTS = DH == 128 ? 5 : 8;
-  static constexpr int q_off = 0, ring_off = 2 * TB;
+  static constexpr int SLOTS = 5;
+  static constexpr int q_off = 0, ring_off = TILES * TB;
   static constexpr int bar_off = ring_off + SLOTS * TB;
   static constexpr int total = bar_off + 256;
 };
 
 struct Geo {
   const int* cu;
-  int nseq, T, Hq, group, D, window, pairs;
+  int nseq, T, Hq, group, D, window, units;
   float scale_log2;
 };
 
@@ -78,7 +78,7 @@ __device__ __forceinline__ f32x2 weights(const uint32_t (&x)[32], float scale, f
 }
 
 template <typename T, int DH>
-__global__ void __launch_bounds__(NT, 1) packed_fwd_kernel(
+__global__ void __launch_bounds__(Cfg<DH>::NT, 3 - Cfg<DH>::TILES) packed_fwd_kernel(
     const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
     T* __restrict__ out, float* __restrict__ lse, const Geo g, int* __restrict__ gerr) {
   using C = Cfg<DH>;
@@ -103,13 +103,12 @@ __global__ void __launch_bounds__(NT, 1) packed_fwd_kernel(
 
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   // the longest rows of a long sequence first
-  const int h = blockIdx.x % g.Hq, two = g.pairs - 1 - blockIdx.x / g.Hq;
-  const int row0 = two * 2 * TILE;
+  const int h = blockIdx.x % g.Hq, row0 = (g.units - 1 - blockIdx.x / g.Hq) * C::TILES * TILE;
   // key blocks [first, last) of a tile; blocks are aligned to 128 rows, so the last one of a tile is its diagonal.  They are
   // taken from the diagonal down: the first copies then wait for nothing that has to be looked up.
-  auto last_block = [&](int a) { return row0 + a * TILE < g.T ? row0 / TILE + a + 1 : 0; };
+  auto last_block = [&](int a) { return a < C::TILES && row0 + a * TILE < g.T ? row0 / TILE + a + 1 : 0; };
   const int last0 = last_block(0), last1 = last_block(1), B1 = max(last0, last1), kh = h / g.group;
-  if (warp == 10) {
+  if (warp == C::LOAD) {
     if (elect_one()) {
       *serr = 0;
       mbar_init(qfull, 1);
@@ -119,15 +118,14 @@ __global__ void __launch_bounds__(NT, 1) packed_fwd_kernel(
         mbar_init(pfull(a), 4);
         mbar_init(pvdone(a), 1);
       }
-      mbar_init(drained, C::TURNS ? 1 : 2);
+      mbar_init(drained, 1);
       for (int s = 0; s < C::SLOTS; ++s) {
         mbar_init(full(s), 1);
-        mbar_init(empty(s), C::TURNS ? 1 : 2);     // one release per issuing warp
+        mbar_init(empty(s), 1);
       }
       fence_barrier_init();
-      mbar_expect_tx(qfull, 2 * C::TB);
-      load_tile<DH>(base + C::q_off, &tmQ, qfull, h, row0);
-      load_tile<DH>(base + C::q_off + C::TB, &tmQ, qfull, h, row0 + TILE);         // rows past the end read as zero
+      mbar_expect_tx(qfull, C::TILES * C::TB);                                     // rows past the end read as zero
+      for (int a = 0; a < C::TILES; ++a) load_tile<DH>(base + C::q_off + a * C::TB, &tmQ, qfull, h, row0 + a * TILE);
       for (int i = 0; i < 2; ++i) {
         mbar_expect_tx(full(i), C::TB);
         load_tile<DH>(base + C::ring_off + i * C::TB, i ? &tmV : &tmK, full(i), kh, (B1 - 1) * TILE);
@@ -135,7 +133,7 @@ __global__ void __launch_bounds__(NT, 1) packed_fwd_kernel(
     }
     __syncwarp();
   }
-  if (warp == 8) tmem_alloc(tslot, 512);
+  if (warp == C::ISSUE) tmem_alloc(tslot, C::COLS);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -143,18 +141,18 @@ __global__ void __launch_bounds__(NT, 1) packed_fwd_kernel(
   // A first row without keys starts at itself: its tile's later rows begin no earlier.
   auto first_block = [&](int a) {
     const int r = row0 + a * TILE;
-    return r < g.T ? first_key(g.cu, g.nseq, g.window, r) / TILE : 0;
+    return a < C::TILES && r < g.T ? first_key(g.cu, g.nseq, g.window, r) / TILE : 0;
   };
   const int first0 = uniform(first_block(0)), first1 = uniform(first_block(1));
   const int B0 = last1 ? min(first0, first1) : first0;
-  auto tS = [&](int a) { return tm + a * C::S_STEP; };
+  const uint32_t tS = tm;
   auto tP = [&](int a) { return tm + C::P_OFF + a * (TILE / 2); };
   auto tO = [&](int a) { return tm + C::O_OFF + a * DH; };
 
-  // 384 threads launch with 168 registers each; 2 x 216 + 72 = 3 x 168
-  if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    if (warp == 10) {
+  // 384 threads launch with 168 registers each, 2 x 216 + 72 = 3 x 168; 256 (twice on an SM) with 128, 216 + 40 = 2 x 128
+  if (warp >= C::ISSUE) {
+    if (C::TILES == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;"); else asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == C::LOAD) {
       // ---------------- TMA loads: K and V of a block in turn ----------------
       const int n = 2 * (B1 - B0);
       int i = 2;                                                    // the first block is on its way
@@ -171,7 +169,7 @@ __global__ void __launch_bounds__(NT, 1) packed_fwd_kernel(
         mbar_wait(qfull, 0, &ignore);
         for (int u = max(0, i - C::SLOTS); u < i; ++u) mbar_wait(full(u % C::SLOTS), (u / C::SLOTS) & 1, &ignore);
       }
-    } else if (warp < (C::TURNS ? 9 : 10)) {
+    } else if (warp == C::ISSUE) {
       // ---------------- products (the whole warp waits, one lane issues) ----------------
       constexpr uint32_t idS = mma_desc<T>(TILE, TILE, 0, 0), idO = mma_desc<T>(TILE, DH, 0, 1);
       const int begin = max(0, __ldg(g.cu)), end = min(g.T, __ldg(g.cu + g.nseq));
@@ -183,7 +181,7 @@ __global__ void __launch_bounds__(NT, 1) packed_fwd_kernel(
         if (elect_one()) {
           const uint64_t q = desc_dims(base + C::q_off + a * C::TB, 0), k = desc_dims(base + C::ring_off + s * C::TB, 0);
 #pragma unroll
-          for (int u = 0; u < DH / 16; ++u) umma_bf16(tS(a), q + dims_step(u), k + dims_step(u), idS, u != 0);
+          for (int u = 0; u < DH / 16; ++u) umma_bf16(tS, q + dims_step(u), k + dims_step(u), idS, u != 0);
           umma_commit(sfull(a));
           if (release) umma_commit(empty(s));
         }
@@ -224,25 +222,15 @@ __global__ void __launch_bounds__(NT, 1) packed_fwd_kernel(
           if (has(1, j)) values(1, j, last1 - 1 - j, true);
         }
       } else {
-        // a warp per tile; the next scores go behind the softmax's read of the last ones
-        const int a = warp - 8, b0 = a ? first1 : first0, b1 = a ? last1 : last0;
-        auto skip = [&](int j) {                                    // a block of the other tile only
-          for (int i = 2 * (B1 - 1 - j); i < 2 * (B1 - 1 - j) + 2; ++i) {
-            slot_full(i);
-            if (elect_one()) mbar_arrive(empty(i % C::SLOTS));
-            __syncwarp();
+        // the next scores go behind the softmax's read of the last ones
+        scores(0, B1 - 1, true);
+        for (int j = B1 - 1, n = 0; j >= B0; --j, ++n) {
+          if (j > B0) {
+            wait(sread(0), n & 1, serr);
+            scores(0, j - 1, true);
           }
-        };
-        for (int j = B1 - 1; j >= (b1 > b0 ? b1 : B0); --j) skip(j);
-        if (b1 > b0) scores(a, b1 - 1, true);
-        for (int j = b1 - 1, n = 0; j >= b0; --j, ++n) {
-          if (j > b0) {
-            wait(sread(a), n & 1, serr);
-            scores(a, j - 1, true);
-          }
-          values(a, j, n, true);
+          values(0, j, n, true);
         }
-        for (int j = b0 - 1; b1 > b0 && j >= B0; --j) skip(j);
       }
       drain_products(drained, serr);
     }
@@ -252,7 +240,7 @@ __global__ void __launch_bounds__(NT, 1) packed_fwd_kernel(
     const int a = warp >> 2, b0 = a ? first1 : first0, b1 = a ? last1 : last0;
     const int row = row0 + a * TILE + (warp & 3) * 32 + lane;
     const uint32_t tl = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_addr = tS(a) + tl, o_addr = tO(a) + tl, p_addr = tP(a) + tl;
+    const uint32_t s_addr = tS + tl, o_addr = tO(a) + tl, p_addr = tP(a) + tl;
     const int lo = row < g.T ? first_key(g.cu, g.nseq, g.window, row) : row + 1;
     const int w_lo = __shfl_sync(0xffffffffu, lo, 31), w_row = row - lane;          // lo ascends with the row
     float m = -INFINITY, l = 0.f;
@@ -270,10 +258,12 @@ __global__ void __launch_bounds__(NT, 1) packed_fwd_kernel(
       const int k0 = j * TILE;
       const bool mask = k0 < w_lo || k0 + TILE - 1 > w_row;          // some row of this warp hides some key of this block
       if (mask) {
-        const int c_lo = lo - k0, c_hi = row - k0;
 #pragma unroll
-        for (int c = 0; c < 128; ++c)
-          if (c < c_lo || c > c_hi) x[c >> 5][c & 31] = 0xff800000u;            // -inf
+        for (int c = 0; c < 4; ++c) {
+          const uint32_t seen = range_bits(k0 + 32 * c, lo, row);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) x[c][i] = seen & (1u << i) ? x[c][i] : 0xff800000u;      // -inf
+        }
       }
       float mx[4];
 #pragma unroll
@@ -364,7 +354,7 @@ __global__ void __launch_bounds__(NT, 1) packed_fwd_kernel(
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 8) tmem_dealloc(tm, 512);
+  if (warp == C::ISSUE) tmem_dealloc(tm, C::COLS);
   if (threadIdx.x == 0 && *serr) atomicExch(gerr, 1);
 }
 
@@ -374,7 +364,7 @@ int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, 
   auto kern = packed_fwd_kernel<T, DH>;
   static std::atomic<unsigned long long> set{0};
   if (int rc = allow_smem(kern, Cfg<DH>::total, set)) return rc;
-  kern<<<dim3((unsigned)((long long)g.Hq * g.pairs)), NT, Cfg<DH>::total, st>>>(mq, mk, mv, (T*)o, lse, g, err);
+  kern<<<(unsigned)(g.Hq * g.units), Cfg<DH>::NT, Cfg<DH>::total, st>>>(mq, mk, mv, (T*)o, lse, g, err);
   DMB_CHECK_LAUNCH();
   return 0;
 }
@@ -395,9 +385,9 @@ extern "C" int dmb_packed_attn_fwd(const void* q, long long q_rs, long long q_hs
   if (rc == 0) rc = make_map_rows(&mk, k, D, Hkv, T, k_rs, k_hs);
   if (rc == 0) rc = make_map_rows(&mv, v, D, Hkv, T, v_rs, v_hs);
   if (rc) return rc;
-  const int pairs = (int)(((long long)T + 2 * TILE - 1) / (2 * TILE));
-  if ((long long)pairs * Hq > 0x7fffffffLL) return -1;
-  const Geo g{cu, nseq, T, Hq, Hq / Hkv, D, window, pairs, scale * LOG2E};
+  const int rows = (D <= 64 ? Cfg<64>::TILES : Cfg<128>::TILES) * TILE, units = (int)(((long long)T + rows - 1) / rows);
+  if ((long long)units * Hq > 0x7fffffffLL) return -1;
+  const Geo g{cu, nseq, T, Hq, Hq / Hkv, D, window, units, scale * LOG2E};
   cudaStream_t st = (cudaStream_t)stream;
   if (half) return D <= 64 ? launch<__half, 64>(mq, mk, mv, o, lse, g, err, st) : launch<__half, 128>(mq, mk, mv, o, lse, g, err, st);
   return D <= 64 ? launch<bf16, 64>(mq, mk, mv, o, lse, g, err, st) : launch<bf16, 128>(mq, mk, mv, o, lse, g, err, st);
