@@ -12,13 +12,13 @@
 // The price is that S and dP are formed twice (seven products of 128 x 128 x D per tile instead of five); one kernel would
 // have to add dQ tiles through memory in whatever order its CTAs run.
 //
-// Both take the steps of the stream in turn on two warpgroups (warps 0..3 the even steps, 4..7 the odd ones; a thread owns a
-// whole row of a step's 128 x 128 scores), because the parts of a step depend on one another: product, 500 cycles until its
-// result is seen, exponentials, product.  While one warpgroup waits, the other computes.  Warp 8 issues all products in one
-// fixed order, warp 9 loads.  Tensor memory holds the accumulators and per warpgroup 128 columns for S, then dP, and 64 for the
-// 16-bit operands (dkv: P, then dS; dq: dS): dP is formed while the exponentials run, and the next S as soon as dP has been
-// read.  At D = 128 the accumulators of dkv leave no such columns: P and dS overwrite S and dP, dP follows the product that
-// reads P, and the next S the one that reads dS.
+// The parts of a step depend on one another: product, 500 cycles until its result is seen, exponentials, product.  So two steps
+// are in work on an SM at any time, each on four math warps (a thread owns a row of the step's 128 x 128 scores, or the fragment
+// of an MMA): at D = 64 in two CTAs of 256 columns of tensor memory, which also start and end independently of one another; at
+// D = 128, where the accumulators fill the columns, in one CTA whose two sets of warps take the steps in turn.  One warp issues
+// all products in a fixed order, one loads.  Tensor memory holds the accumulators and per set 128 columns for S, then dP.  dkv: P
+// and dS overwrite S and dP as they are made, dP follows the product that reads P, and the next S the one that reads dS.  dq: 64
+// more columns for dS, so that dP is formed while the exponentials run, and the next S as soon as dP has been read.
 // P and dS are rounded to bf16 (relative 2^-8 at most, as o was); everything else is fp32.
 //
 // A first small kernel forms -delta and -lse in base 2 (-inf for rows without keys and for the padding of the last tile, which
@@ -29,7 +29,6 @@ using namespace packed;
 
 namespace {
 
-constexpr int NT = 384;
 constexpr int MORE = 4;
 
 // aux: [2][Hq][Tp] fp32 (-lse in base 2, -delta), Tp = T rounded up to whole tiles
@@ -115,17 +114,20 @@ __device__ __forceinline__ void store_row(uint32_t taddr, bf16* dst, int D, floa
 
 template <int DH>
 struct Cfg {
-  static constexpr bool SIDE = DH == 64;                   // dkv: columns for the 16-bit operands
+  static constexpr int SETS = DH == 128 ? 2 : 1;           // steps in work in a CTA
+  static constexpr int NT = (SETS + 1) * 128, ISSUE = SETS * 4, LOAD = ISSUE + 1, COLS = SETS * 256;
   static constexpr int TB = TILE * DH * 2;
   // rings of single tiles: A (dkv: queries, dq: keys) is read by the first and by the last product of a step, B by those between
-  static constexpr int NA = DH == 128 ? 3 : 4, NB = DH == 128 ? 2 : 4;
+  static constexpr int NA = SETS + 1, NB = 2;
   static constexpr int own_off = 0, a_off = 2 * TB, b_off = a_off + NA * TB;
   // dkv: 128 -delta per tile of A and 128 -lse per tile of B, so each lies there until the math warps have read it
   static constexpr int aux_off = b_off + NB * TB;
   static constexpr int bar_off = aux_off + (NA + NB) * 512;
   static constexpr int total = bar_off + 304;
+  static __device__ __forceinline__ int set(int i) { return i % SETS; }                       // of step i
+  static __device__ __forceinline__ uint32_t phase(int i) { return (uint32_t)(i / SETS) & 1; }  // of its set's barriers
 };
-static_assert(Cfg<128>::total <= 227 * 1024 && Cfg<64>::total <= 227 * 1024, "shared memory");
+static_assert(Cfg<128>::total <= 227 * 1024 && Cfg<64>::total <= 113 * 1024, "shared memory");
 
 // P = exp2(s * scale + nl) in place, nl = -lse.  All on the special-function unit: a share of them on the FMA pipe as in the
 // forward pass was slower here (8192 x 16 heads of 64: none 517, one of eight pairs 525, two 534 us; half a row per thread and
@@ -198,20 +200,16 @@ __device__ __forceinline__ void keys_and_values(const CUtensorMap& tmQ, const CU
     return;
   }
   const uint32_t bar0 = base + C::bar_off;
-  // barriers: own, done, drained, sfull[2], sread[2], pfull[2], dpfull[2], dsfull[2], dpread[2], dvdone[2], dkdone[2], then the rings'
+  // barriers: own, done, drained, sfull[2], pfull[2], dpfull[2], dsfull[2], then the rings'
   const uint32_t own = bar0, done = bar0 + 8, drained = bar0 + 16;
   auto sfull = [&](int a) { return bar0 + 24 + 8u * a; };
-  auto sread = [&](int a) { return bar0 + 40 + 8u * a; };
-  auto pfull = [&](int a) { return bar0 + 56 + 8u * a; };
-  auto dpfull = [&](int a) { return bar0 + 72 + 8u * a; };
-  auto dsfull = [&](int a) { return bar0 + 88 + 8u * a; };
-  auto dpread = [&](int a) { return bar0 + 104 + 8u * a; };
-  auto dvdone = [&](int a) { return bar0 + 120 + 8u * a; };
-  auto dkdone = [&](int a) { return bar0 + 136 + 8u * a; };
-  auto qfull = [&](int i) { return bar0 + 152 + 8u * (i % C::NA); };
-  auto qempty = [&](int i) { return bar0 + 152 + 8u * (C::NA + i % C::NA); };
-  auto gfull = [&](int i) { return bar0 + 152 + 8u * (2 * C::NA + i % C::NB); };
-  auto gempty = [&](int i) { return bar0 + 152 + 8u * (2 * C::NA + C::NB + i % C::NB); };
+  auto pfull = [&](int a) { return bar0 + 40 + 8u * a; };
+  auto dpfull = [&](int a) { return bar0 + 56 + 8u * a; };
+  auto dsfull = [&](int a) { return bar0 + 72 + 8u * a; };
+  auto qfull = [&](int i) { return bar0 + 88 + 8u * (i % C::NA); };
+  auto qempty = [&](int i) { return bar0 + 88 + 8u * (C::NA + i % C::NA); };
+  auto gfull = [&](int i) { return bar0 + 88 + 8u * (2 * C::NA + i % C::NB); };
+  auto gempty = [&](int i) { return bar0 + 88 + 8u * (2 * C::NA + C::NB + i % C::NB); };
   auto qphase = [](int i) { return (uint32_t)(i / C::NA) & 1; };
   auto gphase = [](int i) { return (uint32_t)(i / C::NB) & 1; };
   volatile uint32_t* tslot = reinterpret_cast<volatile uint32_t*>(smem + C::bar_off + 280);
@@ -232,7 +230,7 @@ __device__ __forceinline__ void keys_and_values(const CUtensorMap& tmQ, const CU
     load_tile<DH>(sG(i), &tmG, gfull(i), h, q0);
     load_bulk(base + C::aux_off + (C::NA + i % C::NB) * 512, g.aux + (long long)h * g.Tp + q0, 512, gfull(i));
   };
-  if (warp == 9) {
+  if (warp == C::LOAD) {
     if (elect_one()) {
       *serr = 0;
       mbar_init(own, 1);
@@ -240,13 +238,9 @@ __device__ __forceinline__ void keys_and_values(const CUtensorMap& tmQ, const CU
       mbar_init(drained, 1);
       for (int a = 0; a < 2; ++a) {
         mbar_init(sfull(a), 1);
-        mbar_init(sread(a), 4);
         mbar_init(pfull(a), 4);
         mbar_init(dpfull(a), 1);
         mbar_init(dsfull(a), 4);
-        mbar_init(dpread(a), 4);
-        mbar_init(dvdone(a), 1);
-        mbar_init(dkdone(a), 1);
       }
       for (int i = 0; i < C::NA; ++i) { mbar_init(qfull(i), 1); mbar_init(qempty(i), 1); }
       for (int i = 0; i < C::NB; ++i) { mbar_init(gfull(i), 1); mbar_init(gempty(i), 1); }
@@ -260,21 +254,20 @@ __device__ __forceinline__ void keys_and_values(const CUtensorMap& tmQ, const CU
     }
     __syncwarp();
   }
-  if (warp == 8) tmem_alloc(tslot, 512);
+  if (warp == C::ISSUE) tmem_alloc(tslot, C::COLS);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tm = uniform(*tslot);
-  auto tX = [&](int a) { return tm + a * TILE; };                                   // S, then dP
-  // P, then dS
-  auto tP = [&](int a) { return C::SIDE ? tm + 2 * TILE + 2 * DH + a * 64 : tX(a); };
-  const uint32_t tdV = tm + 2 * TILE, tdK = tdV + DH;
+  auto tX = [&](int a) { return tm + a * TILE; };                                   // S, P, dP, dS
+  const uint32_t tdV = tm + C::SETS * TILE, tdK = tdV + DH;
   const int last = last_query(g.cu, g.nseq, g.window, g.T, min(g.T, key0 + TILE) - 1);
   const int nq = uniform(max(kt, last / TILE)) - kt + 1, steps = nq * g.group;     // query tiles kt .. kt + nq - 1 of each head
 
-  if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");          // 2 x 216 + 72 = 3 x 168
-    if (warp == 9) {
+  if (warp >= C::ISSUE) {
+    // 384 threads launch with 168 registers each, 2 x 216 + 72 = 3 x 168; 256 (twice on an SM) with 128, 216 + 40 = 2 x 128
+    if (C::SETS == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;"); else asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == C::LOAD) {
       int i = 1, qi = nq == 1 ? 0 : 1, h = kh * g.group + (nq == 1);        // step 0 is on its way
       for (; i < steps && !*serr; ++i) {
         const int q0 = (kt + qi) * TILE;
@@ -290,7 +283,7 @@ __device__ __forceinline__ void keys_and_values(const CUtensorMap& tmQ, const CU
         for (int u = max(0, i - C::NA); u < i; ++u) mbar_wait(qfull(u), qphase(u), &ignore);
         for (int u = max(0, i - C::NB); u < i; ++u) mbar_wait(gfull(u), gphase(u), &ignore);
       }
-    } else if (warp == 8) {
+    } else if (warp == C::ISSUE) {
       constexpr uint32_t idS = mma_desc<bf16>(TILE, TILE, 0, 0), idG = mma_desc<bf16>(TILE, DH, 0, 1);
       const int begin = max(0, __ldg(g.cu)), end = min(g.T, __ldg(g.cu + g.nseq));
       auto clean = [&](int off, int q0) {                // the padding rows of a tile that has just arrived
@@ -303,42 +296,39 @@ __device__ __forceinline__ void keys_and_values(const CUtensorMap& tmQ, const CU
         if (elect_one()) {
           const uint64_t k = desc_dims(sK, 0), q = desc_dims(sQ(i), 0);
 #pragma unroll
-          for (int u = 0; u < DH / 16; ++u) umma_bf16(tX(i & 1), k + dims_step(u), q + dims_step(u), idS, u != 0);
-          umma_commit(sfull(i & 1));
+          for (int u = 0; u < DH / 16; ++u) umma_bf16(tX(C::set(i)), k + dims_step(u), q + dims_step(u), idS, u != 0);
+          umma_commit(sfull(C::set(i)));
         }
         __syncwarp();
       };
-      auto dscores = [&](int i, bool release) {          // dP^T = V dO_i^T
+      auto dscores = [&](int i) {                        // dP^T = V dO_i^T
         tc_fence_after();
         if (elect_one()) {
           const uint64_t v = desc_dims(sV, 0), go = desc_dims(sG(i), 0);
 #pragma unroll
-          for (int u = 0; u < DH / 16; ++u) umma_bf16(tX(i & 1), v + dims_step(u), go + dims_step(u), idS, u != 0);
-          umma_commit(dpfull(i & 1));
-          if (release) umma_commit(gempty(i));
+          for (int u = 0; u < DH / 16; ++u) umma_bf16(tX(C::set(i)), v + dims_step(u), go + dims_step(u), idS, u != 0);
+          umma_commit(dpfull(C::set(i)));
+          umma_commit(gempty(i));
         }
         __syncwarp();
       };
-      auto values = [&](int i, bool release) {           // dV += P^T dO_i
+      auto values = [&](int i) {                         // dV += P^T dO_i
         tc_fence_after();
         if (elect_one()) {
           const uint64_t go = desc_rows(sG(i), 0);
 #pragma unroll
-          for (int u = 0; u < TILE / 16; ++u) umma_ts(tdV, tP(i & 1) + 8 * u, go + rows_step(u), idG, i > 0 || u != 0);
-          if (release) umma_commit(gempty(i));
-          if (C::SIDE) umma_commit(dvdone(i & 1));
+          for (int u = 0; u < TILE / 16; ++u) umma_ts(tdV, tX(C::set(i)) + 8 * u, go + rows_step(u), idG, i > 0 || u != 0);
         }
         __syncwarp();
       };
       auto keys = [&](int i) {                           // dK += dS^T Q_i
-        wait(dsfull(i & 1), (i >> 1) & 1, serr);
+        wait(dsfull(C::set(i)), C::phase(i), serr);
         tc_fence_after();
         if (elect_one()) {
           const uint64_t q = desc_rows(sQ(i), 0);
 #pragma unroll
-          for (int u = 0; u < TILE / 16; ++u) umma_ts(tdK, tP(i & 1) + 8 * u, q + rows_step(u), idG, i > 0 || u != 0);
+          for (int u = 0; u < TILE / 16; ++u) umma_ts(tdK, tX(C::set(i)) + 8 * u, q + rows_step(u), idG, i > 0 || u != 0);
           umma_commit(qempty(i));
-          if (C::SIDE) umma_commit(dkdone(i & 1));
           if (i + 1 == steps) umma_commit(done);
         }
         __syncwarp();
@@ -348,43 +338,32 @@ __device__ __forceinline__ void keys_and_values(const CUtensorMap& tmQ, const CU
       auto next = [&](int v) { return v + TILE == key0 + nq * TILE ? key0 : v + TILE; };
       scores(0, ahead0);
       ahead0 = next(ahead0);
-      if (steps > 1) { scores(1, ahead0); ahead0 = next(ahead0); }
+      if (C::SETS > 1 && steps > 1) { scores(1, ahead0); ahead0 = next(ahead0); }
       auto gradient_tile = [&](int i) {
         wait(gfull(i), gphase(i), serr);
         clean(C::b_off + (i % C::NB) * C::TB, q0);
         q0 = next(q0);
       };
-      auto next_scores = [&](int i) {                    // of the warpgroup of step i
-        if (i + 2 < steps) { scores(i + 2, ahead0); ahead0 = next(ahead0); }
+      auto begin_step = [&](int i) {                     // P -> dV, and dP in its place behind it
+        wait(gfull(i), gphase(i), serr);
+        clean(C::b_off + (i % C::NB) * C::TB, q0);
+        q0 = next(q0);
+        wait(pfull(C::set(i)), C::phase(i), serr);
+        values(i);
+        dscores(i);
       };
-      if (C::SIDE) {
-        // S read -> dP in its place; the other warpgroup's dP read -> its next S, and its dS -> dK; P -> dV
+      auto finish = [&](int i) {                         // dS -> dK, and the set's next scores
+        keys(i);
+        if (i + C::SETS < steps) { scores(i + C::SETS, ahead0); ahead0 = next(ahead0); }
+      };
+      if (C::SETS == 1) {
         for (int i = 0; i < steps; ++i) {
-          gradient_tile(i);
-          wait(sread(i & 1), (i >> 1) & 1, serr);
-          dscores(i, false);
-          if (i > 0) {
-            wait(dpread((i - 1) & 1), ((i - 1) >> 1) & 1, serr);
-            next_scores(i - 1);
-            keys(i - 1);
-          }
-          wait(pfull(i & 1), (i >> 1) & 1, serr);
-          values(i, true);
+          begin_step(i);
+          finish(i);
         }
-        keys(steps - 1);
       } else {
-        // P -> dV, and dP in its place behind it.  Between this and the end of the step its warpgroup needs the tensor pipe's
-        // latency and the time to form dS; in this order the other warpgroup's products fill it
-        auto finish = [&](int i) {
-          keys(i);
-          next_scores(i);
-        };
-        auto begin_step = [&](int i) {
-          gradient_tile(i);
-          wait(pfull(i & 1), (i >> 1) & 1, serr);
-          values(i, false);
-          dscores(i, true);
-        };
+        // between the two halves of a step its set needs the tensor pipe's latency and the time to form dS: in this order the
+        // other set's products fill it
         for (int i = 0; i < steps; i += 2) {
           begin_step(i);
           if (i > 0) finish(i - 1);
@@ -402,7 +381,7 @@ __device__ __forceinline__ void keys_and_values(const CUtensorMap& tmQ, const CU
     // every thread took as much of shared memory's bandwidth as two of the products (D = 128: 3000 cycles a step).
     const int a = warp >> 2, t4 = lane & 3, first = key0 + (warp & 3) * 32, own_key = first + lane;
     const uint32_t tl = (uint32_t)((warp & 3) * 32) << 16, lower = 16u << 16;
-    const uint32_t x_addr = tX(a) + tl, p_addr = tP(a) + tl;
+    const uint32_t x_addr = tX(a) + tl;
     const int own_hi = own_key < g.T ? last_query(g.cu, g.nseq, g.window, g.T, own_key) : own_key - 1;
     const int w_hi = __shfl_sync(0xffffffffu, own_hi, 0), w_key = first + 31;         // hi ascends with the key
     int hi[2][2];                                                                     // of key first + 16 h + 8 e + lane / 4
@@ -411,10 +390,10 @@ __device__ __forceinline__ void keys_and_values(const CUtensorMap& tmQ, const CU
 #pragma unroll
       for (int e = 0; e < 2; ++e) hi[h][e] = __shfl_sync(0xffffffffu, own_hi, 16 * h + 8 * e + (lane >> 2));
     int qi = a % nq;
-    for (int i = a; i < steps; i += 2) {
-      const uint32_t ph = (i >> 1) & 1;
+    for (int i = a; i < steps; i += C::SETS) {
+      const uint32_t ph = C::phase(i);
       const int q0 = (kt + qi) * TILE;
-      qi = (qi + 2) % nq;
+      qi = (qi + C::SETS) % nq;
       const f32x2* ndelta = reinterpret_cast<const f32x2*>(smem + C::aux_off + (i % C::NA) * 512) + t4;
       const f32x2* nlse = reinterpret_cast<const f32x2*>(smem + C::aux_off + (C::NA + i % C::NB) * 512) + t4;
       wait(sfull(a), ph, serr);
@@ -425,7 +404,6 @@ __device__ __forceinline__ void keys_and_values(const CUtensorMap& tmQ, const CU
       tmem_ld_16x256b_x16(x_addr, x[0]);
       tmem_ld_16x256b_x16(x_addr + lower, x[1]);
       tmem_ld_wait();
-      if (C::SIDE) release(sread(a), lane);
       const bool mask = q0 < w_key || q0 + TILE - 1 > w_hi;
       auto clear = [&]() {                                 // queries that do not see the key
 #pragma unroll
@@ -452,7 +430,7 @@ __device__ __forceinline__ void keys_and_values(const CUtensorMap& tmQ, const CU
           uint32_t w[32];
 #pragma unroll
           for (int u = 0; u < 32; ++u) w[u] = pack_bf16(__uint_as_float(x[h][2 * u]), __uint_as_float(x[h][2 * u + 1]));
-          tmem_st_16x128b_x16(p_addr + h * lower, w);
+          tmem_st_16x128b_x16(x_addr + h * lower, w);
         }
       };
       if (mask) {                                          // two branches with the same exponentials: see queries_only
@@ -460,10 +438,6 @@ __device__ __forceinline__ void keys_and_values(const CUtensorMap& tmQ, const CU
         clear();
       } else {
         exponentials(x, g.scale_log2, nlse);
-      }
-      if (C::SIDE && i >= 2) {                             // the product has read this warpgroup's last dS
-        wait(dkdone(a), ((i >> 1) - 1) & 1, serr);
-        tc_fence_after();
       }
       store();
       hand_over(pfull(a), lane);
@@ -474,7 +448,6 @@ __device__ __forceinline__ void keys_and_values(const CUtensorMap& tmQ, const CU
         uint32_t d[64];
         tmem_ld_16x256b_x16(x_addr + h * lower, d);
         tmem_ld_wait();
-        if (C::SIDE && h) release(dpread(a), lane);
 #pragma unroll
         for (int u = 0; u < 16; ++u) {
           const f32x2 nd = ndelta[4 * u];
@@ -483,10 +456,6 @@ __device__ __forceinline__ void keys_and_values(const CUtensorMap& tmQ, const CU
         }
       }
       if (mask) clear();                                   // 0 x (what a padding row's product left) is not zero
-      if (C::SIDE) {                                       // the product has read P
-        wait(dvdone(a), ph, serr);
-        tc_fence_after();
-      }
       store();
       hand_over(dsfull(a), lane);
     }
@@ -494,12 +463,12 @@ __device__ __forceinline__ void keys_and_values(const CUtensorMap& tmQ, const CU
     tc_fence_after();
     const long long off = ((long long)own_key * g.Hkv + kh) * g.D;
     if (a == 0) store_row<DH>(tdV + tl, dv + off, g.D, 1.f, own_key < g.T);
-    else store_row<DH>(tdK + tl, dk + off, g.D, g.scale, own_key < g.T);
+    if (a == C::SETS - 1) store_row<DH>(tdK + tl, dk + off, g.D, g.scale, own_key < g.T);
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 8) tmem_dealloc(tm, 512);
+  if (warp == C::ISSUE) tmem_dealloc(tm, C::COLS);
   if (threadIdx.x == 0 && *serr) atomicExch(gerr, 1);
 }
 
@@ -546,7 +515,7 @@ __device__ __forceinline__ void queries_only(const CUtensorMap& tmQ, const CUten
     mbar_expect_tx(vfull(i), C::TB);
     load_tile<DH>(sV(i), &tmV, vfull(i), kh, (qt - i) * TILE);
   };
-  if (warp == 9) {
+  if (warp == C::LOAD) {
     if (elect_one()) {
       *serr = 0;
       mbar_init(own, 1);
@@ -571,19 +540,19 @@ __device__ __forceinline__ void queries_only(const CUtensorMap& tmQ, const CUten
     }
     __syncwarp();
   }
-  if (warp == 8) tmem_alloc(tslot, 512);
+  if (warp == C::ISSUE) tmem_alloc(tslot, C::COLS);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tm = uniform(*tslot);
   auto tX = [&](int a) { return tm + a * TILE; };                                   // S, then dP
-  auto tDS = [&](int a) { return tm + 2 * TILE + DH + a * 64; };
-  const uint32_t tdQ = tm + 2 * TILE;
+  auto tDS = [&](int a) { return tm + C::SETS * TILE + DH + a * 64; };
+  const uint32_t tdQ = tm + C::SETS * TILE;
   const int steps = qt - uniform(min(qt, first_key(g.cu, g.nseq, g.window, row0) / TILE)) + 1;
 
-  if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    if (warp == 9) {
+  if (warp >= C::ISSUE) {
+    if (C::SETS == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;"); else asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == C::LOAD) {
       int i = 1;                                           // step 0 is on its way
       for (; i < steps && !*serr; ++i) {
         wait(kempty(i), kphase(i) ^ 1, serr);
@@ -597,7 +566,7 @@ __device__ __forceinline__ void queries_only(const CUtensorMap& tmQ, const CUten
         for (int u = max(0, i - C::NA); u < i; ++u) mbar_wait(kfull(u), kphase(u), &ignore);
         for (int u = max(0, i - C::NB); u < i; ++u) mbar_wait(vfull(u), vphase(u), &ignore);
       }
-    } else if (warp == 8) {
+    } else if (warp == C::ISSUE) {
       constexpr uint32_t idS = mma_desc<bf16>(TILE, TILE, 0, 0), idG = mma_desc<bf16>(TILE, DH, 0, 1);
       const int begin = max(0, __ldg(g.cu)), end = min(g.T, __ldg(g.cu + g.nseq));
       auto scores = [&](int i) {                         // S = Q K_i^T
@@ -608,49 +577,53 @@ __device__ __forceinline__ void queries_only(const CUtensorMap& tmQ, const CUten
         if (elect_one()) {
           const uint64_t q = desc_dims(sQ, 0), k = desc_dims(sK(i), 0);
 #pragma unroll
-          for (int u = 0; u < DH / 16; ++u) umma_bf16(tX(i & 1), q + dims_step(u), k + dims_step(u), idS, u != 0);
-          umma_commit(sfull(i & 1));
+          for (int u = 0; u < DH / 16; ++u) umma_bf16(tX(C::set(i)), q + dims_step(u), k + dims_step(u), idS, u != 0);
+          umma_commit(sfull(C::set(i)));
         }
         __syncwarp();
       };
       auto dscores = [&](int i) {                        // dP = dO V_i^T, once S has been read
         wait(vfull(i), vphase(i), serr);
-        wait(sread(i & 1), (i >> 1) & 1, serr);
+        wait(sread(C::set(i)), C::phase(i), serr);
         tc_fence_after();
         if (elect_one()) {
           const uint64_t go = desc_dims(sG, 0), v = desc_dims(sV(i), 0);
 #pragma unroll
-          for (int u = 0; u < DH / 16; ++u) umma_bf16(tX(i & 1), go + dims_step(u), v + dims_step(u), idS, u != 0);
-          umma_commit(dpfull(i & 1));
+          for (int u = 0; u < DH / 16; ++u) umma_bf16(tX(C::set(i)), go + dims_step(u), v + dims_step(u), idS, u != 0);
+          umma_commit(dpfull(C::set(i)));
           umma_commit(vempty(i));
         }
         __syncwarp();
       };
       auto queries = [&](int i) {                        // dQ += dS K_i
-        wait(dsfull(i & 1), (i >> 1) & 1, serr);
+        wait(dsfull(C::set(i)), C::phase(i), serr);
         tc_fence_after();
         if (elect_one()) {
           const uint64_t k = desc_rows(sK(i), 0);
 #pragma unroll
-          for (int u = 0; u < TILE / 16; ++u) umma_ts(tdQ, tDS(i & 1) + 8 * u, k + rows_step(u), idG, i > 0 || u != 0);
+          for (int u = 0; u < TILE / 16; ++u) umma_ts(tdQ, tDS(C::set(i)) + 8 * u, k + rows_step(u), idG, i > 0 || u != 0);
           umma_commit(kempty(i));
-          umma_commit(dqdone(i & 1));
+          umma_commit(dqdone(C::set(i)));
           if (i + 1 == steps) umma_commit(done);
         }
         __syncwarp();
       };
       wait(own, 0, serr);
       scores(0);
-      if (steps > 1) scores(1);
+      if (C::SETS > 1 && steps > 1) scores(1);
+      constexpr int LAG = C::SETS - 1;                   // with two sets, the other one's last step is in between
       for (int i = 0; i < steps; ++i) {
         dscores(i);
-        if (i > 0) {                                     // the other warpgroup's dP read -> its next S, and its dS -> dQ
-          wait(dpread((i - 1) & 1), ((i - 1) >> 1) & 1, serr);
-          if (i + 1 < steps) scores(i + 1);
-          queries(i - 1);
+        const int e = i - LAG;                           // dP read -> the set's next S, and its dS -> dQ
+        if (e >= 0) {
+          if (e + C::SETS < steps) {
+            wait(dpread(C::set(e)), C::phase(e), serr);
+            scores(e + C::SETS);
+          }
+          queries(e);
         }
       }
-      queries(steps - 1);
+      if (LAG) queries(steps - 1);
       drain_products(drained, serr);
     }
   } else {
@@ -662,8 +635,8 @@ __device__ __forceinline__ void queries_only(const CUtensorMap& tmQ, const CUten
     const int w_lo = __shfl_sync(0xffffffffu, lo, 31), w_row = row - lane;
     const float L = g.aux[(long long)h * g.Tp + row], D = g.aux[((long long)g.Hq + h) * g.Tp + row];
     const f32x2 nl = pair(L, L), nd = pair(D, D);
-    for (int i = a; i < steps; i += 2) {
-      const uint32_t ph = (i >> 1) & 1;
+    for (int i = a; i < steps; i += C::SETS) {
+      const uint32_t ph = C::phase(i);
       const int k0 = (qt - i) * TILE;
       wait(sfull(a), ph, serr);
       tc_fence_after();
@@ -698,8 +671,8 @@ __device__ __forceinline__ void queries_only(const CUtensorMap& tmQ, const CUten
           if (mask) clear_hidden(x[c], 32 * c, c_lo, c_hi);  // 0 x (what a padding row's product left) is not zero
         }
       }
-      if (i >= 2) {                                        // the last dS of this warpgroup has been read
-        wait(dqdone(a), ((i >> 1) - 1) & 1, serr);
+      if (i >= C::SETS) {                                  // the last dS of this set has been read
+        wait(dqdone(a), C::phase(i) ^ 1, serr);
         tc_fence_after();
       }
 #pragma unroll
@@ -713,13 +686,13 @@ __device__ __forceinline__ void queries_only(const CUtensorMap& tmQ, const CUten
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 8) tmem_dealloc(tm, 512);
+  if (warp == C::ISSUE) tmem_dealloc(tm, C::COLS);
   if (threadIdx.x == 0 && *serr) atomicExch(gerr, 1);
 }
 
 // One launch for both: the dkv blocks, which have more to do, come first, and dq blocks fill the SMs that they leave.
 template <int DH>
-__global__ void __launch_bounds__(NT, 1) packed_bwd_kernel(
+__global__ void __launch_bounds__(Cfg<DH>::NT, 3 - Cfg<DH>::SETS) packed_bwd_kernel(
     const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
     const __grid_constant__ CUtensorMap tmG, bf16* __restrict__ dq, bf16* __restrict__ dk, bf16* __restrict__ dv,
     const __grid_constant__ Geo g, int* __restrict__ gerr) {
@@ -733,7 +706,7 @@ int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, 
            const Geo& g, int* err, cudaStream_t st) {
   static std::atomic<unsigned long long> set{0};
   if (int rc = allow_smem(packed_bwd_kernel<DH>, Cfg<DH>::total, set)) return rc;
-  packed_bwd_kernel<DH><<<(unsigned)(g.tiles * (g.Hkv + g.Hq)), NT, Cfg<DH>::total, st>>>(mq, mk, mv, mg, dq, dk, dv, g, err);
+  packed_bwd_kernel<DH><<<(unsigned)(g.tiles * (g.Hkv + g.Hq)), Cfg<DH>::NT, Cfg<DH>::total, st>>>(mq, mk, mv, mg, dq, dk, dv, g, err);
   DMB_CHECK_LAUNCH();
   return 0;
 }
