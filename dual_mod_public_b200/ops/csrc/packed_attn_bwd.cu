@@ -19,9 +19,11 @@
 // all products in a fixed order, one loads.  Tensor memory holds the accumulators and per set 128 columns for S, then dP.  dkv: P
 // and dS overwrite S and dP as they are made, dP follows the product that reads P, and the next S the one that reads dS.  dq: 64
 // more columns for dS, so that dP is formed while the exponentials run, and the next S as soon as dP has been read.
-// P and dS are rounded to bf16 (relative 2^-8 at most, as o was); everything else is fp32.
+// P and dS are rounded to bf16 (relative 2^-8 at most, ); everything else is fp32.
 //
-// A first small kernel forms -delta and -lse in base 2 (-inf for rows without keys and for the padding of the last tile, which
+// A first small kernel forms delta from o and the rest that its rounding left: where a row sees few keys ds is a small difference
+// of dp and delta (zero for a row that sees itself alone), and the rounding of o alone would be most of the gradients' error
+// (8192 rows of eleven documents: 2.9e-3 of dq's norm with o alone).  It leaves -delta and -lse in base 2 (-inf for rows without keys and for the padding of the last tile, which
 // makes their weights zero).
 #include "packed.cuh"
 
@@ -33,13 +35,14 @@ constexpr int MORE = 4;
 
 // aux: [2][Hq][Tp] fp32 (-lse in base 2, -delta), Tp = T rounded up to whole tiles
 template <int LANES>
-__global__ void __launch_bounds__(256) packed_delta_kernel(const bf16* __restrict__ o, const bf16* __restrict__ go, long long g_rs,
+__global__ void __launch_bounds__(256) packed_delta_kernel(const bf16* __restrict__ o, const bf16* __restrict__ o_lo,
+                                                           const bf16* __restrict__ go, long long g_rs,
                                                            long long g_hs, const float* __restrict__ lse, float* __restrict__ aux,
                                                            const int* __restrict__ cu, int nseq, int T, int Tp, int Hq, int D) {
   // a group of LANES threads (8 dims each) takes MORE consecutive (row, head) pairs, whose loads are in flight together
   const long long w0 = ((long long)blockIdx.x * 256 + threadIdx.x) / LANES * MORE;
   const int sub = threadIdx.x % LANES, begin = __ldg(cu), end = __ldg(cu + nseq);
-  uint4 a[MORE], b[MORE];
+  uint4 a[MORE], l[MORE], b[MORE];
   int row[MORE], h[MORE];
   bool inside[MORE];
 #pragma unroll
@@ -47,21 +50,23 @@ __global__ void __launch_bounds__(256) packed_delta_kernel(const bf16* __restric
     row[k] = (int)((w0 + k) / Hq);                        // below Tp: the grid is exact
     h[k] = (int)(w0 + k - (long long)row[k] * Hq);
     inside[k] = row[k] < T && row[k] >= begin && row[k] < end;                  // padding rows may hold anything
-    a[k] = b[k] = make_uint4(0, 0, 0, 0);
+    a[k] = l[k] = b[k] = make_uint4(0, 0, 0, 0);
     if (inside[k] && sub * 8 < D) {
       a[k] = *reinterpret_cast<const uint4*>(o + ((long long)row[k] * Hq + h[k]) * D + sub * 8);
+      if (o_lo) l[k] = *reinterpret_cast<const uint4*>(o_lo + ((long long)row[k] * Hq + h[k]) * D + sub * 8);
       b[k] = *reinterpret_cast<const uint4*>(go + row[k] * g_rs + h[k] * g_hs + sub * 8);
     }
   }
 #pragma unroll
   for (int k = 0; k < MORE; ++k) {
-    const uint32_t x[4] = {a[k].x, a[k].y, a[k].z, a[k].w}, y[4] = {b[k].x, b[k].y, b[k].z, b[k].w};
+    const uint32_t x[4] = {a[k].x, a[k].y, a[k].z, a[k].w}, z[4] = {l[k].x, l[k].y, l[k].z, l[k].w},
+                   y[4] = {b[k].x, b[k].y, b[k].z, b[k].w};
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2 p = unpack_bf16(x[i]), q = unpack_bf16(y[i]);
-      s = fmaf(p.x, q.x, s);
-      s = fmaf(p.y, q.y, s);
+      const float2 p = unpack_bf16(x[i]), r = unpack_bf16(z[i]), q = unpack_bf16(y[i]);
+      s = fmaf(p.x + r.x, q.x, s);
+      s = fmaf(p.y + r.y, q.y, s);
     }
 #pragma unroll
     for (int i = LANES / 2; i > 0; i >>= 1) s += __shfl_xor_sync(0xffffffffu, s, i);
@@ -714,10 +719,10 @@ int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, 
 }  // namespace
 
 // bf16: go (gradient of o) [T, Hq, D] and q, k, v by strides as in dmb_packed_attn_fwd; o, dq [T, Hq, D], dk, dv [T, Hkv, D]
-// contiguous; lse [Hq, T]; aux fp32 [2, Hq, Tp] with Tp = T rounded up to a multiple of 128.  All gradient rows are written.
+// contiguous, o_lo like o or null; lse [Hq, T]; aux fp32 [2, Hq, Tp] with Tp = T rounded up to a multiple of 128.  All gradient rows are written.
 extern "C" int dmb_packed_attn_bwd(const void* go, long long g_rs, long long g_hs, const void* q, long long q_rs, long long q_hs,
                                    const void* k, long long k_rs, long long k_hs, const void* v, long long v_rs, long long v_hs,
-                                   const void* o, const float* lse, const int* cu, int nseq, float* aux, void* dq, void* dk,
+                                   const void* o, const void* o_lo, const float* lse, const int* cu, int nseq, float* aux, void* dq, void* dk,
                                    void* dv, int T, int Hq, int Hkv, int D, int window, float scale, int* err, void* stream) {
   if (T <= 0) return 0;
   if (D <= 0 || D > 128 || (D & 7) || Hkv <= 0 || Hq % Hkv || nseq < 0) return -1;
@@ -735,10 +740,10 @@ extern "C" int dmb_packed_attn_bwd(const void* go, long long g_rs, long long g_h
   const long long rows = (long long)g.Tp * Hq;
   // rows is a multiple of 128, so with 8 or 16 threads for 4 of them every block is full
   if (D <= 64)
-    packed_delta_kernel<8><<<(unsigned)(rows / MORE * 8 / 256), 256, 0, st>>>((const bf16*)o, (const bf16*)go, g_rs, g_hs, lse, aux, cu,
+    packed_delta_kernel<8><<<(unsigned)(rows / MORE * 8 / 256), 256, 0, st>>>((const bf16*)o, (const bf16*)o_lo, (const bf16*)go, g_rs, g_hs, lse, aux, cu,
                                                                                nseq, T, g.Tp, Hq, D);
   else
-    packed_delta_kernel<16><<<(unsigned)(rows / MORE * 16 / 256), 256, 0, st>>>((const bf16*)o, (const bf16*)go, g_rs, g_hs, lse, aux, cu,
+    packed_delta_kernel<16><<<(unsigned)(rows / MORE * 16 / 256), 256, 0, st>>>((const bf16*)o, (const bf16*)o_lo, (const bf16*)go, g_rs, g_hs, lse, aux, cu,
                                                                                  nseq, T, g.Tp, Hq, D);
   DMB_CHECK_LAUNCH();
   return D <= 64 ? launch<64>(mq, mk, mv, mg, (bf16*)dq, (bf16*)dk, (bf16*)dv, g, err, st)

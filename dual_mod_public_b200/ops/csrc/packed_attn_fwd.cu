@@ -77,10 +77,21 @@ __device__ __forceinline__ f32x2 weights(const uint32_t (&x)[32], float scale, f
   return add2(sum[0], sum[1]);
 }
 
+// 16 dims of a row from d0 on, as far as the row has them (dims are a multiple of 8)
+template <typename T>
+__device__ __forceinline__ void store16(T* row, int d0, int D, const uint32_t (&w)[8]) {
+  if (d0 + 16 <= D && (D & 15) == 0) {
+    st_global_32(row + d0, w);
+  } else if (d0 < D) {
+    *reinterpret_cast<uint4*>(row + d0) = make_uint4(w[0], w[1], w[2], w[3]);
+    if (d0 + 8 < D) *reinterpret_cast<uint4*>(row + d0 + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+  }
+}
+
 template <typename T, int DH>
 __global__ void __launch_bounds__(Cfg<DH>::NT, 3 - Cfg<DH>::TILES) packed_fwd_kernel(
     const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-    T* __restrict__ out, float* __restrict__ lse, const Geo g, int* __restrict__ gerr) {
+    T* __restrict__ out, T* __restrict__ out_lo, float* __restrict__ lse, const Geo g, int* __restrict__ gerr) {
   using C = Cfg<DH>;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t base = smem_u32(smem);
@@ -333,17 +344,20 @@ __global__ void __launch_bounds__(Cfg<DH>::NT, 3 - Cfg<DH>::TILES) packed_fwd_ke
       if (row < g.T) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
+          float f[16];
           uint32_t w[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            w[i] = Elem<T>::pack(inv == 0.f ? 0.f : __uint_as_float(o[16 * u + 2 * i]) * inv,
-                                 inv == 0.f ? 0.f : __uint_as_float(o[16 * u + 2 * i + 1]) * inv);
-          const int d0 = 32 * c + 16 * u;
-          if (d0 + 16 <= g.D && (g.D & 15) == 0) {
-            st_global_32(o_row + d0, w);
-          } else if (d0 < g.D) {                                    // dims are a multiple of 8
-            *reinterpret_cast<uint4*>(o_row + d0) = make_uint4(w[0], w[1], w[2], w[3]);
-            if (d0 + 8 < g.D) *reinterpret_cast<uint4*>(o_row + d0 + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+          for (int i = 0; i < 16; ++i) f[i] = inv == 0.f ? 0.f : __uint_as_float(o[16 * u + i]) * inv;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) w[i] = Elem<T>::pack(f[2 * i], f[2 * i + 1]);
+          store16(o_row, 32 * c + 16 * u, g.D, w);
+          if (out_lo) {                                            // what the rounding left
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float2 r = Elem<T>::unpack(w[i]);
+              w[i] = Elem<T>::pack(f[2 * i] - r.x, f[2 * i + 1] - r.y);
+            }
+            store16(out_lo + (o_row - out), 32 * c + 16 * u, g.D, w);
           }
         }
       }
@@ -359,12 +373,12 @@ __global__ void __launch_bounds__(Cfg<DH>::NT, 3 - Cfg<DH>::TILES) packed_fwd_ke
 }
 
 template <typename T, int DH>
-int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, void* o, float* lse, const Geo& g, int* err,
+int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, void* o, void* o_lo, float* lse, const Geo& g, int* err,
            cudaStream_t st) {
   auto kern = packed_fwd_kernel<T, DH>;
   static std::atomic<unsigned long long> set{0};
   if (int rc = allow_smem(kern, Cfg<DH>::total, set)) return rc;
-  kern<<<(unsigned)(g.Hq * g.units), Cfg<DH>::NT, Cfg<DH>::total, st>>>(mq, mk, mv, (T*)o, lse, g, err);
+  kern<<<(unsigned)(g.Hq * g.units), Cfg<DH>::NT, Cfg<DH>::total, st>>>(mq, mk, mv, (T*)o, (T*)o_lo, lse, g, err);
   DMB_CHECK_LAUNCH();
   return 0;
 }
@@ -372,10 +386,10 @@ int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, 
 }  // namespace
 
 // q [T, Hq, D] (row stride, head stride), k / v [T, Hkv, D] likewise, 16-bit elements (half: fp16, else bf16); o [T, Hq, D]
-// contiguous; lse [Hq, T] fp32 or null.  Strides are multiples of 8 elements, pointers 16-byte aligned, D a multiple of 8
+// contiguous; o_lo: like o or null, what the rounding of o left (the backward pass forms do . o from both); lse [Hq, T] fp32 or null.  Strides are multiples of 8 elements, pointers 16-byte aligned, D a multiple of 8
 // up to 128 (the caller checks).
 extern "C" int dmb_packed_attn_fwd(const void* q, long long q_rs, long long q_hs, const void* k, long long k_rs, long long k_hs,
-                                   const void* v, long long v_rs, long long v_hs, const int* cu, int nseq, void* o, float* lse,
+                                   const void* v, long long v_rs, long long v_hs, const int* cu, int nseq, void* o, void* o_lo, float* lse,
                                    int T, int Hq, int Hkv, int D, int window, float scale, int half, int* err, void* stream) {
   if (T <= 0) return 0;
   if (D <= 0 || D > 128 || (D & 7) || Hkv <= 0 || Hq % Hkv || nseq < 0) return -1;
@@ -389,6 +403,6 @@ extern "C" int dmb_packed_attn_fwd(const void* q, long long q_rs, long long q_hs
   if ((long long)units * Hq > 0x7fffffffLL) return -1;
   const Geo g{cu, nseq, T, Hq, Hq / Hkv, D, window, units, scale * LOG2E};
   cudaStream_t st = (cudaStream_t)stream;
-  if (half) return D <= 64 ? launch<__half, 64>(mq, mk, mv, o, lse, g, err, st) : launch<__half, 128>(mq, mk, mv, o, lse, g, err, st);
-  return D <= 64 ? launch<bf16, 64>(mq, mk, mv, o, lse, g, err, st) : launch<bf16, 128>(mq, mk, mv, o, lse, g, err, st);
+  if (half) return D <= 64 ? launch<__half, 64>(mq, mk, mv, o, o_lo, lse, g, err, st) : launch<__half, 128>(mq, mk, mv, o, o_lo, lse, g, err, st);
+  return D <= 64 ? launch<bf16, 64>(mq, mk, mv, o, o_lo, lse, g, err, st) : launch<bf16, 128>(mq, mk, mv, o, o_lo, lse, g, err, st);
 }

@@ -86,8 +86,8 @@ class _Sigs:
     dmb_attn_dkv_tc = [_p, _p, _p, _p, _i, _p, _p, _v, _i, _p, _p, _v, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i, _p, _p]
     dmb_attn_fwd_tc = [_p, _v, _i, _p, _p, _v, _i, _p, _i, _p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i, _i, _i,
                        _i, _i, _p, _p]
-    dmb_packed_attn_fwd = [_p, _ll, _ll, _p, _ll, _ll, _p, _ll, _ll, _p, _i, _p, _p, _i, _i, _i, _i, _i, _f, _i, _p, _p]
-    dmb_packed_attn_bwd = [_p, _ll, _ll, _p, _ll, _ll, _p, _ll, _ll, _p, _ll, _ll, _p, _p, _p, _i, _p, _p, _p, _p, _i, _i, _i, _i,
+    dmb_packed_attn_fwd = [_p, _ll, _ll, _p, _ll, _ll, _p, _ll, _ll, _p, _i, _p, _p, _p, _i, _i, _i, _i, _i, _f, _i, _p, _p]
+    dmb_packed_attn_bwd = [_p, _ll, _ll, _p, _ll, _ll, _p, _ll, _ll, _p, _ll, _ll, _p, _p, _p, _p, _i, _p, _p, _p, _p, _i, _i, _i, _i,
                            _i, _f, _p, _p]
     dmb_cached_attn = [_p, _ll, _ll, _p, _ll, _ll, _ll, _p, _ll, _ll, _ll, _p, _p, _i, _i, _i, _i, _i, _i, _i, _f, _i, _p]
     dmb_logprob_fwd = [_p, _ll, _p, _ll, _i, _i, _i, _p, _p, _p, _p, _p, _p]
@@ -1107,26 +1107,28 @@ class CudaOps(TorchOps):
         return (q.dtype is BF16 or q.dtype is F16) and D <= 128 and not D & 7
 
     @_here
-    def packed_attn_fwd(self, q, k, v, cu, window, scale, need_lse=True):
+    def packed_attn_fwd(self, q, k, v, cu, window, scale, need_lse=True, residual=False):
         if not self._packed_ok(q):
             self._fell_back("packed_attn_fwd")
-            return super().packed_attn_fwd(q, k, v, cu, window, scale, need_lse)
+            return super().packed_attn_fwd(q, k, v, cu, window, scale, need_lse, residual)
         (q, qs), (k, ks), (v, vs) = self._rows16(q), self._rows16(k), self._rows16(v)
         T, Hq, D = q.shape
         o = _empty(q.dtype, T, Hq, D)
         lse = _empty(F32, Hq, T) if need_lse else None
+        o_lo = _empty(q.dtype, T, Hq, D) if residual else None
         if T:
             self._launch(self.lib.dmb_packed_attn_fwd, "packed_attn_fwd", q.data_ptr(), *qs, k.data_ptr(), *ks, v.data_ptr(),
-                         *vs, cu.data_ptr(), cu.shape[0] - 1, o.data_ptr(), lse.data_ptr() if need_lse else None, T, Hq,
+                         *vs, cu.data_ptr(), cu.shape[0] - 1, o.data_ptr(), o_lo.data_ptr() if residual else None,
+                         lse.data_ptr() if need_lse else None, T, Hq,
                          k.shape[1], D, window, scale, q.dtype is F16, self._tc_err_ptr)
-        return o, lse
+        return (o, lse, o_lo) if residual else (o, lse)
 
     @_here
-    def packed_attn_bwd(self, do, q, k, v, o, lse, cu, window, scale):
+    def packed_attn_bwd(self, do, q, k, v, o, lse, cu, window, scale, o_lo=None):
         # dS = P (dP - delta) has no natural scale: in fp16 it underflows where the gradient does, so fp16 takes fp32 math
         if not self._packed_ok(q) or q.dtype is not BF16 or do.dtype is not BF16:
             self._fell_back("packed_attn_bwd")
-            return super().packed_attn_bwd(do, q, k, v, o, lse, cu, window, scale)
+            return super().packed_attn_bwd(do, q, k, v, o, lse, cu, window, scale, o_lo)
         (do, gs), (q, qs), (k, ks), (v, vs) = self._rows16(do), self._rows16(q), self._rows16(k), self._rows16(v)
         T, Hq, D = q.shape
         Hkv = k.shape[1]
@@ -1134,7 +1136,8 @@ class CudaOps(TorchOps):
         if T:
             aux = _empty(F32, 2 * Hq * (-(-T // 128) * 128))
             self._launch(self.lib.dmb_packed_attn_bwd, "packed_attn_bwd", do.data_ptr(), *gs, q.data_ptr(), *qs, k.data_ptr(),
-                         *ks, v.data_ptr(), *vs, o.data_ptr(), lse.data_ptr(), cu.data_ptr(), cu.shape[0] - 1, aux.data_ptr(),
+                         *ks, v.data_ptr(), *vs, o.data_ptr(), None if o_lo is None else o_lo.data_ptr(), lse.data_ptr(),
+                         cu.data_ptr(), cu.shape[0] - 1, aux.data_ptr(),
                          dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), T, Hq, Hkv, D, window, scale, self._tc_err_ptr)
         return dq, dk, dv
 

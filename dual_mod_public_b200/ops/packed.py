@@ -68,16 +68,16 @@ class _PackedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu, window, scale):
         ops = default_ops(q.device)
-        o, lse = ops.packed_attn_fwd(q, k, v, cu, window, scale)
-        ctx.save_for_backward(q, k, v, o, lse, cu)
+        o, lse, o_lo = ops.packed_attn_fwd(q, k, v, cu, window, scale, residual=True)
+        ctx.save_for_backward(q, k, v, o, lse, cu, o_lo)
         ctx.window, ctx.scale = window, scale
         return o
 
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
-        q, k, v, o, lse, cu = ctx.saved_tensors
-        dq, dk, dv = default_ops(q.device).packed_attn_bwd(do, q, k, v, o, lse, cu, ctx.window, ctx.scale)
+        q, k, v, o, lse, cu, o_lo = ctx.saved_tensors
+        dq, dk, dv = default_ops(q.device).packed_attn_bwd(do, q, k, v, o, lse, cu, ctx.window, ctx.scale, o_lo)
         return dq, dk, dv, None, None, None
 
 

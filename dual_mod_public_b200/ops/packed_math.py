@@ -49,10 +49,11 @@ def _inside(x, cu):
 
 
 def packed_attn_fwd(q, k, v, cu, window, scale):
-    """(o [T, Hq, D], lse [Hq, T] fp32)"""
+    """(o [T, Hq, D], lse [Hq, T] fp32, what the rounding of o left)"""
     T, Hq, _ = q.shape
     q, k, v = (_inside(x, cu) for x in (q, k, v))
     o = torch.empty_like(q, memory_format=torch.contiguous_format)
+    o_lo = torch.empty_like(o)
     lse = torch.empty(Hq, T, dtype=torch.float32, device=q.device)
     for rows, s, hidden in _slabs(q, k, cu, window, scale):
         top = s.amax(-1, keepdim=True)
@@ -61,16 +62,18 @@ def packed_attn_fwd(q, k, v, cu, window, scale):
         total = p.sum(-1, keepdim=True)
         vf = v[:rows.stop].float().transpose(0, 1)[:, None]
         some = total != 0
-        o[rows] = _heads_last(torch.where(some, (p @ vf) / total, 0.0)).to(q.dtype)
+        full = _heads_last(torch.where(some, (p @ vf) / total, 0.0))
+        o[rows] = full.to(q.dtype)
+        o_lo[rows] = (full - o[rows].float()).to(q.dtype)
         lse[:, rows] = torch.where(some, top + total.log(), float("-inf")).reshape(Hq, -1)
-    return o, lse
+    return o, lse, o_lo
 
 
-def packed_attn_bwd(do, q, k, v, o, lse, cu, window, scale):
+def packed_attn_bwd(do, q, k, v, o, lse, cu, window, scale, o_lo=None):
     """(dq, dk, dv) in the inputs' type"""
     T, Hq, D = q.shape
     Hkv = k.shape[1]
-    do, q, k, v, o = (_inside(x, cu) for x in (do, q, k, v, o))
+    do, q, k, v, o = (_inside(x, cu) for x in (do, q, k, v, o.float() if o_lo is None else o.float() + o_lo.float()))
     dq = torch.empty_like(q, memory_format=torch.contiguous_format)
     dk = torch.zeros(Hkv, T, D, dtype=torch.float32, device=q.device)
     dv = torch.zeros_like(dk)

@@ -376,13 +376,15 @@ class TorchOps:
         return fm.ce_chunk(logits, targets, inv_n)
 
     # ---- packed sequences (ops/packed.py) ---------------------------------------------------
-    def packed_attn_fwd(self, q, k, v, cu, window, scale, need_lse=True):
-        """Causal attention over packed sequences: (o [T, Hq, D], lse [Hq, T] fp32 or None)."""
-        return pm.packed_attn_fwd(q, k, v, cu, window, scale)
+    def packed_attn_fwd(self, q, k, v, cu, window, scale, need_lse=True, residual=False):
+        """Causal attention over packed sequences: (o [T, Hq, D], lse [Hq, T] fp32 or None) and, with `residual`, what
+        the rounding of o to its type left, in the same type."""
+        o, lse, o_lo = pm.packed_attn_fwd(q, k, v, cu, window, scale)
+        return (o, lse, o_lo) if residual else (o, lse)
 
-    def packed_attn_bwd(self, do, q, k, v, o, lse, cu, window, scale):
-        """Its gradients (dq, dk, dv) from the output, its gradient and lse."""
-        return pm.packed_attn_bwd(do, q, k, v, o, lse, cu, window, scale)
+    def packed_attn_bwd(self, do, q, k, v, o, lse, cu, window, scale, o_lo=None):
+        """Its gradients (dq, dk, dv) from the output (and its residual), its gradient and lse."""
+        return pm.packed_attn_bwd(do, q, k, v, o, lse, cu, window, scale, o_lo)
 
     def cached_attn(self, q, k, v, lengths, window, scale):
         """One query per sequence over the live rows of a cache: o [B, Hq, D]."""

@@ -59,6 +59,18 @@ def test_packed_backward_views(ops):  # noqa: F811
     check(grads(ops, qkv[:, 0], qkv[:, 1], qkv[:, 2], cu, one), ref.packed(qkv[:, 0], qkv[:, 1], qkv[:, 2], cu, do=one))
 
 
+def test_packed_backward_of_rows_that_see_themselves_alone(ops):  # noqa: F811
+    """Sequences of one token: o = v, ds = do . v - do . o = 0, so dq and dk are zero up to what delta is off.  delta comes
+    from o and its residual (2^-16 of every product) and fp32 sums of D products (2^-23 each, twice)."""
+    T, h, d = 300, 2, 64
+    q, k, v, g = (rnd(T, h, d, seed=s) for s in (1, 2, 3, 4))
+    o, dq, dk, dv = grads(ops, q, k, v, cu_of(*range(T + 1)), g)
+    assert torch.equal(o, v) and torch.equal(dv, g)
+    off = (g.double().abs() * v.double().abs()).sum(-1, keepdim=True) * (2.0 ** -16 + 2 * d * 2.0 ** -23) * d ** -0.5 * (1 + 2.0 ** -7)
+    ref.close(dq, (torch.zeros_like(dq, dtype=torch.float64), off * k.double().abs() + 1e-30), "dq")
+    ref.close(dk, (torch.zeros_like(dk, dtype=torch.float64), off * q.double().abs() + 1e-30), "dk")
+
+
 def test_packed_backward_padding_is_not_read(ops):  # noqa: F811
     q, k, v, g = (rnd(500, 2, 64, seed=s) for s in (1, 2, 3, 4))
     cu = cu_of(2, 200, 450)
