@@ -2,7 +2,8 @@
 //
 //   o_h = sum_{j in [lo, len)} softmax(scale q_h . k_j) v_j,   lo = max(0, len - window),   query heads h share key head h / g
 //
-// Bound by reading the live rows of K and V once.  A cluster of 1 to 16 blocks shares the live rows of one (sequence, key head)
+// Bound by reading the live rows of K and V once (64 sequences of up to 8192 rows, 16 query and 4 key heads of 128: 90 us, 5.6
+// TB/s; one sequence of 1190 rows, 16 heads of 64: 8.4 us, all of it latency).  A cluster of 1 to 16 blocks shares the live rows of one (sequence, key head)
 // out evenly; a block's warps take tiles of KEYS keys in turn, each warp with a ring of its own filled by asynchronous copies
 // (no barrier between warps until the end).  All query heads of the group are the 16 rows of a warp-level MMA (m16n8k16): one
 // head or sixteen, the keys are read once and the matrix pipe stays far below its rate, so padding the rows costs nothing that

@@ -115,8 +115,9 @@ def cached_attention(q, k_cache, v_cache, lengths, *, window=0, scale=None):
         raise ValueError("lengths: one entry per sequence is wanted")
     if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
         raise ValueError("cached_attention has no gradient: call it under torch.no_grad()")
-    if k_cache.shape[1] >= 1 << 31:
-        raise ValueError("too many cache rows")
+    if k_cache.shape[1] >= 1 << 31 or q.shape[0] > 65535 or k_cache.shape[2] > 4095:
+        raise ValueError("at most 65535 sequences, 4095 key heads and 2^31 - 1 cache rows are wanted, got "
+                         f"{q.shape[0]}, {k_cache.shape[2]}, {k_cache.shape[1]}")
     return default_ops(q.device).cached_attn(q, k_cache, v_cache, lengths.contiguous(), window, scale)
 
 

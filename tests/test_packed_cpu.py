@@ -151,6 +151,8 @@ def test_attention_refusals():
         (ValueError, (q, kc, kc[:, :5], n), {}),
         (ValueError, (q.clone().requires_grad_(), kc, kc, n), {}),
         (ValueError, (q, kc, kc, n), {"scale": -1.0}),
+        (ValueError, (torch.zeros(65536, 1, 8), torch.zeros(65536, 0, 1, 8), torch.zeros(65536, 0, 1, 8),
+                      torch.zeros(65536, dtype=torch.int32)), {}),
     ]:
         with pytest.raises(error):
             cached_attention(*args, **kw)
