@@ -21,8 +21,8 @@
 // more columns for dS, so that dP is formed while the exponentials run, and the next S as soon as dP has been read.
 // P and dS are rounded to bf16 (relative 2^-8 at most); everything else is fp32.
 //
-// Measured (8192 rows, one sequence): 16 heads of 64 542 us, 16 query and 4 key heads of 128 738 us, 634 and 931 TFLOP/s counted
-// as five products over the visible pairs; eleven documents in 8192 rows, 16 heads of 64: 151 us.  Bound at D = 128 by the tensor
+// Measured (8192 rows, one sequence): 16 heads of 64 534 us, 16 query and 4 key heads of 128 722 us, 644 and 951 TFLOP/s counted
+// as five products over the visible pairs; eleven documents in 8192 rows, 16 heads of 64: 141 us.  Bound at D = 128 by the tensor
 // pipe (66 % busy over both kinds) and its latencies, at D = 64 by the exponentials and the instructions around them: products
 // with 64 columns take as long as ones with 128.
 //
@@ -44,23 +44,26 @@ __global__ void __launch_bounds__(256) packed_delta_kernel(const bf16* __restric
                                                            const bf16* __restrict__ go, long long g_rs,
                                                            long long g_hs, const float* __restrict__ lse, float* __restrict__ aux,
                                                            const int* __restrict__ cu, int nseq, int T, int Tp, int Hq, int D) {
-  // a group of LANES threads (8 dims each) takes MORE consecutive (row, head) pairs, whose loads are in flight together
-  const long long w0 = ((long long)blockIdx.x * 256 + threadIdx.x) / LANES * MORE;
+  // one head, ROWS rows: LANES threads (8 dims each) take a row, MORE rows whose loads are in flight together, and the rows of
+  // a warp's groups follow one another, so the row vectors are read and written in whole sectors: 11.1 us at 8192 rows of 16
+  // heads of 64 with a cold cache (50 MB), 19.7 with the heads of a row in a warp
+  constexpr int GROUPS = 256 / LANES, ROWS = GROUPS * MORE;
+  const int h = blockIdx.x % Hq, row0 = blockIdx.x / Hq * ROWS + threadIdx.x / LANES;
   const int sub = threadIdx.x % LANES, begin = __ldg(cu), end = __ldg(cu + nseq);
   uint4 a[MORE], l[MORE], b[MORE];
-  int row[MORE], h[MORE];
+  float L[MORE];
   bool inside[MORE];
 #pragma unroll
   for (int k = 0; k < MORE; ++k) {
-    row[k] = (int)((w0 + k) / Hq);                        // below Tp: the grid is exact
-    h[k] = (int)(w0 + k - (long long)row[k] * Hq);
-    inside[k] = row[k] < T && row[k] >= begin && row[k] < end;                  // padding rows may hold anything
+    const long long row = row0 + k * GROUPS;              // below Tp, a multiple of ROWS
+    inside[k] = row < T && row >= begin && row < end;     // padding rows may hold anything
     a[k] = l[k] = b[k] = make_uint4(0, 0, 0, 0);
     if (inside[k] && sub * 8 < D) {
-      a[k] = *reinterpret_cast<const uint4*>(o + ((long long)row[k] * Hq + h[k]) * D + sub * 8);
-      if (o_lo) l[k] = *reinterpret_cast<const uint4*>(o_lo + ((long long)row[k] * Hq + h[k]) * D + sub * 8);
-      b[k] = *reinterpret_cast<const uint4*>(go + row[k] * g_rs + h[k] * g_hs + sub * 8);
+      a[k] = *reinterpret_cast<const uint4*>(o + (row * Hq + h) * D + sub * 8);
+      if (o_lo) l[k] = *reinterpret_cast<const uint4*>(o_lo + (row * Hq + h) * D + sub * 8);
+      b[k] = *reinterpret_cast<const uint4*>(go + row * g_rs + h * g_hs + sub * 8);
     }
+    L[k] = inside[k] && sub == 0 ? lse[(long long)h * T + row] : -INFINITY;
   }
 #pragma unroll
   for (int k = 0; k < MORE; ++k) {
@@ -76,9 +79,9 @@ __global__ void __launch_bounds__(256) packed_delta_kernel(const bf16* __restric
 #pragma unroll
     for (int i = LANES / 2; i > 0; i >>= 1) s += __shfl_xor_sync(0xffffffffu, s, i);
     if (sub == 0) {
-      const float L = inside[k] ? lse[(long long)h[k] * T + row[k]] : -INFINITY;
-      aux[(long long)h[k] * Tp + row[k]] = L == -INFINITY ? -INFINITY : -L * LOG2E;
-      aux[((long long)Hq + h[k]) * Tp + row[k]] = -s;
+      const long long at = (long long)h * Tp + row0 + k * GROUPS;
+      aux[at] = L[k] == -INFINITY ? -INFINITY : -L[k] * LOG2E;
+      aux[(long long)Hq * Tp + at] = -s;
     }
   }
 }
@@ -743,13 +746,9 @@ extern "C" int dmb_packed_attn_bwd(const void* go, long long g_rs, long long g_h
   const Geo g{cu, aux, nseq, T, tiles * TILE, Hq, Hkv, Hq / Hkv, D, window, tiles, scale, scale * LOG2E};
   cudaStream_t st = (cudaStream_t)stream;
   const long long rows = (long long)g.Tp * Hq;
-  // rows is a multiple of 128, so with 8 or 16 threads for 4 of them every block is full
-  if (D <= 64)
-    packed_delta_kernel<8><<<(unsigned)(rows / MORE * 8 / 256), 256, 0, st>>>((const bf16*)o, (const bf16*)o_lo, (const bf16*)go, g_rs, g_hs, lse, aux, cu,
-                                                                               nseq, T, g.Tp, Hq, D);
-  else
-    packed_delta_kernel<16><<<(unsigned)(rows / MORE * 16 / 256), 256, 0, st>>>((const bf16*)o, (const bf16*)o_lo, (const bf16*)go, g_rs, g_hs, lse, aux, cu,
-                                                                                 nseq, T, g.Tp, Hq, D);
+  const unsigned blocks = (unsigned)(rows / (256 / (D <= 64 ? 8 : 16) * MORE));     // whole ones: Tp is a multiple of 128
+  auto delta = D <= 64 ? packed_delta_kernel<8> : packed_delta_kernel<16>;
+  delta<<<blocks, 256, 0, st>>>((const bf16*)o, (const bf16*)o_lo, (const bf16*)go, g_rs, g_hs, lse, aux, cu, nseq, T, g.Tp, Hq, D);
   DMB_CHECK_LAUNCH();
   return D <= 64 ? launch<64>(mq, mk, mv, mg, (bf16*)dq, (bf16*)dk, (bf16*)dv, g, err, st)
                  : launch<128>(mq, mk, mv, mg, (bf16*)dq, (bf16*)dk, (bf16*)dv, g, err, st);
