@@ -16,13 +16,13 @@
 // take turns with one S (128 + 2 x (64 P + 128 O)).  The turns cost little, since S is held for a product, its latency and one
 // read, and they keep the two tiles half a block apart: one tile's exponentials run while the tensor pipe works for the other.
 //
-// Measured: 8192 rows of one sequence, 16 heads of 64: 191 us (720 TFLOP/s over the visible pairs); 16384 rows, 16 heads of 128:
-// 862 us (1276 TFLOP/s, 77 % of the library product's measured rate); eleven documents in 8192 rows, where half of the
-// blocks hold a border: 52 us.  What bounds: 128 x 128 exponentials take 1024 cycles of the special-function unit, as long as the products at D = 128 and
-// twice as long at D = 64.  So of every eight pairs EMU are computed by a polynomial on the FMA pipe (packed.cuh), in blocks
-// without masked entries.  The running maximum is allowed to lag by up to 8 octaves (P <= 256, exact in the fp32 accumulator's
-// range and no loss of relative precision in 16 bits): O is rescaled in tensor memory only when a row's maximum outgrows
-// that, which after the first blocks is rare.  Sums are fp32; P is rounded to the operand type.
+// Measured: 8192 rows of one sequence, 16 heads of 64: 190 us (722 TFLOP/s over the visible pairs); 16384 rows, 16 heads of 128:
+// 875 us (1257 TFLOP/s, 76 % of the library product's measured rate); eleven documents in 8192 rows, where half of the
+// blocks hold a border: 53 us.  What bounds: 128 x 128 exponentials take 1024 cycles of the special-function unit, as long as
+// the products at D = 128 and twice as long at D = 64.  So of every eight pairs EMU are computed by a polynomial on the FMA pipe
+// (packed.cuh), in blocks without masked entries.  The running maximum is allowed to lag by up to 8 octaves (P <= 256, exact in
+// the fp32 accumulator's range and no loss of relative precision in 16 bits): O is rescaled in tensor memory only when a row's
+// maximum outgrows that, which after the first blocks is rare.  Sums are fp32; P is rounded to the operand type.
 //
 // Every mbarrier wait is bounded in time; on expiry the kernel raises a flag in global memory, stops waiting, lets its own
 // copies land (bounded) and releases its tensor memory.
@@ -40,8 +40,8 @@ struct Cfg {
   static constexpr bool TURNS = TILES == 2;                // one S for both tiles
   static constexpr int NT = (TILES + 1) * 128, ISSUE = TILES * 4, LOAD = ISSUE + 1;      // threads; the issuing and loading warps
   static constexpr int COLS = TILES * 256;                 // tensor memory
-  // pairs of eight on the FMA pipe; 8192 rows, 16 heads: D = 64 1: 188.0, 2: 186.4, 3: 196.2 us; D = 128 0: 226.4, 1: 230.6,
-  // 2: 229.9, 3: 232.8
+  // pairs of eight on the FMA pipe; 8192 rows, 16 query heads and 16 key heads of 64 / 4 of 128: 0: 199.9 / 222.1,
+  // 1: 194.1 / 229.1, 2: 191.1 / 232.8, 3: 190.9 / 236.3 us
   static constexpr int EMU = DH == 64 ? 2 : 0;
   static constexpr int P_OFF = TILE, O_OFF = TILE + TILES * 64;        // S, then P and O of each tile
   static constexpr int TB = TILE * DH * 2;                 // one tile
@@ -51,10 +51,16 @@ struct Cfg {
   static constexpr int total = bar_off + 256;
 };
 
+struct Rows {                             // element (row, head, dim) at p[row * rs + head * hs + dim]
+  const void* p;
+  long long rs, hs;
+};
+
 struct Geo {
   const int* cu;
   int nseq, T, Hq, group, D, window, units;
   float scale_log2;
+  Rows q, k, v;
 };
 
 // 32 weights of a row from 32 scores: exp2(s * scale - sub); returns their sum, leaves the packed columns in p
@@ -87,6 +93,42 @@ __device__ __forceinline__ void store16(T* row, int d0, int D, const uint32_t (&
   } else if (d0 < D) {
     *reinterpret_cast<uint4*>(row + d0) = make_uint4(w[0], w[1], w[2], w[3]);
     if (d0 + 8 < D) *reinterpret_cast<uint4*>(row + d0 + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+  }
+}
+
+// One output row from the keys that it sees, key by key; a whole warp, a lane holds every 32nd dim.  lse2: log2 sum_j 2^s_ij.
+// The products run over blocks of 128 keys, where a weight of zero times an infinite or NaN value is NaN, so a row that does
+// not see that value would get it all the same.  Rows whose scores are finite and whose outputs are not therefore end here,
+// which costs the others nothing at D = 64 and 1 % at D = 128 (78.4 against 79.6 us for 8192 rows, 16 query and 4 key heads).
+template <typename T>
+__device__ __forceinline__ void redo_row(const Geo& g, T* out, T* out_lo, int h, int row, int lo, float lse2) {
+  const int lane = threadIdx.x & 31;
+  const T* q = (const T*)g.q.p + row * g.q.rs + h * g.q.hs;
+  const T* k = (const T*)g.k.p + h / g.group * g.k.hs;
+  const T* v = (const T*)g.v.p + h / g.group * g.v.hs;
+  float x[4], acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = lane + 32 * i < g.D ? (float)q[lane + 32 * i] : 0.f;
+#pragma unroll 1
+  for (long long j = lo; j <= row; ++j) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (lane + 32 * i < g.D) s = fmaf(x[i], (float)k[j * g.k.rs + lane + 32 * i], s);
+#pragma unroll
+    for (int i = 16; i > 0; i >>= 1) s += __shfl_xor_sync(0xffffffffu, s, i);
+    const float w = ex2(fmaf(s, g.scale_log2, -lse2));
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (lane + 32 * i < g.D) acc[i] = fmaf(w, (float)v[j * g.v.rs + lane + 32 * i], acc[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (lane + 32 * i >= g.D) break;
+    const long long at = ((long long)row * g.Hq + h) * g.D + lane + 32 * i;
+    const T o = (T)acc[i];
+    out[at] = o;
+    if (out_lo) out_lo[at] = (T)(acc[i] - (float)o);
   }
 }
 
@@ -333,6 +375,7 @@ __global__ void __launch_bounds__(Cfg<DH>::NT, 3 - Cfg<DH>::TILES) packed_fwd_ke
     tc_fence_after();
     const float inv = some && l != 0.f ? 1.f / l : 0.f;             // no key: zero (NaN sums stay NaN)
     T* o_row = out + ((long long)row * g.Hq + h) * g.D;
+    float bad[4] = {0.f, 0.f, 0.f, 0.f};                             // one is NaN once an output is not finite
 #pragma unroll
     for (int c = 0; c < DH / 32; ++c) {
       uint32_t o[32];
@@ -351,6 +394,8 @@ __global__ void __launch_bounds__(Cfg<DH>::NT, 3 - Cfg<DH>::TILES) packed_fwd_ke
 #pragma unroll
           for (int i = 0; i < 16; ++i) f[i] = inv == 0.f ? 0.f : __uint_as_float(o[16 * u + i]) * inv;
 #pragma unroll
+          for (int i = 0; i < 16; ++i) bad[i & 3] = fmaf(f[i], 0.f, bad[i & 3]);
+#pragma unroll
           for (int i = 0; i < 8; ++i) w[i] = Elem<T>::pack(f[2 * i], f[2 * i + 1]);
           store16(o_row, 32 * c + 16 * u, g.D, w);
           if (out_lo) {                                            // what the rounding left
@@ -364,8 +409,15 @@ __global__ void __launch_bounds__(Cfg<DH>::NT, 3 - Cfg<DH>::TILES) packed_fwd_ke
         }
       }
     }
-    if (lse && row < g.T)
-      lse[(long long)h * g.T + row] = inv == 0.f ? -INFINITY : (m + log2f(l)) * (1.f / LOG2E);
+    const float lse2 = inv == 0.f ? -INFINITY : m + log2f(l);
+    if (lse && row < g.T) lse[(long long)h * g.T + row] = lse2 * (1.f / LOG2E);
+    const bool again = (bad[0] + bad[1]) + (bad[2] + bad[3]) != 0.f && fabsf(lse2) < INFINITY;
+    unsigned todo = __ballot_sync(0xffffffffu, again);
+    for (; __builtin_expect(todo != 0, 0); todo &= todo - 1) {
+      const int who = __ffs(todo) - 1;
+      __syncwarp();                                                  // after the lane's own stores
+      redo_row<T>(g, out, out_lo, h, w_row + who, __shfl_sync(0xffffffffu, lo, who), __shfl_sync(0xffffffffu, lse2, who));
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -403,7 +455,7 @@ extern "C" int dmb_packed_attn_fwd(const void* q, long long q_rs, long long q_hs
   if (rc) return rc;
   const int rows = (D <= 64 ? Cfg<64>::TILES : Cfg<128>::TILES) * TILE, units = (int)(((long long)T + rows - 1) / rows);
   if ((long long)units * Hq > 0x7fffffffLL) return -1;
-  const Geo g{cu, nseq, T, Hq, Hq / Hkv, D, window, units, scale * LOG2E};
+  const Geo g{cu, nseq, T, Hq, Hq / Hkv, D, window, units, scale * LOG2E, {q, q_rs, q_hs}, {k, k_rs, k_hs}, {v, v_rs, v_hs}};
   cudaStream_t st = (cudaStream_t)stream;
   if (half) return D <= 64 ? launch<__half, 64>(mq, mk, mv, o, o_lo, lse, g, err, st) : launch<__half, 128>(mq, mk, mv, o, o_lo, lse, g, err, st);
   return D <= 64 ? launch<bf16, 64>(mq, mk, mv, o, o_lo, lse, g, err, st) : launch<bf16, 128>(mq, mk, mv, o, o_lo, lse, g, err, st);

@@ -62,7 +62,9 @@ def packed_attn_fwd(q, k, v, cu, window, scale):
         total = p.sum(-1, keepdim=True)
         vf = v[:rows.stop].float().transpose(0, 1)[:, None]
         some = total != 0
-        full = _heads_last(torch.where(some, (p @ vf) / total, 0.0))
+        wild = ~vf.isfinite()                              # a hidden one would reach the row as 0 x NaN, so: who sees one
+        pv = (p @ vf.masked_fill(wild, 0.0)).masked_fill((~hidden).float() @ wild.float() > 0, float("nan"))
+        full = _heads_last(torch.where(some, pv / total, 0.0))
         o[rows] = full.to(q.dtype)
         o_lo[rows] = (full - o[rows].float()).to(q.dtype)
         lse[:, rows] = torch.where(some, top + total.log(), float("-inf")).reshape(Hq, -1)

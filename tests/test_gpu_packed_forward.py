@@ -130,6 +130,30 @@ def test_packed_nonfinite_score_stays_in_its_row(ops):
     assert torch.equal(o[keep], base[keep])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d, residual", [(64, False), (64, True), (128, False), (40, True)])
+def test_packed_nonfinite_value_reaches_the_rows_that_see_it(ops, dtype, d, residual):
+    """Infinite and NaN value rows: every row that does not see them is as without them, in its own sequence (before them, or
+    behind their window) and in the others of the same block of rows."""
+    q, k, v = (rnd(300, 4, d, seed=s).to(dtype) for s in (1, 2, 3))
+    k, v = k[:, :2].contiguous(), v[:, :2].contiguous()
+    cu = cu_of(0, 60, 200, 299)
+    grad = residual                                      # a training call writes what the rounding left as well
+    for window in (0, 25):
+        want = ref.packed(q, k, v, cu, window=window)["o"]
+        w = v.clone()
+        w[30, 0, 3] = float("inf")
+        w[100, 1, 5] = float("nan")
+        w[299] = float("nan")                            # padding
+        o = ops.packed_attention(q.clone().requires_grad_(grad), k, w, cu, window=window).detach()
+        sees = torch.zeros(300, 4, d, dtype=torch.bool, device=DEV)
+        sees[30:min(60, 30 + (window or 300)), :2, 3] = True
+        sees[100:min(200, 100 + (window or 300)), 2:, 5] = True
+        assert not o[sees].isfinite().any() and (o[30, 0, 3] == float("inf")) and o[100, 2, 5].isnan()
+        assert o[~sees].isfinite().all()
+        ref.close(torch.where(sees, want[0].to(dtype), o), want, f"o {window}")
+
+
 def test_packed_wrong_table_reads_nothing_out_of_range(ops):
     """Tables that do not ascend or point outside the rows: any output, but the call ends and the next one is right."""
     q, k, v = (rnd(300, 2, 64, seed=s) for s in (1, 2, 3))

@@ -44,6 +44,18 @@ def test_packed_padding_is_not_read():
         torch.testing.assert_close(got.double(), want[name][0], **F64_NEAR)
 
 
+def test_packed_nonfinite_value_reaches_the_rows_that_see_it():
+    q, k, v = (rnd(20, 2, 8, seed=s) for s in range(3))
+    cu = torch.tensor([0, 8, 20], dtype=torch.int32)
+    want = ref.packed(q, k, v, cu, window=4)["o"][0]
+    v[5, 1, 3] = float("inf")
+    o = packed_attention(q, k, v, cu, window=4)
+    sees = torch.zeros(20, 2, 8, dtype=torch.bool)
+    sees[5:8, 1, 3] = True
+    assert not o[sees].isfinite().any()
+    torch.testing.assert_close(o[~sees].double(), want[~sees], **F64_NEAR)
+
+
 @pytest.mark.parametrize("window", [0, 1, 6])
 def test_cached_statement(window):
     q, k, v = rnd(5, 4, 8, seed=1), rnd(5, 30, 2, 8, seed=2), rnd(5, 30, 2, 8, seed=3)
