@@ -3,14 +3,15 @@
 //   m = max x,  S = sum exp(x - m),  logp = (x_y - m) - log S,  H = log S - sum p (x - m),  p = exp(x - m) / S
 //   d x = g_logp (1[y] - p) - g_H p (log p + H)
 //
-// Both passes stream the row once with 16-byte loads and are bound by DRAM (8191 x 32000 bf16: forward 102 us, 5.1 TB/s, with the
-// greedy entry 117 us; the exponentials take 60 % of the special-function unit meanwhile; backward 169 us, 6.2 TB/s).  Forward: a
-// group of 32 to 1024 threads per row (see `fwd`), two sets of loads in flight per thread, running maximum and sums per thread (fp32; a thread adds
-// its part of the row, the rest is a tree), so nothing of the row is kept.  A block takes rows in turn and requests the next
-// row's first part before it joins the sums of the last.  A row whose entries all are the type's lowest value is uniform, as it
-// should be.
+// Both passes stream the row once with 16-byte loads and are bound by DRAM (8191 x 32000 bf16: forward 100 us, 5.2 TB/s, with the
+// greedy entry 115 us; the exponentials take 60 % of the special-function unit meanwhile; backward 169 us, 6.2 TB/s).  Forward: a
+// group of 32 to 1024 threads per row (see `fwd`), two sets of loads in flight per thread, running maximum and sums per thread
+// (fp32; a thread adds its part of the row, the rest is a tree).  A block takes rows in turn and requests the next row's first
+// part before it joins the sums of the last.  A row whose entries all are the type's lowest value is uniform, as it should be.
+// The rows in flight may not fit L2, so reading an entry again costs a round trip to DRAM under load.  The greedy entry does
+// without: a thread keeps the set of vectors that its maximum came with in shared memory (125 -> 115 us).
 // Alternatives: the maxima of 32 parts of the row are entries of it, so the top-th largest of them bounds the top-th largest
-// entry from below; only threads whose own maximum reaches the bound look at their entries again (from L2), and what reaches
+// entry from below; only threads whose own maximum reaches the bound have their entries looked at again, and what reaches
 // the bound, a few entries more than `top`, is ranked by (value, lower index first).
 // A row has no target where its token is negative: logp = 0, no gradient through it.  A token beyond the vocabulary gives NaN.
 #include "packed.cuh"
@@ -131,9 +132,9 @@ struct Run {
     s += p;
     e = fmaf(p, fmaxf(y, LOWEST), e);
   }
-  // K vectors at once; `live` of them count
+  // K vectors at once; `live` of them count.  Returns their largest entry (NaN aside).
   template <typename T, int K>
-  __device__ __forceinline__ void many(const uint4 (&u)[K], int live) {
+  __device__ __forceinline__ float many(const uint4 (&u)[K], int live) {
     constexpr int N = Vec<T>::N;
     float top = -INFINITY;
 #pragma unroll
@@ -141,7 +142,10 @@ struct Run {
       if (k < live) top = fmaxf(top, Vec<T>::top(u[k]));
     if (top > m) raise(top);
     if (plain(m)) {
-      float s0 = 0.f, s1 = 0.f, e0 = 0.f, e1 = 0.f;
+      // pairs: a packed instruction takes as long as two, but one place in the issue queue
+      using namespace packed;
+      const f32x2 scale = pair(L2E, L2E), off = pair(-ref, -ref);
+      f32x2 ss = pair(0.f, 0.f), ee = ss;
 #pragma unroll
       for (int k = 0; k < K; ++k)
         if (k < live) {
@@ -149,17 +153,21 @@ struct Run {
           Vec<T>::get(u[k], v);
 #pragma unroll
           for (int i = 0; i < N; i += 2) {
-            const float y0 = fmaf(v[i], L2E, -ref), y1 = fmaf(v[i + 1], L2E, -ref), p0 = ex2(y0), p1 = ex2(y1);
-            s0 += p0;
-            s1 += p1;
-            e0 = fmaf(p0, y0, e0);
-            e1 = fmaf(p1, y1, e1);
+            const f32x2 y = fma2(pair(v[i], v[i + 1]), scale, off);
+            float y0, y1;
+            split(y, y0, y1);
+            const f32x2 q = pair(ex2(y0), ex2(y1));
+            ss = add2(ss, q);
+            ee = fma2(q, y, ee);
           }
         }
+      float s0, s1, e0, e1;
+      split(ss, s0, s1);
+      split(ee, e0, e1);
       if (e0 + e1 == e0 + e1) {
         s += s0 + s1;
         e += e0 + e1;
-        return;
+        return top;
       }
     }
 #pragma unroll 1
@@ -174,6 +182,7 @@ struct Run {
       for (int i = 0; i < N; ++i)
         if (k < live) one(v[i]);
     }
+    return top;
   }
   // the sums relative to m itself, e in natural units
   __device__ __forceinline__ void finish() {
@@ -201,23 +210,27 @@ struct Group {
     if (NT == 32) __syncwarp(); else __syncthreads();
   }
 };
-template <int NT>
+enum Top { NONE, GREEDY, RANKED };
+constexpr int AHEAD = 4;                                      // vectors of a set of loads
+template <int NT, Top TOP>
 struct Shared {                                               // of one group
-  float m[Group<NT>::WARPS], s[Group<NT>::WARPS], e[Group<NT>::WARPS], part[32], bound;
-  int n;
-  float cv[Group<NT>::CAP];
-  int ci[Group<NT>::CAP];
+  static constexpr int CAP = TOP == RANKED ? Group<NT>::CAP : 1;
+  float m[Group<NT>::WARPS], s[Group<NT>::WARPS], e[Group<NT>::WARPS], part[32];
+  int n, first[Group<NT>::WARPS];
+  float cv[CAP];
+  int ci[CAP];
+  uint4 kept[AHEAD][TOP == GREEDY ? NT : 1];
 };
 
-template <int NT, typename T, bool TOP>
+template <int NT, typename T, Top TOP>
 __global__ void __launch_bounds__(Group<NT>::BLOCK, Group<NT>::BLOCKS)
 logprob_fwd_kernel(const T* __restrict__ logits, long long rs, const long long* __restrict__ tokens, int rows, int V, int top,
                    float* __restrict__ logp, float* __restrict__ entropy, float2* __restrict__ stats,
                    float* __restrict__ top_logp, long long* __restrict__ top_ids) {
   using G = Group<NT>;
-  constexpr int N = Vec<T>::N, K = 4;
-  __shared__ Shared<NT> shared[G::ROWS];
-  Shared<NT>& sh = shared[threadIdx.x / NT];
+  constexpr int N = Vec<T>::N, K = AHEAD, CAP = Shared<NT, TOP>::CAP;
+  __shared__ Shared<NT, TOP> shared[G::ROWS];
+  Shared<NT, TOP>& sh = shared[threadIdx.x / NT];
   const int t = threadIdx.x % NT, lane = t & 31, warp = t >> 5;
   const long long step = (long long)gridDim.x * G::ROWS;
   long long row = (long long)blockIdx.x * G::ROWS + threadIdx.x / NT;
@@ -246,12 +259,24 @@ logprob_fwd_kernel(const T* __restrict__ logits, long long rs, const long long* 
   for (;;) {
     Run r{-INFINITY, 0.f, 0.f, 0.f};
     const long long target = y;
-    if (t < c.head) r.one(Vec<T>::one(edge0));
-    if (c.tail0 + t < V) r.one(Vec<T>::one(edge1));
+    const float head = t < c.head ? Vec<T>::one(edge0) : NAN, tail = c.tail0 + t < V ? Vec<T>::one(edge1) : NAN;
+    if (t < c.head) r.one(head);
+    if (c.tail0 + t < V) r.one(tail);
+    float best = -INFINITY;                                   // of the vectors; where the set that it came with begins
+    int best_i = 0;
+    auto take = [&](const uint4 (&u)[K], int i) {
+      const float top_u = r.template many<T, K>(u, min(K, (c.nvec - i + NT - 1) / NT));
+      if (TOP == GREEDY && top_u > best) {
+        best = top_u;
+        best_i = i;
+#pragma unroll
+        for (int k = 0; k < K; ++k) sh.kept[k][t] = u[k];
+      }
+    };
     for (int i = t; i < c.nvec; i += 2 * K * NT) {
-      r.template many<T, K>(a, min(K, (c.nvec - i + NT - 1) / NT));
+      take(a, i);
       fetch(a, x, c, i + 2 * K * NT);
-      if (i + K * NT < c.nvec) r.template many<T, K>(b, min(K, (c.nvec - i - K * NT + NT - 1) / NT));
+      if (i + K * NT < c.nvec) take(b, i + K * NT);
       fetch(b, x, c, i + 3 * K * NT);
     }
     // the next row's first vectors travel while this row's sums are joined
@@ -266,7 +291,7 @@ logprob_fwd_kernel(const T* __restrict__ logits, long long rs, const long long* 
     if (t == 0 && target >= 0 && target < V) xy = Vec<T>::one(x[target]);
     // ---- the row's sums: within the warp, then across warps ----
     const float own = r.m;
-    if (TOP) {                                                // maxima of the groups of NT / 32 threads
+    if (TOP == RANKED) {                                      // maxima of the groups of NT / 32 threads
       float part = own;
 #pragma unroll
       for (int o = 1; o < NT / 32; o <<= 1) part = fmaxf(part, __shfl_xor_sync(0xffffffffu, part, o));
@@ -306,8 +331,35 @@ logprob_fwd_kernel(const T* __restrict__ logits, long long rs, const long long* 
       entropy[row] = ls - r.e / r.s;
       if (stats) stats[row] = make_float2(r.m, ls);
     }
+    // ---- the largest entry alone: its first place ----
+    if (TOP == GREEDY) {
+      int at = V;
+      if (r.m == -INFINITY) at = 0;                           // nothing but -inf and NaN
+      else if (head == r.m) at = t;
+      else if (best == r.m) {
+#pragma unroll
+        for (int k = K - 1; k >= 0; --k)
+          if (best_i + k * NT < c.nvec) {
+            float v[N];
+            Vec<T>::get(sh.kept[k][t], v);
+#pragma unroll
+            for (int i = N - 1; i >= 0; --i)
+              if (v[i] == r.m) at = c.head + (best_i + k * NT) * N + i;
+          }
+      } else if (tail == r.m) at = c.tail0 + t;
+      at = __reduce_min_sync(0xffffffffu, at);
+      if (G::WARPS > 1) {
+        if (lane == 0) sh.first[warp] = at;
+        G::sync();
+        at = __reduce_min_sync(0xffffffffu, sh.first[lane % G::WARPS]);
+      }
+      if (t == 0) {
+        top_logp[row] = (r.m - r.m) - ls;
+        top_ids[row] = at;
+      }
+    }
     // ---- alternatives ----
-    if (TOP) {
+    if (TOP == RANKED) {
       float bound = r.m;
       if (top > 1) {
         const float v0 = sh.part[lane];                       // every warp ranks the 32 maxima
@@ -331,29 +383,46 @@ logprob_fwd_kernel(const T* __restrict__ logits, long long rs, const long long* 
       auto offer = [&](float v, int i) {
         if (!(v < bound)) {                                   // NaN goes in as well: it is ranked as the smallest
           const int at = atomicAdd(&sh.n, 1);                 // the list's order does not matter: it is ranked
-          if (at < G::CAP) { sh.cv[at] = v == v ? v : -INFINITY; sh.ci[at] = i; }
+          if (at < CAP) { sh.cv[at] = v == v ? v : -INFINITY; sh.ci[at] = i; }
         }
       };
       if (NT == 32) {
         if (!(own < bound)) each_own(offer);
       } else {
-        // the warp looks at one such thread's entries together: one latency instead of one per vector
-        for (unsigned todo = __ballot_sync(0xffffffffu, !(own < bound)); todo; todo &= todo - 1) {
-          const int tt = warp * 32 + __ffs(todo) - 1;
-          const uint4* body = reinterpret_cast<const uint4*>(x + c.head);
-          for (int i = tt + NT * lane; i < c.nvec; i += NT * 32) {
-            float v[N];
-            Vec<T>::get(__ldg(body + i), v);
+        // the warp looks at such threads' entries together, LOOK stretches of 32 vectors in flight (8191 x 32000 bf16, top 8:
+        // 1: 152, 2: 149, 4: 160 us)
+        constexpr int LOOK = 2;
+        const uint4* body = reinterpret_cast<const uint4*>(x + c.head);
+        unsigned left = __ballot_sync(0xffffffffu, !(own < bound));
+        int from = 0;                                         // next vector of the thread that is looked at, in its own count
+        while (left) {
+          uint4 u[LOOK];
+          int at[LOOK];
 #pragma unroll
-            for (int k = 0; k < N; ++k) offer(v[k], c.head + i * N + k);
+          for (int k = 0; k < LOOK; ++k) {
+            const int tt = warp * 32 + __ffs(left) - 1;
+            at[k] = left ? tt + NT * (from + lane) : c.nvec;
+            if (at[k] < c.nvec) u[k] = __ldg(body + at[k]);
+            from += 32;
+            if (from * NT >= c.nvec) { from = 0; left &= left - 1; }
           }
-          if (lane == 0 && tt < c.head) offer(Vec<T>::one(x[tt]), tt);
-          if (lane == 1 && c.tail0 + tt < V) offer(Vec<T>::one(x[c.tail0 + tt]), c.tail0 + tt);
+#pragma unroll
+          for (int k = 0; k < LOOK; ++k)
+            if (at[k] < c.nvec && !(Vec<T>::top(u[k]) < bound)) {        // all NaN: true
+              float v[N];
+              Vec<T>::get(u[k], v);
+#pragma unroll
+              for (int i = 0; i < N; ++i) offer(v[i], c.head + at[k] * N + i);
+            }
+        }
+        if (!(own < bound)) {
+          if (t < c.head) offer(Vec<T>::one(x[t]), t);
+          if (c.tail0 + t < V) offer(Vec<T>::one(x[c.tail0 + t]), c.tail0 + t);
         }
       }
       G::sync();
       const int n = sh.n;
-      if (n <= G::CAP) {
+      if (n <= CAP) {
         for (int q = t; q < n; q += NT) {
           const float v = sh.cv[q];
           const int i = sh.ci[q];
@@ -475,15 +544,17 @@ int fwd_nt(const T* x, long long rs, const long long* tok, int rows, int V, int 
   using G = Group<NT>;
   // as many blocks as are resident (sharing the rows out evenly over fewer blocks was slower: 108 against 102 us)
   const int grid = min((rows - 1) / G::ROWS + 1, SMS * G::BLOCKS);
-  if (top > 0) logprob_fwd_kernel<NT, T, true><<<grid, G::BLOCK, 0, s>>>(x, rs, tok, rows, V, top, lp, ent, st, tlp, tid);
-  else logprob_fwd_kernel<NT, T, false><<<grid, G::BLOCK, 0, s>>>(x, rs, tok, rows, V, top, lp, ent, st, tlp, tid);
+  // one entry: from the sets of vectors that the threads keep in shared memory (64 bytes each, so not with 1024 threads)
+  constexpr Top ONE = NT < 1024 ? GREEDY : RANKED;
+  auto kern = top == 0 ? logprob_fwd_kernel<NT, T, NONE> : top == 1 ? logprob_fwd_kernel<NT, T, ONE> : logprob_fwd_kernel<NT, T, RANKED>;
+  kern<<<grid, G::BLOCK, 0, s>>>(x, rs, tok, rows, V, top, lp, ent, st, tlp, tid);
   DMB_CHECK_LAUNCH();
   return 0;
 }
 // Threads per row.  Few threads: little to join per row; many: a row alone goes fast.  A warp where a row is short (16384 x 259:
 // 27 us against 420 with 256 threads); 1024 where every row has an SM to itself; between them as few as keep two rounds of
 // rows (8191 x 32000 bf16: 64 threads 102, 128 108, 256 113 us; 1021 x 50257 fp32: 128 61, 256 53 us).  Ranking alternatives
-// wants more of them (8191 x 32000, top 8: 64 176, 128 152, 256 172 us).
+// wants more of them (8191 x 32000, top 8: 64 176, 128 152, 256 172 us before its loads went two at a time).
 template <typename T>
 int fwd(const void* xv, long long rs, const long long* tok, int rows, int V, int top, float* lp, float* ent, float2* st,
         float* tlp, long long* tid, cudaStream_t s) {

@@ -302,3 +302,24 @@ def test_logprobs_views(ops, dtype):
     r = ops.token_logprobs(x, y.view(2, 3) % 100, top=2)
     assert r.logp.shape == (2, 3) and r.top_ids.shape == (2, 3, 2)
     assert ops.token_logprobs(x[:0], y.view(2, 3)[:0], top=2).top_logp.shape == (0, 3, 2)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows, V", [(20, 1000), (9, 1), (300, 17), (20, 5001), (300, 40001), (2500, 3001), (5000, 2503)])
+def test_greedy_entry_is_the_first_of_equals(ops, dtype, rows, V):
+    """Coarse entries: many equals, in the vectors and before and behind them (rows start at any alignment)."""
+    g = torch.Generator(device=DEV).manual_seed(V)
+    x = torch.randint(-6, 7, (rows, V), generator=g, device=DEV).to(dtype)
+    x[1] = float("-inf")
+    x[2, : V // 2] = float("-inf")
+    x[3] = 0
+    x[4, : V - 1] = float("nan")
+    y = torch.zeros(rows, dtype=torch.int64, device=DEV)
+    r = ops.token_logprobs(x, y, top=1)
+    key = x.float().nan_to_num(nan=float("-inf"), neginf=float("-inf"), posinf=float("inf"))
+    first = (key == key.amax(-1, keepdim=True)).int().argmax(-1)
+    assert torch.equal(r.top_ids[:, 0], first)
+    keep = torch.arange(rows, device=DEV) > 4
+    at = ops.token_logprobs(x, first).logp
+    assert torch.equal(r.top_logp[keep, 0], at[keep])
+    assert r.top_logp[1].isnan().all() and r.top_logp[4].isnan().all() or V == 1
