@@ -4,12 +4,12 @@
 //   d x = g_logp (1[y] - p) - g_H p (log p + H)
 //
 // Both passes stream the row once with 16-byte loads and are bound by DRAM (8191 x 32000 bf16: forward 100 us, 5.2 TB/s, with the
-// greedy entry 115 us; the exponentials take 60 % of the special-function unit meanwhile; backward 169 us, 6.2 TB/s).  Forward: a
+// greedy entry 108 us; the exponentials take 60 % of the special-function unit meanwhile; backward 169 us, 6.2 TB/s).  Forward: a
 // group of 32 to 1024 threads per row (see `fwd`), two sets of loads in flight per thread, running maximum and sums per thread
 // (fp32; a thread adds its part of the row, the rest is a tree).  A block takes rows in turn and requests the next row's first
 // part before it joins the sums of the last.  A row whose entries all are the type's lowest value is uniform, as it should be.
 // The rows in flight may not fit L2, so reading an entry again costs a round trip to DRAM under load.  The greedy entry does
-// without: a thread keeps the set of vectors that its maximum came with in shared memory (125 -> 115 us).
+// without: a thread keeps the set of vectors that its maximum came with in shared memory (116 -> 108 us).
 // Alternatives: the maxima of 32 parts of the row are entries of it, so the top-th largest of them bounds the top-th largest
 // entry from below; only threads whose own maximum reaches the bound have their entries looked at again, and what reaches
 // the bound, a few entries more than `top`, is ranked by (value, lower index first).
@@ -132,15 +132,16 @@ struct Run {
     s += p;
     e = fmaf(p, fmaxf(y, LOWEST), e);
   }
-  // K vectors at once; `live` of them count.  Returns their largest entry (NaN aside).
+  // K vectors at once; `live` of them count.  Returns whether the maximum moved.
   template <typename T, int K>
-  __device__ __forceinline__ float many(const uint4 (&u)[K], int live) {
+  __device__ __forceinline__ bool many(const uint4 (&u)[K], int live) {
     constexpr int N = Vec<T>::N;
     float top = -INFINITY;
 #pragma unroll
     for (int k = 0; k < K; ++k)
       if (k < live) top = fmaxf(top, Vec<T>::top(u[k]));
-    if (top > m) raise(top);
+    const bool up = top > m;
+    if (up) raise(top);
     if (plain(m)) {
       // pairs: a packed instruction takes as long as two, but one place in the issue queue
       using namespace packed;
@@ -167,7 +168,7 @@ struct Run {
       if (e0 + e1 == e0 + e1) {
         s += s0 + s1;
         e += e0 + e1;
-        return top;
+        return up;
       }
     }
 #pragma unroll 1
@@ -182,7 +183,7 @@ struct Run {
       for (int i = 0; i < N; ++i)
         if (k < live) one(v[i]);
     }
-    return top;
+    return up;
   }
   // the sums relative to m itself, e in natural units
   __device__ __forceinline__ void finish() {
@@ -219,7 +220,8 @@ struct Shared {                                               // of one group
   int n, first[Group<NT>::WARPS];
   float cv[CAP];
   int ci[CAP];
-  uint4 kept[AHEAD][TOP == GREEDY ? NT : 1];
+  uint4 kept[AHEAD][TOP == GREEDY ? NT : 1];                  // the vectors that a thread's maximum came with, the first's place
+  int kept_i[TOP == GREEDY ? NT : 1];
 };
 
 template <int NT, typename T, Top TOP>
@@ -259,16 +261,9 @@ logprob_fwd_kernel(const T* __restrict__ logits, long long rs, const long long* 
   for (;;) {
     Run r{-INFINITY, 0.f, 0.f, 0.f};
     const long long target = y;
-    const float head = t < c.head ? Vec<T>::one(edge0) : NAN, tail = c.tail0 + t < V ? Vec<T>::one(edge1) : NAN;
-    if (t < c.head) r.one(head);
-    if (c.tail0 + t < V) r.one(tail);
-    float best = -INFINITY;                                   // of the vectors; where the set that it came with begins
-    int best_i = 0;
     auto take = [&](const uint4 (&u)[K], int i) {
-      const float top_u = r.template many<T, K>(u, min(K, (c.nvec - i + NT - 1) / NT));
-      if (TOP == GREEDY && top_u > best) {
-        best = top_u;
-        best_i = i;
+      if (r.template many<T, K>(u, min(K, (c.nvec - i + NT - 1) / NT)) && TOP == GREEDY) {
+        sh.kept_i[t] = i;
 #pragma unroll
         for (int k = 0; k < K; ++k) sh.kept[k][t] = u[k];
       }
@@ -279,6 +274,9 @@ logprob_fwd_kernel(const T* __restrict__ logits, long long rs, const long long* 
       if (i + K * NT < c.nvec) take(b, i + K * NT);
       fetch(b, x, c, i + 3 * K * NT);
     }
+    const float best = r.m, head = t < c.head ? Vec<T>::one(edge0) : NAN, tail = c.tail0 + t < V ? Vec<T>::one(edge1) : NAN;
+    if (t < c.head) r.one(head);
+    if (c.tail0 + t < V) r.one(tail);
     // the next row's first vectors travel while this row's sums are joined
     const long long next = row + step;
     const T* xn = logits + next * rs;
@@ -337,14 +335,15 @@ logprob_fwd_kernel(const T* __restrict__ logits, long long rs, const long long* 
       if (r.m == -INFINITY) at = 0;                           // nothing but -inf and NaN
       else if (head == r.m) at = t;
       else if (best == r.m) {
+        const int i0 = sh.kept_i[t];
 #pragma unroll
         for (int k = K - 1; k >= 0; --k)
-          if (best_i + k * NT < c.nvec) {
+          if (i0 + k * NT < c.nvec) {
             float v[N];
             Vec<T>::get(sh.kept[k][t], v);
 #pragma unroll
             for (int i = N - 1; i >= 0; --i)
-              if (v[i] == r.m) at = c.head + (best_i + k * NT) * N + i;
+              if (v[i] == r.m) at = c.head + (i0 + k * NT) * N + i;
           }
       } else if (tail == r.m) at = c.tail0 + t;
       at = __reduce_min_sync(0xffffffffu, at);
