@@ -114,7 +114,7 @@ class PackedDecoder:
         return self
 
     def step(self, tokens):
-        """tokens int64 [rows] -> (next ids, log probabilities) [rows]."""
+        """tokens int64 [rows] -> (next ids, log probabilities) [rows].  Captured, every step returns the same two tensors."""
         self.tok.copy_(tokens)
         if self.graph is None:
             return self._step()
