@@ -99,7 +99,9 @@ __device__ __forceinline__ void store16(T* row, int d0, int D, const uint32_t (&
 // One output row from the keys that it sees, key by key; a whole warp, a lane holds every 32nd dim.  lse2: log2 sum_j 2^s_ij.
 // The products run over blocks of 128 keys, where a weight of zero times an infinite or NaN value is NaN, so a row that does
 // not see that value would get it all the same.  Rows whose scores are finite and whose outputs are not therefore end here,
-// which costs the others nothing at D = 64 and 1 % at D = 128 (78.4 against 79.6 us for 8192 rows, 16 query and 4 key heads).
+// which costs the others up to 1 % (8192 mixed rows, 16 query and 4 key heads of 128: 78.4 against 79.6 us), and the smallest
+// launches up to a microsecond of instruction fetches (731 rows, 16 heads of 64: 8.4 us with and without on some devices, 8.4
+// against 9.5 on others).
 template <typename T>
 __device__ __forceinline__ void redo_row(const Geo& g, T* out, T* out_lo, int h, int row, int lo, float lse2) {
   const int lane = threadIdx.x & 31;
