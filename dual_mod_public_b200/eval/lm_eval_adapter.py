@@ -225,7 +225,7 @@ class DualModEval(_Base):
             if batch and held + len(toks) > self.packed_tokens:
                 self._score_pack(batch, out)
                 batch, held = [], 0
-            batch.append((i, toks, min(n_c, len(toks) - 1)))
+            batch.append((i, toks, min(n_c, max(0, len(toks) - 1))))
             held += len(toks)
         if batch:
             self._score_pack(batch, out)
