@@ -96,9 +96,11 @@ __device__ __forceinline__ void store16(T* row, int d0, int D, const uint32_t (&
   }
 }
 
-// One output row from the keys that it sees, key by key; a whole warp, a lane holds every 32nd dim.  lse2: log2 sum_j 2^s_ij.
+// One output row from the keys that it sees; a whole warp: a lane scores one of 32 keys, then holds every 32nd dim.  lse2: log2 of
+// the row's sum.
 // The products run over blocks of 128 keys, where a weight of zero times an infinite or NaN value is NaN, so a row that does
-// not see that value would get it all the same.  Rows whose scores are finite and whose outputs are not therefore end here,
+// not see that value would get it all the same.  Rows whose scores are finite and whose outputs are not therefore end here
+// (with an infinite value in every row of one sequence of 16384, 16 heads of 64: 271 ms),
 // which costs the others up to 1 % (8192 mixed rows, 16 query and 4 key heads of 128: 78.4 against 79.6 us), and the smallest
 // launches up to a microsecond of instruction fetches (731 rows, 16 heads of 64: 8.4 us with and without on some devices, 8.4
 // against 9.5 on others).
@@ -108,21 +110,32 @@ __device__ __forceinline__ void redo_row(const Geo& g, T* out, T* out_lo, int h,
   const T* q = (const T*)g.q.p + row * g.q.rs + h * g.q.hs;
   const T* k = (const T*)g.k.p + h / g.group * g.k.hs;
   const T* v = (const T*)g.v.p + h / g.group * g.v.hs;
-  float x[4], acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = lane + 32 * i < g.D ? (float)q[lane + 32 * i] : 0.f;
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
-  for (long long j = lo; j <= row; ++j) {
+  for (long long j0 = lo; j0 <= row; j0 += 32) {
     float s = 0.f;
+    if (j0 + lane <= row) {
+#pragma unroll 2
+      for (int d = 0; d < g.D; d += 8) {
+        const uint4 a = *reinterpret_cast<const uint4*>(q + d), b = *reinterpret_cast<const uint4*>(k + (j0 + lane) * g.k.rs + d);
+        const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (lane + 32 * i < g.D) s = fmaf(x[i], (float)k[j * g.k.rs + lane + 32 * i], s);
-#pragma unroll
-    for (int i = 16; i > 0; i >>= 1) s += __shfl_xor_sync(0xffffffffu, s, i);
+        for (int i = 0; i < 4; ++i) {
+          const float2 e = Elem<T>::unpack(x[i]), f = Elem<T>::unpack(y[i]);
+          s = fmaf(e.x, f.x, s);
+          s = fmaf(e.y, f.y, s);
+        }
+      }
+    }
     const float w = ex2(fmaf(s, g.scale_log2, -lse2));
+    const int n = (int)min(32LL, row + 1 - j0);
+#pragma unroll 4
+    for (int u = 0; u < n; ++u) {
+      const float p = __shfl_sync(0xffffffffu, w, u);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (lane + 32 * i < g.D) acc[i] = fmaf(w, (float)v[j * g.v.rs + lane + 32 * i], acc[i]);
+      for (int i = 0; i < 4; ++i)
+        if (lane + 32 * i < g.D) acc[i] = fmaf(p, (float)v[(j0 + u) * g.v.rs + lane + 32 * i], acc[i]);
+    }
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
