@@ -237,7 +237,7 @@ __device__ __forceinline__ float ex2(float v) {               // special-functio
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
-// 2^y of a pair on the FMA pipe, for finite y <= 126 (below -126: 2^-126).  y = n + f with n = round(y), |f| <= 1/2; 2^f by the
+// 2^y of a pair on the FMA pipe, for y <= 126 (below -126, and for NaN: 2^-126).  y = n + f with n = round(y), |f| <= 1/2; 2^f by the
 // minimax polynomial of degree 4 in relative error (Remez exchange on [-1/2, 1/2]: 2.7e-6), n added to the exponent field.
 __device__ __forceinline__ void ex2_pair(f32x2 y, float& lo, float& hi) {
   float a, b;

@@ -388,6 +388,11 @@ __global__ void __launch_bounds__(Cfg<DH>::NT, 3 - Cfg<DH>::TILES) packed_fwd_ke
     const bool some = n > 0;
     if (some) wait(pvdone(a), (n - 1) & 1, serr);
     tc_fence_after();
+    // A row whose maximum is infinite is decided here and not by its weights, as the polynomial turns the exponents NaN and -inf
+    // into 2^-126: a score of +inf makes the row NaN, and a row that has seen nothing but -inf is a row without keys.  (Such
+    // weights beside a finite maximum are at most 2^-118 of the sum.)
+    if (m == INFINITY) l = NAN;
+    if (m == -INFINITY) l = 0.f;
     const float inv = some && l != 0.f ? 1.f / l : 0.f;             // no key: zero (NaN sums stay NaN)
     T* o_row = out + ((long long)row * g.Hq + h) * g.D;
     float bad[4] = {0.f, 0.f, 0.f, 0.f};                             // one is NaN once an output is not finite

@@ -90,8 +90,9 @@ def packed_attention(q, k, v, cu_seqlens, *, window=0, scale=None):
     [cu_seqlens[0], cu_seqlens[N]) are padding: their output and gradients are zero and what they hold is not read into
     any other row.  `scale` defaults to 1 / sqrt(D).  Returns o [T, Hq, D] in q's type; differentiable in q, k and v.
 
-    An output row depends on the rows that it sees and on no other, whatever those hold: an infinite or NaN value makes the
-    rows that see it infinite or NaN.  The gradients want finite inputs: their products run over blocks of 128 rows, and a
+    An output row depends on the rows that it sees and on no other, whatever those hold: an infinite or NaN entry of v makes
+    the rows that see it infinite or NaN, and so does a NaN score or one of +inf.  A score of -inf has weight zero; a row whose
+    scores all are -inf is zero, like a row without keys.  The gradients want finite inputs: their products run over blocks of 128 rows, and a
     weight of zero times an infinite or NaN entry is NaN, so such a row reaches the gradients of others in its block."""
     scale = _check_attention(q, k, v, cu_seqlens, "cu_seqlens", 3, scale, window)
     if cu_seqlens.shape[0] < 1:
