@@ -108,10 +108,12 @@ __device__ __forceinline__ Cut cut_row(const T* x, int V) {
 
 // Running maximum m, s = sum of 2^y and e = sum of 2^y y with y = x log2(e) - ref, ref the whole number above m log2(e): the
 // product and the difference are one rounding of a small value, and moving ref scales the sums by an exact power of two.
-// Where |m| is huge (a row of the type's lowest value, infinities) differences are formed first and ref is not used.
+// Where |m| is above 1e9 (rows of a mask's value, infinities) differences are formed first and ref is not used.  Up to there m log2(e)
+// lies within 64 of ref, half of what fp32 values of that size are apart: the maximum's own 2^y is at most 2^65.  Above, distinct
+// values differ by at least 64, so sums relative to a smaller maximum count for nothing and are dropped.
 struct Run {
   float m, ref, s, e;
-  static __device__ __forceinline__ bool plain(float v) { return fabsf(v) < 1e30f; }
+  static __device__ __forceinline__ bool plain(float v) { return fabsf(v) <= 1e9f; }
   __device__ __forceinline__ void raise(float top) {          // `top` > m
     if (plain(m) && plain(top)) {
       const float r = ceilf(top * L2E), k = ref - r, f = ex2(k);
