@@ -23,8 +23,9 @@ NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", 
               "-Xcompiler", "-fPIC", "-Xcompiler", "-O3"]
 # Fast math (approximate exp / division / sqrt, flush-to-zero) is a choice for the bf16 activation kernels,
 # whose results are rounded to 8 mantissa bits anyway.  The optimizer updates fp32 master weights and
-# moments and is compiled with IEEE division and square root.
-PRECISE = {"fused_optim.cu"}
+# moments and is compiled with IEEE division and square root.  Token scores are fp32 results: the logarithm and the
+# divisions that end a row are the accurate ones.
+PRECISE = {"fused_optim.cu", "logprob.cu"}
 
 
 def _nvcc() -> str:

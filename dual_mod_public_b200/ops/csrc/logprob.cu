@@ -189,7 +189,7 @@ struct Run {
   }
   // the sums relative to m itself, e in natural units
   __device__ __forceinline__ void finish() {
-    const float t = plain(m) ? fmaf(m, L2E, -ref) : 0.f, f = ex2(-t);
+    const float t = plain(m) ? fmaf(m, L2E, -ref) : 0.f, f = 1.f / ex2(t);     // the maximum's own term becomes 1
     e = f * LN2 * fmaf(-t, s, e);
     s *= f;
   }
@@ -325,6 +325,10 @@ logprob_fwd_kernel(const T* __restrict__ logits, long long rs, const long long* 
       if (t == 0) sh.n = 0;
       G::sync();
     }
+    // The sum has a term of one and its other terms are positive, those of e negative: roundings do not carry over that, so a log
+    // probability is at most zero and an entropy at least (a NaN stays, and so do the zeros of a row of nothing but -inf).
+    if (r.s < 1.f && r.m > -INFINITY) r.s = 1.f;
+    if (r.e > 0.f) r.e = 0.f;
     const float ls = logf(r.s);
     if (t == 0) {
       logp[row] = target < 0 ? 0.f : target < V ? (xy - r.m) - ls : NAN;
