@@ -17,7 +17,8 @@ expanded dims) are copied first.
 
 Arguments that the host can see are checked and refused with TypeError or ValueError.  Device values are not: `cu_seqlens`
 that do not ascend or lengths outside the cache give wrong outputs but never an access out of range (`lengths` are clamped
-to [0, P]).
+to [0, P]).  Gradients are those of reverse mode, once: an input with a forward-mode tangent is refused with
+NotImplementedError on every device.
 """
 
 from __future__ import annotations
@@ -26,6 +27,7 @@ import math
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import default_ops
@@ -64,6 +66,15 @@ def _check_attention(q, k, v, index, name, kv_dims, scale, window):
     return scale
 
 
+def _check_tangents(name, *tensors):
+    """Refuses dual tensors: the kernels read values only, so a tangent would be lost without a word."""
+    if getattr(forward_ad, "_current_level", 0) < 0:              # no dual level is open
+        return
+    for t in tensors:
+        if forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{name} has no forward-mode derivative")
+
+
 class _PackedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu, window, scale):
@@ -99,6 +110,7 @@ def packed_attention(q, k, v, cu_seqlens, *, window=0, scale=None):
         raise ValueError("cu_seqlens: at least one entry is wanted")
     if q.shape[0] >= (1 << 31) - 256:
         raise ValueError("too many rows")
+    _check_tangents("packed_attention", q, k, v)
     cu_seqlens = cu_seqlens.contiguous()
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _PackedAttention.apply(q, k, v, cu_seqlens, window, scale)
@@ -117,6 +129,7 @@ def cached_attention(q, k_cache, v_cache, lengths, *, window=0, scale=None):
         raise ValueError("lengths: one entry per sequence is wanted")
     if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
         raise ValueError("cached_attention has no gradient: call it under torch.no_grad()")
+    _check_tangents("cached_attention", q, k_cache, v_cache)
     if k_cache.shape[1] >= 1 << 31 or q.shape[0] > 65535 or k_cache.shape[2] > 4095:
         raise ValueError("at most 65535 sequences, 4095 key heads and 2^31 - 1 cache rows are wanted, got "
                          f"{q.shape[0]}, {k_cache.shape[2]}, {k_cache.shape[1]}")
@@ -173,6 +186,7 @@ def token_logprobs(logits, tokens, *, top=0):
         raise ValueError("too many rows or columns")
     if not isinstance(top, int) or not 0 <= top <= min(MAX_TOP, V):
         raise ValueError(f"top: 0 to {min(MAX_TOP, V)} is wanted, got {top!r}")
+    _check_tangents("token_logprobs", logits)
     flat = len(lead) == 1
     x, y = (logits, tokens.contiguous()) if flat else (logits.reshape(-1, V), tokens.reshape(-1).contiguous())
     if logits.requires_grad and torch.is_grad_enabled():
