@@ -37,7 +37,7 @@ import os
 import torch
 import torch.nn.functional as F
 
-from ..ops import token_logprobs
+from ..ops import default_ops, token_logprobs
 from ..utils.checkpoint import load_checkpoint, model_from_checkpoint
 
 try:                                                     # optional dependency
@@ -244,6 +244,7 @@ class DualModEval(_Base):
             logits = self.model(idx, cu_seqlens=edges, logit_rows=rows)[0]
         r = token_logprobs(logits, y, top=1)
         logp, greedy = r.logp.double().tolist(), (r.top_ids[:, 0] == y).tolist()
+        default_ops(y.device).tc_check()
         at = 0
         for i, _, n_c in batch:
             out[i] = (sum(logp[at:at + n_c]), all(greedy[at:at + n_c]))

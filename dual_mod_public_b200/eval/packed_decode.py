@@ -16,7 +16,7 @@ import copy
 
 import torch
 
-from ..ops import cached_attention, packed_attention, token_logprobs
+from ..ops import cached_attention, default_ops, packed_attention, token_logprobs
 
 
 class PackedDecoder:
@@ -123,7 +123,7 @@ class PackedDecoder:
 
     def generate(self, prompts, max_new, eos_id=None, stop_fn=None):
         """Greedy continuations of up to `rows` prompts -> (list of id lists, list of their log probabilities).  A row ends at
-        `eos_id` (not included), when `stop_fn(its ids)` says so, after max_new tokens or when its cache is full."""
+        `eos_id` (not included), when `stop_fn(its ids)` says so, after max_new tokens or when its cache is full.  RuntimeError where a kernel gave up on the way."""
         ids, logp = self.prefill(prompts)
         n = len(prompts)
         out, scores, alive = [[] for _ in prompts], [[] for _ in prompts], [True] * n
@@ -143,4 +143,5 @@ class PackedDecoder:
             nxt = torch.zeros_like(self.tok)
             nxt[:n] = ids[:n]
             ids, logp = self.step(nxt)
+        default_ops(self.dev).tc_check()
         return out, scores

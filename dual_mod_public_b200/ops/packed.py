@@ -17,7 +17,10 @@ expanded dims) are copied first.
 
 Arguments that the host can see are checked and refused with TypeError or ValueError.  Device values are not: `cu_seqlens`
 that do not ascend or lengths outside the cache give wrong outputs but never an access out of range (`lengths` are clamped
-to [0, P]).  Gradients are those of reverse mode, once: an input with a forward-mode tangent is refused with
+to [0, P]).  An attention kernel whose pipeline stands still for two seconds ends with wrong outputs and sets a flag instead of
+holding the device: `default_ops(device).tc_check()` reads it (one value to the host) and raises RuntimeError.  Call it
+before results are used outside of the device; what the framework itself answers or trains with is checked (`PackedDecoder.generate`,
+packed scoring in the evaluation adapter, `train_baseline --packed_docs`).  Gradients are those of reverse mode, once: an input with a forward-mode tangent is refused with
 NotImplementedError on every device.
 """
 

@@ -376,6 +376,9 @@ class TorchOps:
         return fm.ce_chunk(logits, targets, inv_n)
 
     # ---- packed sequences (ops/packed.py) ---------------------------------------------------
+    def tc_check(self):
+        """Raises where a kernel gave up on a pipeline wait since the table was made; torch statements never do."""
+
     def packed_attn_fwd(self, q, k, v, cu, window, scale, need_lse=True, residual=False):
         """Causal attention over packed sequences: (o [T, Hq, D], lse [Hq, T] fp32 or None) and, with `residual`, what
         the rounding of o to its type left, in the same type."""

@@ -36,6 +36,7 @@ from ..data.packed import SyntheticStream, memmap_stream
 from ..engines.schedule import cosine_lr
 from ..models import DualModLM
 from ..models import baselines as B
+from ..ops import default_ops
 from ..parallel.fused_optim import decay_groups
 from ..utils.checkpoint import save_atomic
 from .governors import MetricsLogger, SkipRule
@@ -158,6 +159,8 @@ def main(argv=None):
                 loss.backward()
             loss_acc += loss.item()
         gn = torch.nn.utils.clip_grad_norm_(params, 1.0).item()
+        if args.packed_docs:
+            default_ops(dev).tc_check()                  # before gradients of a kernel that gave up reach the weights
         skipped = skip.decide(gn, loss_acc, False)
         if not skipped:
             opt.step()
