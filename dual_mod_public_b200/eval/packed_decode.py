@@ -123,7 +123,8 @@ class PackedDecoder:
 
     def generate(self, prompts, max_new, eos_id=None, stop_fn=None):
         """Greedy continuations of up to `rows` prompts -> (list of id lists, list of their log probabilities).  A row ends at
-        `eos_id` (not included), when `stop_fn(its ids)` says so, after max_new tokens or when its cache is full.  RuntimeError where a kernel gave up on the way."""
+        `eos_id` (not included), when `stop_fn(its ids)` says so, after max_new tokens or when its cache is full.
+        RuntimeError where a kernel gave up on the way."""
         ids, logp = self.prefill(prompts)
         n = len(prompts)
         out, scores, alive = [[] for _ in prompts], [[] for _ in prompts], [True] * n
