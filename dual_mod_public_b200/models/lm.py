@@ -77,7 +77,8 @@ class DualModLM(nn.Module):
 
         `cu_seqlens` (attn_mode "vanilla"): idx / targets are [T] (or [1,T]), sequences of any lengths packed one behind
         the other, sequence s being the rows [cu_seqlens[s], cu_seqlens[s+1]); no row sees another sequence and positions
-        restart with each.  Returns logits [T,V] (of the rows `logit_rows` only, where given: int64 [n], targets [n])."""
+        restart with each.  Returns logits [T,V] (of the rows `logit_rows` only, where given: int64 [n], targets [n]).
+        The loss is the mean over targets >= 0; zero, with zero gradients, where there is none."""
         if cu_seqlens is not None:
             return self._forward_packed(idx, targets, inputs_embeds, cu_seqlens, logit_rows)
         x = self.tok_emb(idx) if inputs_embeds is None else inputs_embeds
@@ -124,7 +125,7 @@ class DualModLM(nn.Module):
         loss = None
         if targets is not None:
             targets = targets.reshape(-1)
-            loss = -token_logprobs(logits, targets).logp.sum() / (targets >= 0).sum()
+            loss = -token_logprobs(logits, targets).logp.sum() / (targets >= 0).sum().clamp_min(1)
         return logits, loss
 
     # ---- incremental decode ----------------------------------------------------------

@@ -8,8 +8,8 @@
   --arch gdn       gated delta-rule network (`models.baselines.build_gdn`)
   --arch fbt | looped | rdepth | lstm   the small-scale baselines of the formal-language harness
 
-  --packed_docs --eos_id 2   (vanilla, ematch) rows are streams of documents that end with that token: attention and positions
-                   stay inside a document (`ops.packed_attention`, loss by `ops.token_logprobs`)
+  --packed_docs --eos_id 2   (vanilla, ematch) rows are streams of documents that end with that token: attention, positions and
+                   targets stay inside a document (`ops.packed_attention`, loss by `ops.token_logprobs`)
 
 Same AdamW(0.9, 0.95), weight decay on matrices only, warm-up + cosine, clip 1.0, EMA outlier batch skip
 with non-finite always skipped (`governors.SkipRule`), as the Dual-Mod arm.  Micro-batch accumulation
@@ -71,6 +71,11 @@ def document_edges(x, eos_id):
     ends[:, -1] = True
     last = ends.reshape(-1).nonzero().squeeze(-1) + 1
     return torch.cat((last.new_zeros(1), last)).to(torch.int32)
+
+
+def document_targets(x, y, eos_id):
+    """Targets y [B, T] of rows x without those that would ask a document for the first token of the next (-1: no target)."""
+    return torch.where(x == eos_id, -1, y)
 
 
 def logits_of(model, x):
@@ -151,6 +156,7 @@ def main(argv=None):
             with hold:
                 with torch.autocast(dev.type, dtype=torch.bfloat16, enabled=cuda):
                     if args.packed_docs:
+                        y = document_targets(x, y, args.eos_id)
                         loss = net(x.reshape(-1), targets=y.reshape(-1), cu_seqlens=document_edges(x, args.eos_id))[1] / accum
                     else:
                         lg = logits_of(net, x)
