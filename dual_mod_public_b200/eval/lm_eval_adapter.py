@@ -238,8 +238,8 @@ class DualModEval(_Base):
             where += range(end - n_c - 1, end - 1)               # the row before a token predicts it
             targets += toks[len(toks) - n_c:]
             edges.append(end)
-        idx = torch.tensor([t for _, toks, _ in batch for t in toks], device=self.dev)
-        rows, y = torch.tensor(where, device=self.dev, dtype=torch.long), torch.tensor(targets, device=self.dev, dtype=torch.long)
+        idx, rows, y = (torch.tensor(ids, device=self.dev, dtype=torch.long)
+                        for ids in ([t for _, toks, _ in batch for t in toks], where, targets))
         with self._amp():
             logits = self.model(idx, cu_seqlens=edges, logit_rows=rows)[0]
         r = token_logprobs(logits, y, top=1)
@@ -247,7 +247,7 @@ class DualModEval(_Base):
         default_ops(y.device).tc_check()
         at = 0
         for i, _, n_c in batch:
-            out[i] = (sum(logp[at:at + n_c]), all(greedy[at:at + n_c]))
+            out[i] = (sum(logp[at:at + n_c], 0.0), all(greedy[at:at + n_c]))
             at += n_c
 
     def loglikelihood(self, requests):

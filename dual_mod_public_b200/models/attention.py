@@ -303,7 +303,7 @@ class DualModAttention(nn.Module):
 
     def _packed_qkv(self, xhat, cos, sin):
         """x̂ [T,d], the angles of every row [T, dh/2] -> rotated q [T,h,dh], rotated k and v [T,h_kv,dh]."""
-        heads = lambda x: x.view(x.shape[0], -1, self.head_dim)
+        heads = lambda x: x.view(x.shape[0], x.shape[1] // self.head_dim, self.head_dim)
         c, s = cos[:, None], sin[:, None]
         return apply_rope(heads(self.wq(xhat)), c, s), apply_rope(heads(self.wk(xhat)), c, s), heads(self.project_v(xhat))
 
