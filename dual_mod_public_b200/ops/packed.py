@@ -38,6 +38,7 @@ from . import default_ops
 MAX_TOP = 32
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 _T = torch.Tensor
+_SCALES = 2.0 ** -126, 2.0 ** 127     # the kernels hold scale log2(e) in fp32: as zero it would turn a hidden key's -inf into NaN
 
 
 def _check_attention(q, k, v, index, name, kv_dims, scale, window):
@@ -64,8 +65,8 @@ def _check_attention(q, k, v, index, name, kv_dims, scale, window):
     if scale is None:
         return 1.0 / math.sqrt(D)
     scale = float(scale)
-    if not 0 < scale < math.inf:
-        raise ValueError(f"scale has to be positive and finite, got {scale}")
+    if not _SCALES[0] <= scale <= _SCALES[1]:
+        raise ValueError(f"scale has to be positive and a normal fp32 number, 2^-126 to 2^127, got {scale}")
     return scale
 
 
@@ -102,7 +103,8 @@ def packed_attention(q, k, v, cu_seqlens, *, window=0, scale=None):
     cu_seqlens int32 [N + 1], ascending: sequence s is the rows [cu_seqlens[s], cu_seqlens[s + 1]) and may be empty.  A row
     sees the rows of its own sequence up to itself, the last `window` of them when window > 0.  Rows outside
     [cu_seqlens[0], cu_seqlens[N]) are padding: their output and gradients are zero and what they hold is not read into
-    any other row.  `scale` defaults to 1 / sqrt(D).  Returns o [T, Hq, D] in q's type; differentiable in q, k and v.
+    any other row.  `scale` defaults to 1 / sqrt(D); 2^-126 to 2^127 are taken.  Returns o [T, Hq, D] in q's type;
+    differentiable in q, k and v.
 
     An output row depends on the rows that it sees and on no other, whatever those hold: an infinite or NaN entry of v makes
     the rows that see it infinite or NaN, and so does a NaN score or one of +inf.  A score of -inf has weight zero; a row whose
