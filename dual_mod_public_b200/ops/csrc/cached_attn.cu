@@ -143,14 +143,14 @@ __global__ void __launch_bounds__(WARPS * 32) cached_kernel(const T* __restrict_
           if (left < KEYS && 8 * n + (lane & 3) * 2 + i >= left) x[n][2 * r + i] = -INFINITY;
           top = fmaxf(top, x[n][2 * r + i]);
         }
-      top = quad_max(top) * g.scale_log2;
-      const float mn = fmaxf(m[r], top), sub = mn == -INFINITY ? 0.f : mn;
-      const float f = exp2f(m[r] - sub);
+      // m is a score, and differences of scores are formed before the factor: exact next to the maximum however large it is
+      const float mn = fmaxf(m[r], quad_max(top)), sub = mn == -INFINITY ? 0.f : mn;
+      const float f = exp2f((m[r] - sub) * g.scale_log2);
       m[r] = mn;
       float sum = 0.f;
 #pragma unroll
       for (int n = 0; n < KEYS / 8; ++n) {
-        const float p0 = exp2f(fmaf(x[n][2 * r], g.scale_log2, -sub)), p1 = exp2f(fmaf(x[n][2 * r + 1], g.scale_log2, -sub));
+        const float p0 = exp2f((x[n][2 * r] - sub) * g.scale_log2), p1 = exp2f((x[n][2 * r + 1] - sub) * g.scale_log2);
         sum += p0 + p1;
         pa[n >> 1][r + 2 * (n & 1)] = E::pack(p0, p1);
       }
@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(WARPS * 32) cached_kernel(const T* __restrict_
     float2 a = make_float2(0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
-      const float f = exp2f(sm[w][r] - sub);
+      const float f = exp2f((sm[w][r] - sub) * g.scale_log2);
       const float2 u = *reinterpret_cast<const float2*>(so + (w * ROWS + r) * DH + d);
       sum = fmaf(f, sl[w][r], sum);
       a.x = fmaf(f, u.x, a.x);
@@ -238,7 +238,7 @@ __global__ void __launch_bounds__(WARPS * 32) cached_kernel(const T* __restrict_
 #pragma unroll
     for (int w = 0; w < MAX_CLUSTER; ++w)
       if (w < blocks) {
-        const float f = exp2f(mb[w] - sub);
+        const float f = exp2f((mb[w] - sub) * g.scale_log2);
         const float2 u = ld_cluster2(tc05::map_to_cta(so_a + 4 * (r * DH + d), w));
         sum = fmaf(f, ld_cluster(tc05::map_to_cta(bl_a + 4 * r, w)), sum);
         a0 = fmaf(f, u.x, a0);

@@ -33,6 +33,9 @@ using namespace packed;
 namespace {
 
 constexpr float LAG = 8.f;              // octaves
+// Exponents are one FMA, the score in octaves minus the rounded maximum.  Up to 2^24 octaves that rounding is at most one octave
+// and common to the row; beyond, the weights may leave the range of fp16 or fp32, and the row is computed again.
+constexpr float FAR = 16777216.f;
 
 template <int DH>
 struct Cfg {
@@ -96,25 +99,26 @@ __device__ __forceinline__ void store16(T* row, int d0, int D, const uint32_t (&
   }
 }
 
-// One output row from the keys that it sees; a whole warp: a lane scores one of 32 keys, then holds every 32nd dim.  lse2: log2 of
-// the row's sum.
+// One output row from the keys that it sees, at least one with a score above -inf; a whole warp: a lane scores one of 32 keys, then
+// holds every 32nd dim.  Maximum and sum are its own: fp32 sums of another order than the tensor pipe's.
 // The products run over blocks of 128 keys, where a weight of zero times an infinite or NaN value is NaN, so a row that does
-// not see that value would get it all the same.  Rows whose scores are finite and whose outputs are not therefore end here
-// (with an infinite value in every row of one sequence of 16384, 16 heads of 64: 271 ms),
+// not see that value would get it all the same.  Rows whose scores are finite and whose outputs are not therefore end here,
+// and rows of finite scores whose maximum is beyond FAR (every row of one sequence of 16384, 16 heads of 64: 275 ms),
 // which costs the others up to 1 % (8192 mixed rows, 16 query and 4 key heads of 128: 78.4 against 79.6 us), and the smallest
 // launches up to a microsecond of instruction fetches (731 rows, 16 heads of 64: 8.4 us with and without on some devices, 8.4
 // against 9.5 on others).
 template <typename T>
-__device__ __forceinline__ void redo_row(const Geo& g, T* out, T* out_lo, int h, int row, int lo, float lse2) {
+__device__ __forceinline__ void redo_row(const Geo& g, T* out, T* out_lo, float* lse, int h, int row, int lo) {
   const int lane = threadIdx.x & 31;
   const T* q = (const T*)g.q.p + row * g.q.rs + h * g.q.hs;
   const T* k = (const T*)g.k.p + h / g.group * g.k.hs;
   const T* v = (const T*)g.v.p + h / g.group * g.v.hs;
-  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  float acc[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
 #pragma unroll 1
   for (long long j0 = lo; j0 <= row; j0 += 32) {
-    float s = 0.f;
+    float s = -INFINITY;
     if (j0 + lane <= row) {
+      s = 0.f;
 #pragma unroll 2
       for (int d = 0; d < g.D; d += 8) {
         const uint4 a = *reinterpret_cast<const uint4*>(q + d), b = *reinterpret_cast<const uint4*>(k + (j0 + lane) * g.k.rs + d);
@@ -127,7 +131,18 @@ __device__ __forceinline__ void redo_row(const Geo& g, T* out, T* out_lo, int h,
         }
       }
     }
-    const float w = ex2(fmaf(s, g.scale_log2, -lse2));
+    float top = s;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (top > m) {
+      const float f = ex2((m - top) * g.scale_log2);
+      m = top;
+      l *= f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] *= f;
+    }
+    const float w = m == -INFINITY ? 0.f : ex2((s - m) * g.scale_log2);
+    l += w;
     const int n = (int)min(32LL, row + 1 - j0);
 #pragma unroll 4
     for (int u = 0; u < n; ++u) {
@@ -138,12 +153,17 @@ __device__ __forceinline__ void redo_row(const Geo& g, T* out, T* out_lo, int h,
     }
   }
 #pragma unroll
+  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  if (lse && lane == 0) lse[(long long)h * g.T + row] = fmaf(m, g.scale_log2, log2f(l)) * (1.f / LOG2E);
+  l = 1.f / l;
+#pragma unroll
   for (int i = 0; i < 4; ++i) {
     if (lane + 32 * i >= g.D) break;
     const long long at = ((long long)row * g.Hq + h) * g.D + lane + 32 * i;
-    const T o = (T)acc[i];
+    const float f = acc[i] * l;
+    const T o = (T)f;
     out[at] = o;
-    if (out_lo) out_lo[at] = (T)(acc[i] - (float)o);
+    if (out_lo) out_lo[at] = (T)(f - (float)o);
   }
 }
 
@@ -352,7 +372,7 @@ __global__ void __launch_bounds__(Cfg<DH>::NT, 3 - Cfg<DH>::TILES) packed_fwd_ke
         wait(pvdone(a), (n - 1) & 1, serr);                          // n > 0: some row has an m
         tc_fence_after();
         const float f = grow ? ex2(m - m_new) : 1.f;                 // m = -inf: 0, and O is still zero
-        l *= f;
+        l = f == 0.f && l == INFINITY ? 0.f : l * f;                 // infinite: weights of a maximum far below (see FAR)
 #pragma unroll
         for (int c = 0; c < DH / 32; ++c) {
           uint32_t o[32];
@@ -431,12 +451,13 @@ __global__ void __launch_bounds__(Cfg<DH>::NT, 3 - Cfg<DH>::TILES) packed_fwd_ke
     }
     const float lse2 = inv == 0.f ? -INFINITY : m + log2f(l);
     if (lse && row < g.T) lse[(long long)h * g.T + row] = lse2 * (1.f / LOG2E);
-    const bool again = (bad[0] + bad[1]) + (bad[2] + bad[3]) != 0.f && fabsf(lse2) < INFINITY;
+    // outputs that are not finite though the scores are: a value that the row does not see, or weights of a maximum far below
+    const bool again = row < g.T && fabsf(m) < INFINITY && l == l && ((bad[0] + bad[1]) + (bad[2] + bad[3]) != 0.f || fabsf(m) > FAR);
     unsigned todo = __ballot_sync(0xffffffffu, again);
     for (; __builtin_expect(todo != 0, 0); todo &= todo - 1) {
       const int who = __ffs(todo) - 1;
       __syncwarp();                                                  // after the lane's own stores
-      redo_row<T>(g, out, out_lo, h, w_row + who, __shfl_sync(0xffffffffu, lo, who), __shfl_sync(0xffffffffu, lse2, who));
+      redo_row<T>(g, out, out_lo, lse, h, w_row + who, __shfl_sync(0xffffffffu, lo, who));
     }
   }
   tc_fence_before();
