@@ -13,6 +13,7 @@ using namespace tc05;
 
 constexpr int TILE = 128;               // rows of a query tile and of a key block
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr float FAR = 16777216.f;       // octaves: fp32 holds a row's maximum or log sum to within one up to here
 
 // ---- sequences -------------------------------------------------------------------------------------------------------
 // `cu` holds n + 1 ascending row numbers; sequence s is the rows [cu[s], cu[s + 1]).  A row outside [cu[0], cu[n]) belongs

@@ -29,7 +29,8 @@
 // A first small kernel forms delta from o and the rest that its rounding left: where a row sees few keys ds is a small difference
 // of dp and delta (zero for a row that sees itself alone), and the rounding of o alone would be most of the gradients' error (up
 // to 3.9e-3 of dq's norm over documents of some ten tokens, 2.6e-3 with the rest).  It leaves -delta and -lse in base 2 (-inf for
-// rows without keys and for the padding of the last tile, which makes their weights zero).
+// rows without keys and for the padding of the last tile, which makes their weights zero; NaN where fp32 does not hold lse to
+// within an octave, as weights would be off by that: the gradients of such a row and of the keys that it sees are NaN).
 #include "packed.cuh"
 
 using namespace packed;
@@ -80,7 +81,8 @@ __global__ void __launch_bounds__(256) packed_delta_kernel(const bf16* __restric
     for (int i = LANES / 2; i > 0; i >>= 1) s += __shfl_xor_sync(0xffffffffu, s, i);
     if (sub == 0) {
       const long long at = (long long)h * Tp + row0 + k * GROUPS;
-      aux[at] = L[k] == -INFINITY ? -INFINITY : -L[k] * LOG2E;
+      const float n = -L[k] * LOG2E;
+      aux[at] = n == INFINITY ? -INFINITY : fabsf(n) <= FAR ? n : NAN;
       aux[(long long)Hq * Tp + at] = -s;
     }
   }

@@ -34,8 +34,7 @@ namespace {
 
 constexpr float LAG = 8.f;              // octaves
 // Exponents are one FMA, the score in octaves minus the rounded maximum.  Up to 2^24 octaves that rounding is at most one octave
-// and common to the row; beyond, the weights may leave the range of fp16 or fp32, and the row is computed again.
-constexpr float FAR = 16777216.f;
+// and common to the row; beyond (FAR), the weights may leave the range of fp16 or fp32, and the row is computed again.
 
 template <int DH>
 struct Cfg {

@@ -4,9 +4,12 @@ value is read back to the host, so the statements can be captured like the kerne
 
 from __future__ import annotations
 
+import math
+
 import torch
 
 ROWS = 1024                       # query rows per slab: bounds the scores held at a time
+FAR = 2.0 ** 24 * math.log(2.0)   # fp32 holds a log sum to within an octave up to here; beyond it gives no weights back
 
 
 def _bounds(cu, T, window):
@@ -83,6 +86,7 @@ def packed_attn_bwd(do, q, k, v, o, lse, cu, window, scale, o_lo=None):
     for rows, s, hidden in _slabs(q, k, cu, window, scale):
         n, keys = rows.stop - rows.start, rows.stop
         L = lse[:, rows].view(Hkv, Hq // Hkv, n, 1)
+        L = torch.where((L.abs() <= FAR) | (L == float("-inf")), L, float("nan"))
         p = (s - L.masked_fill(L == float("-inf"), 0.0)).exp().masked_fill(hidden, 0.0)
         dof, of, qf = split(do[rows]), split(o[rows]), split(q[rows])
         dp = dof @ v[:keys].float().permute(1, 2, 0)[:, None]

@@ -1,5 +1,5 @@
 """Scores far from zero: finite ones of up to 2^120 give the softmax that they have.  They are exact here, so the bound is that of
-the rounded weights and outputs alone."""
+the rounded weights and outputs alone.  Gradients are NaN where fp32 does not hold a row's log sum to within an octave."""
 
 import math
 
@@ -56,3 +56,29 @@ def test_forward(dev, dtype, dim, signs, log_size):
     wild = packed_attention(q, k, v, cu, scale=scale)
     assert not wild[300:, :, 3].isfinite().any()
     ref.close(wild[:300], (o[:300], bound[:300]), "behind a non-finite value")
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("log_size", [25, 40])
+def test_gradients_beyond_fp32_are_nan(dev, dim, dtype, log_size):
+    """Of the sequence with such scores; the other one, in the same blocks of rows, has its gradients."""
+    q, k, v = inputs(dev, dtype, dim, (1,))
+    n = 190
+    g = torch.Generator().manual_seed(2)
+    scale = 2.0 ** (log_size - 30)
+    unit = 1 / math.sqrt(scale * math.sqrt(dim))
+    if dtype is torch.float16 and log_size == 40:
+        unit = 2.0 ** -8
+    for x, h in ((q, 2), (k, 1)):
+        x[:n] = (torch.randn(n, h, dim, generator=g) * unit).to(dev, dtype)
+    do = torch.randn(T, 2, dim, generator=g).to(dev, dtype)
+    cu = torch.tensor([0, n, T], dtype=torch.int32, device=dev)
+    leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+    grads = torch.autograd.grad(packed_attention(*leaves, cu, scale=scale), leaves, do)
+    alone = ref.packed(q[:n], k[:n], v[:n], cu[:2], scale=scale, do=do[:n])
+    for got, name in zip(grads, ("dq", "dk", "dv")):
+        assert got[n:].isnan().all(), name
+        assert got[:n].isfinite().all(), name
+        ref.close(got[:n], alone[name], name)
