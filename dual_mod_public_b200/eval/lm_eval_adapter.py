@@ -327,16 +327,25 @@ class DualModEval(_Base):
                 logits = self.model.decode_step(nxt[:, None], plen + j, caches)
         return [self._cut(t, stop_strs) for t in toks]
 
-    def _greedy_packed(self, prompts, max_new, stop_strs):
+    def _packed_decoder(self, rows, P):
+        """The decoder for `rows` prompts in caches of P entries.  One is resident at a time: another shape takes over the
+        weights (a copy in the compute type, where the model has another one) once the caches and the graph of the last are gone."""
         from .packed_decode import PackedDecoder
-        rows = max(self.gen_rows, len(prompts))
+        dec = self._engines.pop("packed", None)
+        if dec is None or (dec.rows, dec.P) != (rows, P):
+            weights = self.model if dec is None else dec.m
+            dec = None
+            dec = PackedDecoder(weights, rows, P)
+            if torch.device(self.dev).type == "cuda":
+                dec.capture()
+        self._engines["packed"] = dec
+        return dec
+
+    def _greedy_packed(self, prompts, max_new, stop_strs):
         P = min(-(-(max(map(len, prompts)) + max_new) // 256) * 256, self.model.cfg.max_seq_len)
-        key = ("packed", rows, P)
-        if key not in self._engines:
-            dec = PackedDecoder(self.model, rows, P)
-            self._engines[key] = dec.capture() if torch.device(self.dev).type == "cuda" else dec
         stop = (lambda ids: any(s in self.tok.decode(ids) for s in stop_strs)) if stop_strs else None
-        ids, _ = self._engines[key].generate(prompts, max_new, eos_id=self.tok.eos_token_id, stop_fn=stop)
+        dec = self._packed_decoder(max(self.gen_rows, len(prompts)), P)
+        ids, _ = dec.generate(prompts, max_new, eos_id=self.tok.eos_token_id, stop_fn=stop)
         return [self._cut(t, stop_strs) for t in ids]
 
     def _greedy(self, prompt_ids, max_new, stop_strs):
@@ -366,6 +375,8 @@ class DualModEval(_Base):
                 ids = trunc_keep_head([self.bos] + self.tok_encode(prompt), max(1, self.max_length - max_new))
                 groups[(0 if self.packed else len(ids), until, max_new)].append((i, key, ids))
         for (_, until, max_new), items in sorted(groups.items(), key=lambda kv: kv[0][0]):
+            if self.packed:
+                items.sort(key=lambda it: len(it[2]))            # rows of one batch share a cache length
             for b0 in range(0, len(items), self.gen_rows):
                 part = items[b0:b0 + self.gen_rows]
                 texts = self._greedy_batch([ids for _, _, ids in part], max_new, list(until))
