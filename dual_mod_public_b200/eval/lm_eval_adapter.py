@@ -338,6 +338,7 @@ class DualModEval(_Base):
             dec = PackedDecoder(weights, rows, P)
             if torch.device(self.dev).type == "cuda":
                 dec.capture()
+        dec.refresh(self.model)                                  # it may have been trained on
         self._engines["packed"] = dec
         return dec
 

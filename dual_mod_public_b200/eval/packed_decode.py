@@ -7,7 +7,7 @@ The prompts are packed one behind the other and run through the layers in ONE pa
 values are written to the rows' caches, and every further token is a step over the whole batch in which each row has a
 position and a live length of its own (`ops.cached_attention`); the next token and its log probability come from
 `ops.token_logprobs`.  Grouped KV heads, sliding windows and the log-n scale work as in training.  `capture()` records the
-step as one CUDA graph.  (`eval.graph_decode.GraphDecoder` is the decoder for batches that share one position, and for the
+step as one CUDA graph.  Weights of another type than `dtype` are copied once; `refresh(model)` copies them again.  (`eval.graph_decode.GraphDecoder` is the decoder for batches that share one position, and for the
 Dual-Mod write law.)"""
 
 from __future__ import annotations
@@ -43,6 +43,15 @@ class PackedDecoder:
         self.tok = torch.zeros(rows, dtype=torch.long, device=self.dev)
         self.no_target = torch.full((rows,), -1, dtype=torch.long, device=self.dev)
         self.graph = None
+
+    @torch.no_grad()
+    def refresh(self, model):
+        """Takes over the weights of `model`, which this decoder was made from, where it decodes from a copy of them (in place: a
+        recorded step sees them)."""
+        if model is not self.m:
+            for mine, theirs in ((self.m.parameters(), model.parameters()), (self.m.buffers(), model.buffers())):
+                for a, b in zip(mine, theirs):
+                    a.copy_(b)
 
     def _pick(self, logits):
         r = token_logprobs(logits, self.no_target[:logits.shape[0]], top=1)

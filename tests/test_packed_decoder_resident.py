@@ -17,7 +17,7 @@ DEVICES = ["cpu", pytest.param("cuda:0", marks=pytest.mark.gpu)]
 @pytest.mark.parametrize("dev", DEVICES)
 def test_one_decoder_at_a_time(dev, monkeypatch):
     torch.manual_seed(0)
-    m = DualModLM(DualModConfig(d_model=64, n_layers=1, n_heads=2, mlp_hidden_override=64, vocab_size=300, max_seq_len=1024,
+    m = DualModLM(DualModConfig(d_model=64, n_layers=1, n_heads=2, mlp_hidden_override=64, vocab_size=259, max_seq_len=1024,
                                 attn_mode="vanilla", dtype="fp32"))
     made, weights, most = [], set(), [0]
     inner = packed_decode.PackedDecoder.__init__
