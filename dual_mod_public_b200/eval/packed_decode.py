@@ -104,21 +104,23 @@ class PackedDecoder:
         return self._pick(logits)
 
     def capture(self):
-        """Records the step as a CUDA graph (caches and lengths keep their contents); returns self."""
-        keep = self.lengths.clone()
-        side = torch.cuda.Stream(self.dev)
-        side.wait_stream(torch.cuda.current_stream(self.dev))
-        with torch.cuda.stream(side):
-            held = [(K[:, -1].clone(), V[:, -1].clone()) for K, V in zip(self.K, self.V)]
-            self.lengths.fill_(self.P - 1)               # the warm-up writes the caches' last rows only
-            self._step()
-            for (k, v), K, V in zip(held, self.K, self.V):
-                K[:, -1], V[:, -1] = k, v
-            self.lengths.copy_(keep)
-        torch.cuda.current_stream(self.dev).wait_stream(side)
-        graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(graph):
-            self.out = self._step()
+        """Records the step as a CUDA graph, on this decoder's device whichever is current (caches and lengths keep their
+        contents); returns self."""
+        with torch.cuda.device(self.dev):
+            keep = self.lengths.clone()
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                held = [(K[:, -1].clone(), V[:, -1].clone()) for K, V in zip(self.K, self.V)]
+                self.lengths.fill_(self.P - 1)           # the warm-up writes the caches' last rows only
+                self._step()
+                for (k, v), K, V in zip(held, self.K, self.V):
+                    K[:, -1], V[:, -1] = k, v
+                self.lengths.copy_(keep)
+            torch.cuda.current_stream().wait_stream(side)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):   # the stream that torch records on by default is of one device for good
+                self.out = self._step()
         self.graph = graph
         return self
 
