@@ -132,14 +132,15 @@ def cached_attention(q, k_cache, v_cache, lengths, *, window=0, scale=None):
     never read, whatever they hold.  A length of zero gives zeros.  Returns o [B, Hq, D].  Not differentiable: a tensor
     that requires a gradient is refused while gradients are enabled."""
     scale = _check_attention(q, k_cache, v_cache, lengths, "lengths", 4, scale, window)
-    if lengths.shape[0] != q.shape[0]:
+    (B, Hq, _), (_, P, Hkv, _) = q.shape, k_cache.shape
+    if lengths.shape[0] != B:
         raise ValueError("lengths: one entry per sequence is wanted")
     if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
         raise ValueError("cached_attention has no gradient: call it under torch.no_grad()")
     _check_tangents("cached_attention", q, k_cache, v_cache)
-    if k_cache.shape[1] >= 1 << 31 or q.shape[0] > 65535 or k_cache.shape[2] > 4095:
-        raise ValueError("at most 65535 sequences, 4095 key heads and 2^31 - 1 cache rows are wanted, got "
-                         f"{q.shape[0]}, {k_cache.shape[2]}, {k_cache.shape[1]}")
+    if P >= 1 << 31 or B > 65535 or Hkv > 4095 or (Hq > 65535 and Hkv * -(-Hq // (16 * Hkv)) > 65535):
+        raise ValueError("at most 65535 sequences, 4095 key heads, 65535 groups of up to 16 query heads of one key head and 2^31 - 1 "
+                         f"cache rows are wanted, got {B}, {Hkv}, {Hq} query heads and {P}")
     return default_ops(q.device).cached_attn(q, k_cache, v_cache, lengths.contiguous(), window, scale)
 
 
