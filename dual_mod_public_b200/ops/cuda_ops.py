@@ -114,11 +114,36 @@ def _dense_tail(t: torch.Tensor, n_tail: int) -> bool:
     return True
 
 
-try:                                                     # half of torch.empty's time per call
-    from torch._C._dynamo.guards import _empty_strided_cuda
-except ImportError:
-    def _empty_strided_cuda(size, stride, dtype):
-        return torch.empty_strided(size, stride, dtype=dtype, device="cuda")
+def _public_empty(dtype, *size):
+    """Contiguous and uninitialised, on the current device."""
+    return torch.empty(size, dtype=dtype, device="cuda")
+
+
+def _choose_empty():
+    """`_public_empty`, or the same in 0.8 us of host time instead of 2.4 by an entry of torch that is not public: where that exists
+    and gives what is asked for, and only while no dispatch mode is active, as it does not pass the dispatcher, where such modes
+    (memory and operation counters) would see the allocation."""
+    try:
+        from torch._C import _len_torch_dispatch_stack as modes
+        from torch._C._dynamo.guards import _empty_strided_cuda as fast
+        t = fast((2, 3), (3, 1), torch.bfloat16)
+        if modes() < 0 or (t.shape, t.stride(), t.dtype, t.is_cuda) != ((2, 3), (3, 1), torch.bfloat16, True):
+            return _public_empty
+    except Exception:                                    # whatever another version of torch answers
+        return _public_empty
+
+    def empty(dtype, *size):
+        if modes():
+            return _public_empty(dtype, *size)
+        stride, n = [], 1
+        for k in reversed(size):
+            stride.append(n)
+            n *= k if k > 1 else 1
+        return fast(size, tuple(stride[::-1]), dtype)
+    return empty
+
+
+_empty = None                                            # chosen when the first table is made
 
 
 def _raw_stream(index):
@@ -142,15 +167,6 @@ def _here(method):
     return call
 
 
-def _empty(dtype, *size):
-    """Contiguous and uninitialised, on the current device."""
-    stride, n = [], 1
-    for k in reversed(size):
-        stride.append(n)
-        n *= k if k > 1 else 1
-    return _empty_strided_cuda(size, tuple(stride[::-1]), dtype)
-
-
 class CudaOps(TorchOps):
     name = "sm100a"
 
@@ -165,6 +181,8 @@ class CudaOps(TorchOps):
         self.strict = os.environ.get("DMB_STRICT_OPS", "0") == "1"
         self._tc_err = torch.zeros(1, dtype=torch.int32, device=self.device)   # raised by the tcgen05 attention kernels
         self._tc_err_ptr = self._tc_err.data_ptr()
+        global _empty
+        _empty = _empty or _choose_empty()
         if os.environ.get("DMB_GEMM", "tcgen05") == "tcgen05":
             from .gemm import Tcgen05Gemm
             self.gemm = Tcgen05Gemm(self.lib, self.device)
