@@ -71,9 +71,8 @@ def _check_attention(q, k, v, index, name, kv_dims, scale, window):
 
 
 def _check_tangents(name, *tensors):
-    """Refuses dual tensors: the kernels read values only, so a tangent would be lost without a word."""
-    if getattr(forward_ad, "_current_level", 0) < 0:              # no dual level is open
-        return
+    """Refuses dual tensors: the kernels read values only, so a tangent would be lost without a word.  Callers look for an open
+    dual level first, which is all that a call outside of one pays for."""
     for t in tensors:
         if forward_ad.unpack_dual(t).tangent is not None:
             raise NotImplementedError(f"{name} has no forward-mode derivative")
@@ -117,7 +116,8 @@ def packed_attention(q, k, v, cu_seqlens, *, window=0, scale=None):
         raise ValueError("cu_seqlens: at least one entry is wanted")
     if q.shape[0] >= (1 << 31) - 256:
         raise ValueError("too many rows")
-    _check_tangents("packed_attention", q, k, v)
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        _check_tangents("packed_attention", q, k, v)
     cu_seqlens = cu_seqlens.contiguous()
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _PackedAttention.apply(q, k, v, cu_seqlens, window, scale)
@@ -137,7 +137,8 @@ def cached_attention(q, k_cache, v_cache, lengths, *, window=0, scale=None):
         raise ValueError("lengths: one entry per sequence is wanted")
     if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
         raise ValueError("cached_attention has no gradient: call it under torch.no_grad()")
-    _check_tangents("cached_attention", q, k_cache, v_cache)
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        _check_tangents("cached_attention", q, k_cache, v_cache)
     if P >= 1 << 31 or B > 65535 or Hkv > 4095 or (Hq > 65535 and Hkv * -(-Hq // (16 * Hkv)) > 65535):
         raise ValueError("at most 65535 sequences, 4095 key heads, 65535 groups of up to 16 query heads of one key head and 2^31 - 1 "
                          f"cache rows are wanted, got {B}, {Hkv}, {Hq} query heads and {P}")
@@ -194,7 +195,8 @@ def token_logprobs(logits, tokens, *, top=0):
         raise ValueError("too many rows or columns")
     if not isinstance(top, int) or not 0 <= top <= min(MAX_TOP, V):
         raise ValueError(f"top: 0 to {min(MAX_TOP, V)} is wanted, got {top!r}")
-    _check_tangents("token_logprobs", logits)
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        _check_tangents("token_logprobs", logits)
     flat = len(lead) == 1
     x, y = (logits, tokens.contiguous()) if flat else (logits.reshape(-1, V), tokens.reshape(-1).contiguous())
     if logits.requires_grad and torch.is_grad_enabled():
