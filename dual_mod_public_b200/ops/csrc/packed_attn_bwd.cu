@@ -354,11 +354,6 @@ __device__ __forceinline__ void keys_and_values(const CUtensorMap& tmQ, const CU
       scores(0, ahead0);
       ahead0 = next(ahead0);
       if (C::SETS > 1 && steps > 1) { scores(1, ahead0); ahead0 = next(ahead0); }
-      auto gradient_tile = [&](int i) {
-        wait(gfull(i), gphase(i), serr);
-        clean(C::b_off + (i % C::NB) * C::TB, q0);
-        q0 = next(q0);
-      };
       auto begin_step = [&](int i) {                     // P -> dV, and dP in its place behind it
         wait(gfull(i), gphase(i), serr);
         clean(C::b_off + (i % C::NB) * C::TB, q0);
