@@ -495,7 +495,9 @@ __global__ void __launch_bounds__(Group<NT>::BLOCK) logprob_bwd_kernel(const T* 
   const float gh = g_ent ? g_ent[row] : 0.f, gl = g_logp && y >= 0 ? (y < V ? g_logp[row] : NAN) : 0.f;
   const float base = fmaf(gh, entropy[row], gl);
   const int yi = y >= 0 && y < V ? (int)y : -1;
+  const bool none = y < 0 && gh == 0.f;                       // no gradient reaches the row: zero also where its p is NaN
   auto grad = [&](float v) {
+    if (none) return 0.f;
     const float lp = (v - st.x) - st.y;
     return -ex2(lp * L2E) * fmaf(gh, fmaxf(lp, LOWEST), base);
   };

@@ -177,7 +177,7 @@ def token_logprobs(logits, tokens, *, top=0):
     logits [..., V] (bf16, fp16 or fp32), tokens int64 [...].  Returns `TokenLogprobs`: logp = log softmax(logits)[token],
     entropy of the row, and with top > 0 (at most 32) the `top` largest log probabilities with their ids, largest first,
     equal ones by ascending id.  All sums in fp32; outputs fp32.  A negative token means the row has no target: logp 0 and no
-    gradient through it; a token >= V gives NaN.  logp and entropy are differentiable in the logits, the alternatives
+    gradient through it, whatever the row holds; a token >= V gives NaN.  logp and entropy are differentiable in the logits, the alternatives
     are not.  -inf logits (masked entries) are fine; a row of nothing else gives NaN."""
     if not isinstance(logits, _T) or not isinstance(tokens, _T):
         raise TypeError("logits and tokens: tensors are wanted")

@@ -142,6 +142,7 @@ def token_logprobs_bwd(x, tokens, stats, entropy, g_logp, g_entropy):
     gl = zero if g_logp is None else torch.where(tokens < 0, zero, torch.where(tokens >= V, float("nan"), g_logp))
     gh = zero if g_entropy is None else g_entropy
     d = -p * (gh[:, None] * lp.clamp_min(-200.0) + (gl + gh * entropy)[:, None])
+    d = d.masked_fill(((tokens < 0) & (gh == 0))[:, None], 0.0)          # no gradient reaches the row: also where its p is NaN
     has = (tokens >= 0) & (tokens < V)
     d.scatter_add_(-1, tokens.clamp(0, V - 1)[:, None], torch.where(has, gl, 0.0)[:, None])
     return d.to(x.dtype)
