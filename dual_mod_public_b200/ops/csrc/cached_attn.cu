@@ -10,6 +10,8 @@
 // bounds.  Rows behind the live length are never read: they are filled with zeros in shared memory, whatever the cache holds
 // there.  The blocks of a cluster join their parts through each other's shared memory, in block order: one launch, no
 // workspace, no atomics.
+#include <climits>
+
 #include "packed.cuh"
 
 namespace {
@@ -287,7 +289,7 @@ extern "C" int dmb_cached_attn(const void* q, long long q_bs, long long q_hs, co
                                void* o, int B, int P, int Hq, int Hkv, int D, int window, int blocks, float scale, int half,
                                void* stream) {
   if (B <= 0) return 0;
-  if (P < 0 || D <= 0 || D > 128 || (D & 7) || Hkv <= 0 || Hq % Hkv || B > 65535) return -1;
+  if (P < 0 || P > INT_MAX - 4095 || D <= 0 || D > 128 || (D & 7) || Hkv <= 0 || Hq % Hkv || B > 65535) return -1;
   if (blocks < 1 || blocks > MAX_CLUSTER || (blocks & (blocks - 1))) return -1;
   const Geo g{q_bs, q_hs, k_bs, k_rs, k_hs, v_bs, v_rs, v_hs, P, Hq, Hq / Hkv, D, window, scale * packed::LOG2E};
   if ((long long)Hkv * ((g.group + ROWS - 1) / ROWS) > 65535) return -1;

@@ -36,6 +36,7 @@ from torch.autograd.function import once_differentiable
 from . import default_ops
 
 MAX_TOP = 32
+MAX_CACHE = (1 << 31) - 4096          # rows: the kernel shares them out in whole tiles, whose ends have to be 32-bit numbers too
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 _T = torch.Tensor
 _SCALES = 2.0 ** -126, 2.0 ** 127     # the kernels hold scale log2(e) in fp32: as zero it would turn a hidden key's -inf into NaN
@@ -139,9 +140,9 @@ def cached_attention(q, k_cache, v_cache, lengths, *, window=0, scale=None):
         raise ValueError("cached_attention has no gradient: call it under torch.no_grad()")
     if getattr(forward_ad, "_current_level", 0) >= 0:
         _check_tangents("cached_attention", q, k_cache, v_cache)
-    if P >= 1 << 31 or B > 65535 or Hkv > 4095 or (Hq > 65535 and Hkv * -(-Hq // (16 * Hkv)) > 65535):
-        raise ValueError("at most 65535 sequences, 4095 key heads, 65535 groups of up to 16 query heads of one key head and 2^31 - 1 "
-                         f"cache rows are wanted, got {B}, {Hkv}, {Hq} query heads and {P}")
+    if P > MAX_CACHE or B > 65535 or Hkv > 4095 or (Hq > 65535 and Hkv * -(-Hq // (16 * Hkv)) > 65535):
+        raise ValueError("at most 65535 sequences, 4095 key heads, 65535 groups of up to 16 query heads of one key head and "
+                         f"{MAX_CACHE} cache rows are wanted, got {B}, {Hkv}, {Hq} query heads and {P}")
     return default_ops(q.device).cached_attn(q, k_cache, v_cache, lengths.contiguous(), window, scale)
 
 
