@@ -14,6 +14,8 @@
 // entry from below; only threads whose own maximum reaches the bound have their entries looked at again, and what reaches
 // the bound, a few entries more than `top`, is ranked by (value, lower index first).
 // A row has no target where its token is negative: logp = 0, no gradient through it.  A token beyond the vocabulary gives NaN.
+#include <climits>
+
 #include "packed.cuh"
 
 namespace {
@@ -598,7 +600,7 @@ int bwd(const void* xv, long long rs, const long long* tok, int rows, int V, con
 extern "C" int dmb_logprob_fwd(const void* x, long long rs, const long long* tokens, long long rows, int V, int type, int top,
                                float* logp, float* entropy, float* stats, float* top_logp, long long* top_ids, void* stream) {
   if (rows <= 0) return 0;
-  if (V <= 0 || rows > 0x7fffffffLL || top < 0 || top > MAX_TOP || top > V) return -1;
+  if (V <= 0 || V > INT_MAX - 4095 || rows > 0x7fffffffLL || top < 0 || top > MAX_TOP || top > V) return -1;
   cudaStream_t s = (cudaStream_t)stream;
   float2* st = (float2*)stats;
   if (type == 0) return fwd<float>(x, rs, tokens, (int)rows, V, top, logp, entropy, st, top_logp, top_ids, s);
@@ -611,7 +613,7 @@ extern "C" int dmb_logprob_bwd(const void* x, long long rs, const long long* tok
                                const float* stats, const float* entropy, const float* g_logp, const float* g_entropy, void* dx,
                                void* stream) {
   if (rows <= 0) return 0;
-  if (V <= 0 || rows > 0x7fffffffLL) return -1;
+  if (V <= 0 || V > INT_MAX - 4095 || rows > 0x7fffffffLL) return -1;
   cudaStream_t s = (cudaStream_t)stream;
   const float2* st = (const float2*)stats;
   if (type == 0) return bwd<float>(x, rs, tokens, (int)rows, V, st, entropy, g_logp, g_entropy, dx, s);

@@ -37,6 +37,7 @@ from . import default_ops
 
 MAX_TOP = 32
 MAX_CACHE = (1 << 31) - 4096          # rows: the kernel shares them out in whole tiles, whose ends have to be 32-bit numbers too
+MAX_VOCAB = (1 << 31) - 4096          # columns: a row's last vector and the 1024 threads behind it are 32-bit numbers too
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 _T = torch.Tensor
 _SCALES = 2.0 ** -126, 2.0 ** 127     # the kernels hold scale log2(e) in fp32: as zero it would turn a hidden key's -inf into NaN
@@ -192,8 +193,8 @@ def token_logprobs(logits, tokens, *, top=0):
     if len(shape) == 0 or shape[:-1] != lead or shape[-1] == 0:
         raise ValueError(f"tokens of the logits' leading shape are wanted, got {tuple(shape)} and {tuple(lead)}")
     V = shape[-1]
-    if V >= 1 << 31 or tokens.numel() >= 1 << 31:
-        raise ValueError("too many rows or columns")
+    if V > MAX_VOCAB or tokens.numel() >= 1 << 31:
+        raise ValueError(f"at most {MAX_VOCAB} columns and 2^31 - 1 rows are wanted, got {V} and {tokens.numel()}")
     if not isinstance(top, int) or not 0 <= top <= min(MAX_TOP, V):
         raise ValueError(f"top: 0 to {min(MAX_TOP, V)} is wanted, got {top!r}")
     if getattr(forward_ad, "_current_level", 0) >= 0:
