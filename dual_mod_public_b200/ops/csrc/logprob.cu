@@ -3,13 +3,14 @@
 //   m = max x,  S = sum exp(x - m),  logp = (x_y - m) - log S,  H = log S - sum p (x - m),  p = exp(x - m) / S
 //   d x = g_logp (1[y] - p) - g_H p (log p + H)
 //
-// Both passes stream the row once with 16-byte loads and are bound by DRAM (8191 x 32000 bf16: forward 100 us, 5.2 TB/s, with the
-// greedy entry 108 us; the exponentials take 60 % of the special-function unit meanwhile; backward 169 us, 6.2 TB/s).  Forward: a
-// group of 32 to 1024 threads per row (see `fwd`), two sets of loads in flight per thread, running maximum and sums per thread
+// Both passes stream the row once with 16-byte loads and are bound by DRAM (8191 x 32000 bf16: forward 95 us, 5.5 TB/s, with the
+// greedy entry 102 us, with eight alternatives 137 us; the exponentials take 60 % of the special-function unit meanwhile;
+// backward 169 us, 6.2 TB/s).  -inf among a thread's entries sends its set of vectors through a scalar loop (every second entry: 307
+// us).  Forward: a group of 32 to 1024 threads per row (see `fwd`), two sets of loads in flight per thread, running maximum and sums per thread
 // (fp32; a thread adds its part of the row, the rest is a tree).  A block takes rows in turn and requests the next row's first
 // part before it joins the sums of the last.  A row whose entries all are the type's lowest value is uniform, as it should be.
 // The rows in flight may not fit L2, so reading an entry again costs a round trip to DRAM under load.  The greedy entry does
-// without: a thread keeps the set of vectors that its maximum came with in shared memory (116 -> 108 us).
+// without: a thread keeps the set of vectors that its maximum came with in shared memory (116 -> 108 us when built).
 // Alternatives: the maxima of 32 parts of the row are entries of it, so the top-th largest of them bounds the top-th largest
 // entry from below; only threads whose own maximum reaches the bound have their entries looked at again, and what reaches
 // the bound, a few entries more than `top`, is ranked by (value, lower index first).

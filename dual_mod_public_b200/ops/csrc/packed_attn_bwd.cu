@@ -21,9 +21,9 @@
 // more columns for dS, so that dP is formed while the exponentials run, and the next S as soon as dP has been read.
 // P and dS are rounded to bf16 (relative 2^-8 at most); everything else is fp32.
 //
-// Measured (8192 rows, one sequence): 16 heads of 64 534 us, 16 query and 4 key heads of 128 722 us, 644 and 951 TFLOP/s counted
-// as five products over the visible pairs; eleven documents in 8192 rows, 16 heads of 64: 141 us.  Bound at D = 128 by the tensor
-// pipe (66 % busy over both kinds) and its latencies, at D = 64 by the exponentials and the instructions around them: products
+// Measured (8192 rows, one sequence): 16 heads of 64 534 us, 16 query and 4 key heads of 128 745 us, 644 and 923 TFLOP/s counted
+// as five products over the visible pairs; eleven documents in 8192 rows, 16 heads of 64: 145 us.  Bound at D = 128 by the tensor
+// pipe (65 % busy over both kinds) and its latencies, at D = 64 by the exponentials and the instructions around them: products
 // with 64 columns take as long as ones with 128.
 //
 // A first small kernel forms delta from o and the rest that its rounding left: where a row sees few keys ds is a small difference
@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(256) packed_delta_kernel(const bf16* __restric
                                                            long long g_hs, const float* __restrict__ lse, float* __restrict__ aux,
                                                            const int* __restrict__ cu, int nseq, int T, int Tp, int Hq, int D) {
   // one head, ROWS rows: LANES threads (8 dims each) take a row, MORE rows whose loads are in flight together, and the rows of
-  // a warp's groups follow one another, so the row vectors are read and written in whole sectors: 11.1 us at 8192 rows of 16
+  // a warp's groups follow one another, so the row vectors are read and written in whole sectors: 12.3 us at 8192 rows of 16
   // heads of 64 with a cold cache (50 MB), 19.7 with the heads of a row in a warp
   constexpr int GROUPS = 256 / LANES, ROWS = GROUPS * MORE;
   const int h = blockIdx.x % Hq, row0 = blockIdx.x / Hq * ROWS + threadIdx.x / LANES;

@@ -17,9 +17,10 @@
 // read, and they keep the two tiles half a block apart: one tile's exponentials run while the tensor pipe works for the other.
 //
 // Measured: 8192 rows of one sequence, 16 heads of 64: 190 us (722 TFLOP/s over the visible pairs); 16384 rows, 16 heads of 128:
-// 875 us (1257 TFLOP/s, 76 % of the library product's measured rate); eleven documents in 8192 rows, where half of the
-// blocks hold a border: 53 us.  What bounds: 128 x 128 exponentials take 1024 cycles of the special-function unit, as long as
-// the products at D = 128 and twice as long at D = 64.  So of every eight pairs EMU are computed by a polynomial on the FMA pipe
+// 895 us (1228 TFLOP/s, 75 % of the library product's measured rate); eleven documents in 8192 rows, where half of the
+// blocks hold a border: 53 us.  128 x 128 exponentials take 1024 cycles of the special-function unit, as long as the products at
+// D = 128 and twice as long at D = 64 (where no unit is full: special-function unit 54 %, issue slots 51 %, tensor pipe 35 %; a
+// tile's next scores wait until the softmax has read the last).  So of every eight pairs EMU are computed by a polynomial on the FMA pipe
 // (packed.cuh), in blocks without masked entries.  The running maximum is allowed to lag by up to 8 octaves (P <= 256, exact in
 // the fp32 accumulator's range and no loss of relative precision in 16 bits): O is rescaled in tensor memory only when a row's
 // maximum outgrows that, which after the first blocks is rare.  Sums are fp32; P is rounded to the operand type.

@@ -8,7 +8,8 @@
 
 On a B200 these run the kernels of csrc/packed_attn_fwd.cu, packed_attn_bwd.cu, cached_attn.cu and logprob.cu, on the
 tensors' own device and its current stream; on CPU the torch statements of `packed_math.py`.  No call reads a value back to
-the host, so each can be captured into a CUDA graph, and none keeps state between calls.  Results are bitwise repeatable.
+the host, so each can be captured into a CUDA graph, and none keeps state between calls.  (A captured backward pass wants what torch
+asks of any: a first run on a side stream, and no eager graph of the same leaves alive.)  Results are bitwise repeatable.
 
 Kernel arguments: bf16 or fp16 (attention; gradients: bf16), bf16, fp16 or fp32 (scores); head dims that are multiples of 8
 up to 128.  Attention of other types or head dims runs the torch statement and is counted in `default_ops(device).fallbacks`
