@@ -30,6 +30,7 @@ Reference parity: lm/eval/lm_eval_adapter.py:69-781 (`DualModEval`: likelihood :
 
 from __future__ import annotations
 
+import copy
 import hashlib
 import json
 import os
@@ -331,7 +332,9 @@ class DualModEval(_Base):
         """The decoder for `rows` prompts in caches of P entries.  One is resident at a time: another shape takes over the
         weights (a copy in the compute type, where the model has another one) once the caches and the graph of the last are gone."""
         from .packed_decode import PackedDecoder
-        dec = self._engines.pop("packed", None)
+        dec, cfg = self._engines.pop("packed", (None, None))
+        if cfg != self.model.cfg:                                # none yet, or one of longer or shorter tables, another window
+            dec = None
         if dec is None or (dec.rows, dec.P) != (rows, P):
             weights = self.model if dec is None else dec.m
             dec = None
@@ -339,7 +342,7 @@ class DualModEval(_Base):
             if torch.device(self.dev).type == "cuda":
                 dec.capture()
         dec.refresh(self.model)                                  # it may have been trained on
-        self._engines["packed"] = dec
+        self._engines["packed"] = dec, copy.copy(self.model.cfg)
         return dec
 
     def _greedy_packed(self, prompts, max_new, stop_strs):

@@ -7,8 +7,9 @@ The prompts are packed one behind the other and run through the layers in ONE pa
 values are written to the rows' caches, and every further token is a step over the whole batch in which each row has a
 position and a live length of its own (`ops.cached_attention`); the next token and its log probability come from
 `ops.token_logprobs`.  Grouped KV heads, sliding windows and the log-n scale work as in training.  `capture()` records the
-step as one CUDA graph.  Weights of another type than `dtype` are copied once; `refresh(model)` copies them again.  (`eval.graph_decode.GraphDecoder` is the decoder for batches that share one position, and for the
-Dual-Mod write law.)"""
+step as one CUDA graph.  Weights of another type than `dtype` are copied once; `refresh(model)` copies them again.
+Where they are not copied, the model's tensors have to stay where they are, and its configuration as it is, while the decoder
+lives.  (`eval.graph_decode.GraphDecoder` is the decoder for batches that share one position, and for the Dual-Mod write law.)"""
 
 from __future__ import annotations
 
