@@ -110,7 +110,8 @@ def packed_attention(q, k, v, cu_seqlens, *, window=0, scale=None):
 
     An output row depends on the rows that it sees and on no other, whatever those hold: an infinite or NaN entry of v makes
     the rows that see it infinite or NaN, and so does a NaN score or one of +inf.  A score of -inf has weight zero; a row whose
-    scores all are -inf is zero, like a row without keys.  Finite scores may have any size.
+    scores all are -inf is zero, like a row without keys.  Finite scores may have any size; rows whose
+    largest is beyond 1.2e7, and rows that share a block with a non-finite v that they do not see, are computed one by one, slowly.
     The gradients want finite inputs: their products run over blocks of 128 rows, and a weight of zero times an infinite or NaN
     entry is NaN, so such a row reaches the gradients of others in its block.  They form the weights from the logarithm of the
     row's sum in fp32: beyond 2^24 log 2 = 1.2e7 the gradients of the row and of the keys that it sees are NaN."""
